@@ -114,8 +114,10 @@ enum tria_status {
     TRIA_ERR_UNSUPPORTED = -5,  /* geometry or cache type not supported */
     TRIA_ERR_NO_DEVICE   = -6,  /* no CUDA device / not an sm_100 device */
     TRIA_ERR_TIMEOUT     = -7,  /* a bounded wait inside a kernel gave up; that step's output is undefined */
-    TRIA_ERR_BOUNDS      = -8   /* checked build only: an index or extent was out of range; the access was
+    TRIA_ERR_BOUNDS      = -8,  /* checked build only: an index or extent was out of range; the access was
                                    skipped and that step's output is undefined */
+    TRIA_ERR_ROWS        = -9   /* tria_attend / tria_append / tria_accept: a row count on the device does not fit
+                                   its cache, or an accepted path is not ascending; see those functions */
 };
 
 /* Cache element types (ggml type ids). */
@@ -409,6 +411,119 @@ TRIA_API int tria_select_key(const float *scores, int64_t score_stride, const in
 TRIA_API int tria_key_gather(const float *scores, int64_t score_stride, const int32_t *n_rows,
                              int32_t units, uint32_t key_min, float *out, int32_t cap, int32_t *count,
                              void *stream);
+
+/* ---- Serving from an evicted cache ----
+ * New; the reference leaves attention and the cache's writes to its runtime.
+ * After an eviction every (layer, kv-head) unit of a view has its own rows,
+ * positions and row count.  These calls write, read and evict such a cache:
+ *   tria_append      new tokens' K and V behind each unit's rows
+ *   tria_attend      attention of the query tokens over each unit's rows
+ *   tria_evict_mass  eviction of the rows that attention weighted least
+ *   tria_accept      the accepted path of a tree of drafted tokens
+ * They share these conventions:
+ *   - Row counts are device data, [n_layer*n_head_kv] int32 (tria_evict's
+ *     n_kept_out), so a captured graph may be replayed as the counts change;
+ *     tria_evict_mass alone takes them from the host, as tria_evict does.
+ *   - A view lists caches of equal shape: the layers of one model, or one
+ *     layer of several sequences.  layer0 and head0 are not looked at (no
+ *     stats are read) except by tria_evict_mass, whose budget is per layer.
+ *   - Keys are stored as attention reads them: the view needs
+ *     TRIA_VIEW_POST_ROPE.  Rows are f16 or q8_0, head_dim 64 or 128.
+ *   - Row order matters: a call's n_tok tokens are the last n_tok rows of each
+ *     unit, token t at row n - n_tok + t, as tria_append leaves them.
+ *   - A bad row count or path is found by the kernel: that unit is skipped
+ *     (tria_attend clamps the count) and TRIA_ERR_ROWS reported by the next
+ *     tria_ctx_check or tria_get_n_kv.
+ *   - A call may be captured in a CUDA graph after one eager call with the
+ *     same sizes; workspaces that graphs hold are kept until the context is
+ *     destroyed. */
+
+/* One call's attention.  With q the query of (token t, head h) and k, v row j
+ * of kv head h / gqa:
+ *     s = scale * (q . k)
+ *     s = softcap * tanh(s / softcap)                   if softcap > 0
+ *     s = s - slopes[h] * (tok_pos[t] - pos[j])         if slopes
+ *     out = sum_j softmax_j(s) * v_j                    over the rows j that t sees.
+ * Token t sees the rows before the last n_tok, and of those n_tok the ones up
+ * to its own (tree == NULL), or those whose bit is set in its row of `tree`
+ * (bit j % 32 of word j / 32; its own bit too if it sees itself).  With
+ * window > 0 it sees of all these only rows with pos >= tok_pos[t] - window or
+ * pos < sink.  A token that sees no row gets out = 0 and lse = -inf.  Rows it
+ * does not see may hold anything, infinities and NaN included. */
+struct tria_attend_params {
+    int32_t n_tok;             /* query tokens per cache, >= 0 */
+    int32_t window;            /* 0: no window */
+    int32_t sink;
+    int32_t tree_words;        /* words per row of tree, at least (n_tok + 31) / 32 */
+    float   scale;
+    float   softcap;           /* 0: none */
+    float   mass_decay;        /* factor of mass_in */
+    int32_t reserved;          /* 0 */
+    const float    *slopes;    /* device [n_head_kv*gqa], or NULL */
+    const int32_t  *tok_pos;   /* device [n_tok] (one per cache with a stride); needed for window or slopes */
+    const uint32_t *tree;      /* device [n_tok][tree_words], or NULL: causal */
+    int64_t tok_pos_stride;    /* elements from one cache to the next, 0: shared by all */
+    int64_t tree_stride;       /* words from one cache to the next, 0: shared by all */
+    int64_t q_cache_stride, q_tok_stride, q_head_stride;   /* elements; multiples of 8 */
+    int64_t o_cache_stride, o_tok_stride, o_head_stride;
+};
+
+/* q, out: device f16 [n_layer][n_tok][n_head_kv*gqa][head_dim] by the strides
+ * of `p`, 16-byte aligned; they must not overlap.  lse: device fp32 [n_layer]
+ * [n_tok][n_head_kv*gqa], the natural log of the softmax's denominator, or
+ * NULL.  mass_out: device fp32 [n_layer][n_head_kv][n_cells], or NULL; row j
+ * of a unit gets mass_decay * mass_in[j] + the sum of its weights over the
+ * tokens and the query heads of its group (mass_in NULL: 0; it may be
+ * mass_out), rows at and behind the unit's count are left as they were.
+ * Scores, softmax statistics and masses are held in fp32. */
+TRIA_API int tria_attend(tria_ctx *ctx, const struct tria_kv_view *kv, const int32_t *n_rows,
+                         const struct tria_attend_params *p, const void *q, void *out, float *lse,
+                         const float *mass_in, float *mass_out, void *stream);
+
+/* Source types of tria_append (ggml type ids). */
+#define TRIA_SRC_F32 0
+#define TRIA_SRC_F16 1
+
+/* Writes n_tok tokens' keys and values behind each unit's rows (row n of the
+ * unit first), rounded to f16 or quantised to q8_0 (d = max|x| / 127, q =
+ * round-half-even(x * (1 / d)), in fp32), their positions, and 0 as their mass
+ * (mass may be NULL); n_rows_out = n_rows + n_tok (it may be n_rows).  k, v:
+ * device [n_layer][n_tok][n_head_kv][head_dim] of src_type; the strides are
+ * elements, each a multiple of 16 bytes, the same for k and v.  tok_pos:
+ * device int32 [n_tok], one per cache with a stride.  A unit whose cells do
+ * not hold n_tok more rows is left as it was, its count too.  With shared
+ * positions (pos_shared) every unit of the view must have the same count. */
+struct tria_append_params {
+    int32_t n_tok;
+    int32_t src_type;
+    int64_t cache_stride, tok_stride, head_stride;
+    const int32_t *tok_pos;
+    int64_t tok_pos_stride;    /* 0: shared by all */
+};
+TRIA_API int tria_append(tria_ctx *ctx, const struct tria_kv_view *kv, const int32_t *n_rows,
+                         const struct tria_append_params *p, const void *k, const void *v, float *mass,
+                         int32_t *n_rows_out, void *stream);
+
+/* Keeps of each unit's last n_tok rows the drafted tokens path[0..n_path), in
+ * order, and drops the rest: row n - n_tok + path[i] moves to row n - n_tok + i
+ * (K, V, position, and mass unless NULL), in place; n_rows_out = n - n_tok +
+ * n_path (it may be n_rows).  path: device int32, strictly ascending indices
+ * in [0, n_tok), one list for all caches (path_stride 0, n_path [1]) or one
+ * per cache (path_stride elements apart, n_path [n_layer]).  A unit whose path
+ * or count does not fit is left as it was. */
+TRIA_API int tria_accept(tria_ctx *ctx, const struct tria_kv_view *kv, const int32_t *n_rows, int32_t n_tok,
+                         const int32_t *path, int64_t path_stride, const int32_t *n_path, float *mass,
+                         int32_t *n_rows_out, void *stream);
+
+/* One eviction step ranked by mass instead of by the frequency series: the
+ * counts, protected rows and ties of tria_evict, with mass [n_layer]
+ * [n_head_kv][n_cells of src] as the scores; the kept rows' masses move to
+ * mass_dst [n_layer][n_head_kv][n_cells of dst] (NULL: dropped).  n_rows is a
+ * host array.  tria_get_n_kv returns the counts as after tria_evict.  Key
+ * positions are not checked against cur_pos. */
+TRIA_API int tria_evict_mass(tria_ctx *ctx, const struct tria_kv_view *src, const struct tria_kv_view *dst,
+                             const int32_t *n_rows, const float *mass, float *mass_dst,
+                             const struct tria_evict_params *params, int32_t *n_kept_out, void *stream);
 
 #ifdef __cplusplus
 }

@@ -21,52 +21,17 @@
 #include <new>
 #include <vector>
 
-#include "tria_internal.h"
+#include "tria_ctx.cuh"
 #include "tria_kernels.cuh"
 
 using namespace tria;
-
-/* The step's completion event.  Inside a stream capture a plain record only
- * orders work within the capture; recorded as an external event node it is
- * recorded again at every replay of the graph, so tria_get_n_kv waits for the
- * replayed step. */
-static cudaError_t record_done(cudaEvent_t ev, cudaStream_t st) {
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    cudaError_t e = cudaStreamIsCapturing(st, &cs);
-    if (e != cudaSuccess) return e;
-    return cs == cudaStreamCaptureStatusActive ? cudaEventRecordWithFlags(ev, st, cudaEventRecordExternal)
-                                               : cudaEventRecord(ev, st);
-}
-
-/* NVTX ranges on the host timeline (a profiler shows them beside the
- * kernels; ncu --nvtx filters launches by them): a call, and the stages of an
- * eviction step.  With no tool attached a push or pop is a branch. */
-struct NvtxRange {
-    explicit NvtxRange(const char *name) { nvtxRangePushA(name); }
-    ~NvtxRange() { nvtxRangePop(); }
-    NvtxRange(const NvtxRange &) = delete;
-    NvtxRange &operator=(const NvtxRange &) = delete;
-};
-struct NvtxStages {
-    bool open = false;
-    void next(const char *name) {
-        close();
-        nvtxRangePushA(name);
-        open = true;
-    }
-    void close() {
-        if (open) nvtxRangePop();
-        open = false;
-    }
-    ~NvtxStages() { close(); }
-};
 
 /* Raises a kernel's dynamic shared-memory limit on the current device to at
  * least `bytes`.  The attribute belongs to each device's copy of the kernel
  * (a process may drive several GPUs, as llama.cpp does when it splits layers),
  * so it is tracked per (kernel, device) and set only when a launch needs more
  * than before. */
-static cudaError_t raise_smem_limit(const void *fn, int bytes) {
+cudaError_t raise_smem_limit(const void *fn, int bytes) {
     static std::mutex mu;
     static std::map<std::pair<const void *, int>, int> set_to;
     int dev = 0;
@@ -106,23 +71,10 @@ extern "C" TRIA_API const char *tria_status_str(int st) {
         case TRIA_ERR_NO_DEVICE: return "no sm_100 CUDA device";
         case TRIA_ERR_TIMEOUT: return "a bounded wait inside a kernel gave up";
         case TRIA_ERR_BOUNDS: return "a bounds check of the checked build failed";
+        case TRIA_ERR_ROWS: return "a row count or an accepted path on the device does not fit its cache";
         default: return "unknown status";
     }
 }
-
-#define FAIL(code, ...) do { tria_set_error(__VA_ARGS__); return (code); } while (0)
-#define CUDA_TRY(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) \
-    FAIL(e_ == cudaErrorMemoryAllocation ? TRIA_ERR_NOMEM : TRIA_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); } while (0)
-
-/* Restores the caller's current device on scope exit. */
-struct DeviceGuard {
-    int prev = -1;
-    explicit DeviceGuard(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) cudaSetDevice(dev);
-    }
-    ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
-};
 
 /* The status word the kernels set (ST_* bits) as a tria_status, with the
  * message of the first bit found.  A pipeline timeout is reported before a
@@ -139,65 +91,15 @@ static int status_of_bits(int32_t bits, const char *what) {
     if (bits & ST_BOUNDS)
         FAIL(TRIA_ERR_BOUNDS, "%s: a bounds check of the checked build failed (status 0x%x): an index or "
              "extent from the device or the call was out of range and that access was skipped", what, bits);
+    if (bits & ST_ROWS)
+        FAIL(TRIA_ERR_ROWS, "%s: a row count outside [0, n_cells], too few free cells, or an accepted path that is "
+             "not ascending within the drafted tokens (status 0x%x); those units were left as they were", what, bits);
     FAIL(TRIA_ERR_CUDA, "%s: unknown kernel status bits 0x%x", what, bits);
 }
 
 /* ------------------------------------------------------------------ */
 /* Context                                                              */
 /* ------------------------------------------------------------------ */
-
-struct tria_ctx {
-    int device = 0;
-    uint32_t L = 0, H = 0, KV = 0, hd = 0, fc = 0, G = 0;
-    std::vector<float> scales;           /* layer budget scales (host) */
-    float attn_scale = 1.0f;             /* rope attention scaling of the stats (post-RoPE keys) */
-    /* position table for post-RoPE views: rows p in [0, ptab_cur] of trigger ptab_cur */
-    float2 *d_ptab = nullptr;
-    int64_t ptab_cap = 0, ptab_cur = -1;
-    int64_t ptab_t_lo = 0, ptab_t_len = 0;
-    float *d_q = nullptr;                /* [L][H][3][fc] */
-    float *d_omega = nullptr;            /* [fc] */
-    /* delta table: entries for d in [t_lo, t_lo + t_len), capacity t_cap rows */
-    float2 *d_table = nullptr;
-    int64_t t_lo = 0, t_len = 0, t_cap = 0;
-    /* scratch */
-    uint8_t *d_scratch = nullptr;
-    size_t scratch_cap = 0;
-    float *raw = nullptr;
-    float2 *ms = nullptr;
-    uint32_t *keys = nullptr;
-    int32_t *kept = nullptr;
-    int32_t *cnt = nullptr;
-    int64_t raw_stride = 0, cell_stride = 0;
-    int sm_count = 148;
-    /* host-API staging */
-    uint8_t *d_io = nullptr;
-    size_t io_cap = 0;
-    cudaStream_t own_stream = nullptr;
-    /* status / counts read-back */
-    int32_t *d_status = nullptr;         /* ST_* bits the kernels set; cleared when read back */
-    long long wait_limit = WAIT_LIMIT_DEFAULT;   /* bound of the scoring kernel's pipeline waits */
-    int select_split = 0;                        /* CTAs per unit in selection: 0 automatic, 1 one block */
-    int32_t *h_pinned = nullptr;         /* [0] = status, [1..] counts */
-    int32_t pinned_cap = 0;
-    int32_t last_units = 0;
-    cudaEvent_t ev_done = nullptr;
-    bool have_step = false;
-    /* stage timing (tria_ctx_set_timing) */
-    bool timing = false, have_timing = false;
-    cudaEvent_t ev_stage[6] = {};
-    int64_t launches = 0;
-    std::mutex mu;
-    /* tria_evict_host: double-buffered device staging of K (and positions) */
-    cudaStream_t copy_stream = nullptr;
-    uint8_t *hs_k[2] = {nullptr, nullptr};
-    int32_t *hs_pos[2] = {nullptr, nullptr};
-    size_t hs_k_cap = 0, hs_pos_cap = 0;
-    cudaEvent_t hs_copied[2] = {nullptr, nullptr}, hs_freed[2] = {nullptr, nullptr};
-    bool hs_used[2] = {false, false};
-    int32_t *d_cnt_all = nullptr;
-    int64_t cnt_all_cap = 0;
-};
 
 static int check_device(int device) {
     int n = 0;
@@ -237,6 +139,11 @@ extern "C" TRIA_API void tria_ctx_destroy(tria_ctx *ctx) {
             if (ctx->hs_freed[b]) cudaEventDestroy(ctx->hs_freed[b]);
         }
         cudaFree(ctx->d_cnt_all);
+        if (ctx->d_attend) {
+            cudaDeviceSynchronize();      /* no event follows the serving calls */
+            cudaFree(ctx->d_attend);
+        }
+        for (void *p : ctx->outgrown) cudaFree(p);
     }
     delete ctx;
 }
@@ -331,10 +238,21 @@ static int ensure_table(tria_ctx *c, int64_t lo, int64_t hi, cudaStream_t st) {
     return TRIA_OK;
 }
 
-static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+int note_capture(tria_ctx *c, cudaStream_t st) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    CUDA_TRY(cudaStreamIsCapturing(st, &cs));
+    if (cs == cudaStreamCaptureStatusNone) return 0;
+    c->captured = true;
+    return 1;
+}
+
+void drop_scratch(tria_ctx *c, void *p) {
+    if (c->captured) c->outgrown.push_back(p);
+    else cudaFree(p);
+}
 
 /* Scratch for `units` units of up to `cells` rows. */
-static int ensure_scratch(tria_ctx *c, int64_t units, int64_t cells, cudaStream_t st) {
+int ensure_scratch(tria_ctx *c, int64_t units, int64_t cells, cudaStream_t st) {
     const int64_t stride = (cells + 63) & ~(int64_t)63;
     const size_t raw_b = align256((size_t)units * c->G * stride * 4);
     const size_t ms_b = align256((size_t)units * c->G * sizeof(float2));
@@ -342,9 +260,13 @@ static int ensure_scratch(tria_ctx *c, int64_t units, int64_t cells, cudaStream_
     const size_t kept_b = align256((size_t)units * stride * 4);
     const size_t cnt_b = align256((size_t)units * 4);
     const size_t need = raw_b + ms_b + key_b + kept_b + cnt_b;
+    const int cap = note_capture(c, st);
+    if (cap < 0) return cap;
     if (need > c->scratch_cap) {
+        if (cap) FAIL(TRIA_ERR_INVALID, "the scratch has to grow to %zu bytes inside a stream capture: make one eager "
+                      "call with these sizes first", need);
         cudaDeviceSynchronize();      /* earlier calls may still use it, on any stream */
-        if (c->d_scratch) cudaFree(c->d_scratch);
+        if (c->d_scratch) drop_scratch(c, c->d_scratch);
         c->d_scratch = nullptr;
         c->scratch_cap = 0;
         CUDA_TRY(cudaMalloc(&c->d_scratch, need));
@@ -372,13 +294,13 @@ static int ensure_scratch(tria_ctx *c, int64_t units, int64_t cells, cudaStream_
 /* View validation                                                      */
 /* ------------------------------------------------------------------ */
 
-static int64_t view_row_bytes(int type, int hd) {
+int64_t view_row_bytes(int type, int hd) {
     if (type == TRIA_TYPE_F16) return 2LL * hd;
     if (type == TRIA_TYPE_Q8_0) return (int64_t)hd / 32 * 34;
     return -1;
 }
 
-static int validate_view(const tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, const char *what,
+int validate_view(const tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, const char *what,
                          bool need_v) {
     if (!v) FAIL(TRIA_ERR_INVALID, "%s: null view", what);
     if (v->type != TRIA_TYPE_F16 && v->type != TRIA_TYPE_Q8_0)
@@ -699,7 +621,7 @@ static int run_scoring(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows
     return rc ? rc : run_znorm(c, v, n_rows, st);
 }
 
-static void keep_requests(const tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
+void keep_requests(const tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
                           const tria_evict_params *p, std::vector<int32_t> &keep) {
     keep.resize((size_t)v->n_layer * v->n_head_kv);
     for (int l = 0; l < v->n_layer; l++) {
@@ -767,7 +689,7 @@ static int select_split(const tria_ctx *c, int units, int n_max, bool fused) {
     return 1;
 }
 
-static int launch_select(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, const std::vector<int32_t> &keep,
+int launch_select(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, const std::vector<int32_t> &keep,
                          const tria_evict_params *p, bool fused, const float *scores, int32_t *kept_idx,
                          int64_t kept_stride, int32_t *n_kept, cudaStream_t st) {
     return for_layer_chunks(v, [&](int l0, int nl) -> int {
@@ -841,9 +763,9 @@ static int launch_select(tria_ctx *c, const tria_kv_view *v, const int32_t *n_ro
 
 /* rows_hint: expected kept rows per unit, only sizes the grid (the kernel is
  * grid-stride, so any count on the device is copied whatever the hint). */
-static int launch_compact(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d, const int32_t *n_rows,
+int launch_compact(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d, const int32_t *n_rows,
                           const int32_t *kept_idx, int64_t kept_stride, const int32_t *n_kept, cudaStream_t st,
-                          int rows_hint = -1) {
+                          int rows_hint) {
     const int64_t rb = view_row_bytes(s->type, (int)c->hd);
     auto al = [](int64_t x) { return x & 15 ? (x & 7 ? 4 : 8) : 16; };
     int vec = std::min({al(rb), al(s->cell_stride), al(s->head_stride), al(d->cell_stride), al(d->head_stride)});
@@ -1000,7 +922,7 @@ extern "C" TRIA_API int tria_select(tria_ctx *c, const tria_kv_view *v, const in
     return launch_select(c, v, n_rows, keep, p, false, scores, kept_idx, v->n_cells, n_kept, st);
 }
 
-static int check_pair(const tria_kv_view *s, const tria_kv_view *d) {
+int check_pair(const tria_kv_view *s, const tria_kv_view *d) {
     if (d->type != s->type || d->n_layer != s->n_layer || d->n_head_kv != s->n_head_kv ||
         d->layer0 != s->layer0 || d->head0 != s->head0)
         FAIL(TRIA_ERR_INVALID, "src/dst views differ in type or geometry");

@@ -1,0 +1,399 @@
+/*
+ * tria_serve.cu - host side of the calls that write, read and evict a ragged
+ * cache by attention: tria_append, tria_attend, tria_accept, tria_evict_mass.
+ */
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "tria_attend.cuh"
+#include "tria_cache.cuh"
+#include "tria_ctx.cuh"
+
+using namespace tria;
+
+/* A view whose rows attention reads or the serving calls write: any number of
+ * caches (no stats are read), post-RoPE keys, K and V. */
+static int validate_cache(const tria_kv_view *v, const char *what) {
+    if (!v) FAIL(TRIA_ERR_INVALID, "%s: null view", what);
+    if (v->type != TRIA_TYPE_F16 && v->type != TRIA_TYPE_Q8_0)
+        FAIL(TRIA_ERR_UNSUPPORTED, "%s: cache type %d unsupported", what, v->type);
+    if (v->n_layer < 1 || v->n_head_kv < 1 || v->n_head_kv > TRIA_MAX_UNITS)
+        FAIL(TRIA_ERR_INVALID, "%s: %d caches of %d kv heads", what, v->n_layer, v->n_head_kv);
+    if ((int64_t)v->n_layer * v->n_head_kv > INT32_MAX)
+        FAIL(TRIA_ERR_INVALID, "%s: more than 2^31 units", what);
+    if (v->n_cells < 0) FAIL(TRIA_ERR_INVALID, "%s: negative n_cells", what);
+    if (v->flags & ~TRIA_VIEW_POST_ROPE) FAIL(TRIA_ERR_INVALID, "%s: unknown view flags 0x%x", what, v->flags);
+    if (!(v->flags & TRIA_VIEW_POST_ROPE))
+        FAIL(TRIA_ERR_UNSUPPORTED, "%s: the cache must hold keys as attention reads them (TRIA_VIEW_POST_ROPE)", what);
+    if (!v->k || !v->v || !v->pos) FAIL(TRIA_ERR_INVALID, "%s: null k, v or pos", what);
+    if ((v->cell_stride & 3) || (v->head_stride & 3) || v->cell_stride <= 0 || v->head_stride < 0)
+        FAIL(TRIA_ERR_INVALID, "%s: strides must be positive multiples of 4", what);
+    if ((uintptr_t)v->pos & 3) FAIL(TRIA_ERR_INVALID, "%s: pos misaligned", what);
+    for (int l = 0; l < v->n_layer; l++)
+        if (!v->k[l] || ((uintptr_t)v->k[l] & 15) || !v->v[l] || ((uintptr_t)v->v[l] & 15))
+            FAIL(TRIA_ERR_INVALID, "%s: k[%d] or v[%d] null or not 16-byte aligned", what, l, l);
+    return TRIA_OK;
+}
+
+/* The context's part of the checks, after all that needs none. */
+static int check_ctx(const tria_ctx *c, const char *what) {
+    if (!c) FAIL(TRIA_ERR_INVALID, "%s: null context", what);
+    if (c->hd != 64 && c->hd != 128)
+        FAIL(TRIA_ERR_UNSUPPORTED, "%s: head_dim %u unsupported (64 or 128)", what, c->hd);
+    return TRIA_OK;
+}
+
+static int check_ints(const char *what, const char *name, const void *p) {
+    if (!p || ((uintptr_t)p & 3)) FAIL(TRIA_ERR_INVALID, "%s: %s null or misaligned", what, name);
+    return TRIA_OK;
+}
+
+/* Whether the counts are updated in place; arrays that overlap in part are refused. */
+static int counts_alias(const char *what, const int32_t *in, const int32_t *out, int64_t units, bool *alias) {
+    const uintptr_t r0 = (uintptr_t)in, r1 = (uintptr_t)out, len = (uintptr_t)units * 4;
+    *alias = r0 < r1 + len && r1 < r0 + len;
+    if (*alias && in != out) FAIL(TRIA_ERR_INVALID, "%s: n_rows and n_rows_out overlap in part", what);
+    return TRIA_OK;
+}
+
+/* Launches of at most TRIA_MAX_LAYERS caches and TRIA_MAX_UNITS units. */
+template <class F>
+static int for_cache_chunks(const tria_kv_view *v, F &&fn) {
+    const int per = std::max(1, std::min(TRIA_MAX_LAYERS, TRIA_MAX_UNITS / v->n_head_kv));
+    for (int l0 = 0; l0 < v->n_layer; l0 += per) {
+        const int rc = fn(l0, std::min(per, v->n_layer - l0));
+        if (rc) return rc;
+    }
+    return TRIA_OK;
+}
+
+/* ------------------------------------------------------------------ */
+/* Append                                                               */
+/* ------------------------------------------------------------------ */
+
+template <int KT, int HD>
+static void launch_append(const AppendArgs &a, bool f32, dim3 grid, cudaStream_t st) {
+    if (f32) k_append<KT, HD, true><<<grid, APPEND_THREADS, 0, st>>>(a);
+    else k_append<KT, HD, false><<<grid, APPEND_THREADS, 0, st>>>(a);
+}
+
+extern "C" TRIA_API int tria_append(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
+                                    const tria_append_params *p, const void *k, const void *vv, float *mass,
+                                    int32_t *n_rows_out, void *stream) {
+    NvtxRange range("tria_append");
+    const char *fn = "tria_append";
+    if (!p) FAIL(TRIA_ERR_INVALID, "%s: null parameters", fn);
+    int rc = validate_cache(v, fn);
+    if (!rc) rc = check_ints(fn, "n_rows", n_rows);
+    if (!rc) rc = check_ints(fn, "n_rows_out", n_rows_out);
+    if (rc) return rc;
+    if (p->n_tok < 0) FAIL(TRIA_ERR_INVALID, "%s: n_tok %d < 0", fn, p->n_tok);
+    if (p->src_type != TRIA_SRC_F16 && p->src_type != TRIA_SRC_F32)
+        FAIL(TRIA_ERR_UNSUPPORTED, "%s: source type %d unsupported", fn, p->src_type);
+    if (p->tok_pos_stride < 0) FAIL(TRIA_ERR_INVALID, "%s: negative tok_pos_stride", fn);
+    if (v->pos_shared && p->tok_pos_stride) FAIL(TRIA_ERR_INVALID, "%s: shared positions take one tok_pos for all caches", fn);
+    const bool f32 = p->src_type == TRIA_SRC_F32;
+    const int esz = f32 ? 4 : 2, unit16 = 16 / esz;
+    if (p->n_tok > 0) {
+        if ((rc = check_ints(fn, "tok_pos", p->tok_pos))) return rc;
+        if (!k || !vv || ((uintptr_t)k & 15) || ((uintptr_t)vv & 15))
+            FAIL(TRIA_ERR_INVALID, "%s: k or v null or not 16-byte aligned", fn);
+        if (p->cache_stride % unit16 || p->tok_stride % unit16 || p->head_stride % unit16)
+            FAIL(TRIA_ERR_INVALID, "%s: source strides must be multiples of 16 bytes", fn);
+        if (mass && ((uintptr_t)mass & 3)) FAIL(TRIA_ERR_INVALID, "%s: mass misaligned", fn);
+    }
+    /* a unit's count may be overwritten only once all its blocks have read it */
+    const int units_all = v->n_layer * v->n_head_kv;
+    bool alias = false;
+    if ((rc = counts_alias(fn, n_rows, n_rows_out, units_all, &alias))) return rc;
+    if ((rc = check_ctx(c, fn))) return rc;
+    DeviceGuard g(c->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    if ((rc = note_capture(c, st)) < 0) return rc;
+    /* enough blocks per unit to fill the GPU; one when the rows are few */
+    const int rows_per_block = APPEND_THREADS / 32 * (256 / (int)c->hd);
+    const int want = std::max(1, 4 * c->sm_count / std::max(1, std::min(units_all, TRIA_MAX_UNITS)));
+    const int bx = std::max(1, std::min((p->n_tok + rows_per_block - 1) / rows_per_block, want));
+    const bool later = alias && bx > 1;
+    rc = for_cache_chunks(v, [&](int l0, int nl) -> int {
+        AppendArgs a;
+        memset(&a, 0, sizeof a);
+        const int64_t u0 = (int64_t)l0 * v->n_head_kv;
+        for (int l = 0; l < nl; l++) { a.k[l] = (uint8_t *)v->k[l0 + l]; a.v[l] = (uint8_t *)v->v[l0 + l]; }
+        a.cell_stride = v->cell_stride;
+        a.head_stride = v->head_stride;
+        a.pos = v->pos_shared ? v->pos : v->pos + u0 * v->n_cells;
+        a.pos_shared = v->pos_shared ? 1 : 0;
+        a.n_cells = v->n_cells;
+        a.n_head_kv = v->n_head_kv;
+        a.n_tok = p->n_tok;
+        a.first = l0 == 0;
+        a.n_rows = n_rows + u0;
+        a.n_rows_out = later ? nullptr : n_rows_out + u0;
+        a.src_cache = p->cache_stride * esz;
+        a.src_tok = p->tok_stride * esz;
+        a.src_head = p->head_stride * esz;
+        a.src_k = (const uint8_t *)k + l0 * a.src_cache;
+        a.src_v = (const uint8_t *)vv + l0 * a.src_cache;
+        a.tok_pos = p->tok_pos + l0 * p->tok_pos_stride;
+        a.tok_pos_stride = p->tok_pos_stride;
+        a.mass = mass ? mass + u0 * v->n_cells : nullptr;
+        a.status = c->d_status;
+        const dim3 grid((unsigned)bx, (unsigned)(nl * v->n_head_kv));
+        if (v->type == TRIA_TYPE_F16) {
+            if (c->hd == 128) launch_append<KT_F16, 128>(a, f32, grid, st);
+            else launch_append<KT_F16, 64>(a, f32, grid, st);
+        } else {
+            if (c->hd == 128) launch_append<KT_Q8_0, 128>(a, f32, grid, st);
+            else launch_append<KT_Q8_0, 64>(a, f32, grid, st);
+        }
+        CUDA_TRY(cudaGetLastError());
+        c->launches++;
+        return TRIA_OK;
+    });
+    if (rc) return rc;
+    if (later) {
+        k_append_counts<<<(units_all + 255) / 256, 256, 0, st>>>(n_rows, n_rows_out, units_all, p->n_tok, v->n_cells);
+        CUDA_TRY(cudaGetLastError());
+        c->launches++;
+    }
+    return TRIA_OK;
+}
+
+/* ------------------------------------------------------------------ */
+/* Accept                                                               */
+/* ------------------------------------------------------------------ */
+
+extern "C" TRIA_API int tria_accept(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, int32_t n_tok,
+                                    const int32_t *path, int64_t path_stride, const int32_t *n_path, float *mass,
+                                    int32_t *n_rows_out, void *stream) {
+    NvtxRange range("tria_accept");
+    const char *fn = "tria_accept";
+    int rc = validate_cache(v, fn);
+    if (!rc) rc = check_ints(fn, "n_rows", n_rows);
+    if (!rc) rc = check_ints(fn, "n_rows_out", n_rows_out);
+    if (!rc) rc = check_ints(fn, "path", path);
+    if (!rc) rc = check_ints(fn, "n_path", n_path);
+    if (rc) return rc;
+    if (n_tok < 0 || path_stride < 0) FAIL(TRIA_ERR_INVALID, "%s: negative n_tok or path_stride", fn);
+    if (v->pos_shared && path_stride) FAIL(TRIA_ERR_INVALID, "%s: shared positions take one path for all caches", fn);
+    if (mass && ((uintptr_t)mass & 3)) FAIL(TRIA_ERR_INVALID, "%s: mass misaligned", fn);
+    bool alias = false;
+    if ((rc = counts_alias(fn, n_rows, n_rows_out, (int64_t)v->n_layer * v->n_head_kv, &alias))) return rc;
+    if ((rc = check_ctx(c, fn))) return rc;
+    DeviceGuard g(c->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    if ((rc = note_capture(c, st)) < 0) return rc;
+    return for_cache_chunks(v, [&](int l0, int nl) -> int {
+        AcceptArgs a;
+        memset(&a, 0, sizeof a);
+        const int64_t u0 = (int64_t)l0 * v->n_head_kv;
+        for (int l = 0; l < nl; l++) { a.k[l] = (uint8_t *)v->k[l0 + l]; a.v[l] = (uint8_t *)v->v[l0 + l]; }
+        a.cell_stride = v->cell_stride;
+        a.head_stride = v->head_stride;
+        a.pos = v->pos_shared ? v->pos : v->pos + u0 * v->n_cells;
+        a.pos_shared = v->pos_shared ? 1 : 0;
+        a.n_cells = v->n_cells;
+        a.n_head_kv = v->n_head_kv;
+        a.row_words = (int32_t)(view_row_bytes(v->type, (int)c->hd) / 4);
+        a.n_tok = n_tok;
+        a.first = l0 == 0;
+        a.n_rows = n_rows + u0;
+        a.n_rows_out = n_rows_out + u0;
+        a.path = path + l0 * path_stride;
+        a.n_path = n_path + (path_stride ? l0 : 0);
+        a.path_stride = path_stride;
+        a.mass = mass ? mass + u0 * v->n_cells : nullptr;
+        a.status = c->d_status;
+        k_accept<<<nl * v->n_head_kv, ACCEPT_THREADS, 0, st>>>(a);
+        CUDA_TRY(cudaGetLastError());
+        c->launches++;
+        return TRIA_OK;
+    });
+}
+
+/* ------------------------------------------------------------------ */
+/* Eviction by mass                                                     */
+/* ------------------------------------------------------------------ */
+
+extern "C" TRIA_API int tria_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d,
+                                        const int32_t *n_rows, const float *mass, float *mass_dst,
+                                        const tria_evict_params *p, int32_t *n_kept_out, void *stream) {
+    NvtxRange range("tria_evict_mass");
+    const char *fn = "tria_evict_mass";
+    if (!n_rows || !p || !mass) FAIL(TRIA_ERR_INVALID, "%s: null argument", fn);
+    if (p->cur_pos < 0) FAIL(TRIA_ERR_INVALID, "%s: cur_pos %d < 0", fn, p->cur_pos);
+    if (((uintptr_t)mass & 3) || ((uintptr_t)mass_dst & 3)) FAIL(TRIA_ERR_INVALID, "%s: mass misaligned", fn);
+    if (mass == mass_dst) FAIL(TRIA_ERR_INVALID, "%s: mass and mass_dst must be different arrays", fn);
+    if (!c) FAIL(TRIA_ERR_INVALID, "%s: null context", fn);
+    int rc = validate_view(c, s, n_rows, "tria_evict_mass src", false);
+    if (!rc) rc = validate_view(c, d, nullptr, "tria_evict_mass dst", false);
+    if (!rc) rc = check_pair(s, d);
+    if (rc) return rc;
+    const int KV = s->n_head_kv;
+    const int64_t units = (int64_t)s->n_layer * KV;
+    int max_rows = 0;
+    for (int64_t u = 0; u < units; u++) {
+        if (n_rows[u] > d->n_cells)   /* the kept count is only known on the device */
+            FAIL(TRIA_ERR_INVALID, "dst n_cells %d < n_rows[%lld] = %d", d->n_cells, (long long)u, n_rows[u]);
+        max_rows = std::max(max_rows, n_rows[u]);
+    }
+    DeviceGuard g(c->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    if ((rc = ensure_scratch(c, units, s->n_cells, st))) return rc;
+    std::vector<int32_t> keep;
+    keep_requests(c, s, n_rows, p, keep);
+    int32_t *cnt = n_kept_out ? n_kept_out : c->cnt;
+    if ((rc = launch_select(c, s, n_rows, keep, p, false, mass, c->kept, c->cell_stride, cnt, st))) return rc;
+    int64_t hint = 0;
+    for (int32_t k : keep) hint = std::max<int64_t>(hint, k);
+    if (p->window > 0 || p->sink > 0) hint += (int64_t)std::max(0, p->window) + std::max(0, p->sink) + 1;
+    hint = std::min<int64_t>(hint, max_rows);
+    if ((rc = launch_compact(c, s, d, n_rows, c->kept, c->cell_stride, cnt, st, (int)hint))) return rc;
+    if (mass_dst && max_rows > 0) {
+        for (int64_t u0 = 0; u0 < units; u0 += TRIA_MAX_UNITS) {
+            const int nu = (int)std::min<int64_t>(TRIA_MAX_UNITS, units - u0);
+            const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((hint + 1023) / 1024, 64)), (unsigned)nu);
+            k_carry_mass<<<grid, 256, 0, st>>>(mass + u0 * s->n_cells, s->n_cells, mass_dst + u0 * d->n_cells, d->n_cells,
+                                               c->kept + u0 * c->cell_stride, c->cell_stride, cnt + u0);
+            CUDA_TRY(cudaGetLastError());
+            c->launches++;
+        }
+    }
+    c->have_timing = false;
+    CUDA_TRY(cudaMemcpyAsync(c->h_pinned, c->d_status, 4, cudaMemcpyDeviceToHost, st));
+    CUDA_TRY(cudaMemcpyAsync(c->h_pinned + 1, cnt, (size_t)units * 4, cudaMemcpyDeviceToHost, st));
+    CUDA_TRY(record_done(c->ev_done, st));
+    c->last_units = (int32_t)units;
+    c->have_step = true;
+    return TRIA_OK;
+}
+
+/* ------------------------------------------------------------------ */
+/* Attention                                                            */
+/* ------------------------------------------------------------------ */
+
+/* Grows tria_attend's workspace to `need` bytes. */
+static int ensure_attend(tria_ctx *c, size_t need, cudaStream_t st) {
+    const int cap = note_capture(c, st);
+    if (cap < 0) return cap;
+    if (need <= c->attend_cap) return TRIA_OK;
+    if (cap) FAIL(TRIA_ERR_INVALID, "tria_attend: the workspace has to grow to %zu bytes inside a stream capture: make "
+                  "one eager call with these sizes first", need);
+    need += need / 4;
+    CUDA_TRY(cudaDeviceSynchronize());        /* earlier calls may still use it, on any stream */
+    if (c->d_attend) drop_scratch(c, c->d_attend);
+    c->d_attend = nullptr;
+    c->attend_cap = 0;
+    CUDA_TRY(cudaMalloc(&c->d_attend, need));
+    c->attend_cap = need;
+    CUDA_TRY(cudaMemset(c->d_attend, 0, need));
+    CUDA_TRY(cudaDeviceSynchronize());
+    return TRIA_OK;
+}
+
+template <int KT, int HD>
+static int run_attend(tria_ctx *c, const AttendArgs &a, cudaStream_t st) {
+    const int units = a.n_layer * a.n_head_kv;
+    if (a.T > 0) {
+        k_attend_rows<KT, HD><<<(unsigned)(units * a.G * a.T), ROW_THREADS, 0, st>>>(a);
+        CUDA_TRY(cudaGetLastError());
+        c->launches++;
+    }
+    if (a.mass_out) {
+        k_mass_rows<KT, HD><<<dim3((unsigned)std::max(1, std::min((a.n_cells + 127) / 128, 1024)), (unsigned)units), 128, 0, st>>>(a);
+        CUDA_TRY(cudaGetLastError());
+        c->launches++;
+    }
+    return TRIA_OK;
+}
+
+extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
+                                    const tria_attend_params *p, const void *q, void *out, float *lse,
+                                    const float *mass_in, float *mass_out, void *stream) {
+    NvtxRange range("tria_attend");
+    const char *fn = "tria_attend";
+    if (!p) FAIL(TRIA_ERR_INVALID, "%s: null parameters", fn);
+    int rc = validate_cache(v, fn);
+    if (!rc) rc = check_ints(fn, "n_rows", n_rows);
+    if (rc) return rc;
+    const int T = p->n_tok, KV = v->n_head_kv;
+    if (T < 0 || p->window < 0 || p->sink < 0) FAIL(TRIA_ERR_INVALID, "%s: negative n_tok, window or sink", fn);
+    if (p->reserved) FAIL(TRIA_ERR_INVALID, "%s: reserved must be 0", fn);
+    if (!std::isfinite(p->scale) || !std::isfinite(p->mass_decay) || !std::isfinite(p->softcap) || p->softcap < 0.0f)
+        FAIL(TRIA_ERR_INVALID, "%s: scale %g, softcap %g or mass_decay %g not finite, or softcap < 0", fn,
+             (double)p->scale, (double)p->softcap, (double)p->mass_decay);
+    if (mass_in && !mass_out) FAIL(TRIA_ERR_INVALID, "%s: mass_in without mass_out", fn);
+    if (((uintptr_t)mass_in & 3) || ((uintptr_t)mass_out & 3) || ((uintptr_t)lse & 3))
+        FAIL(TRIA_ERR_INVALID, "%s: lse or mass misaligned", fn);
+    if (T > 0) {
+        if (!q || !out || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))
+            FAIL(TRIA_ERR_INVALID, "%s: q or out null or not 16-byte aligned", fn);
+        const int64_t s[6] = {p->q_cache_stride, p->q_tok_stride, p->q_head_stride,
+                              p->o_cache_stride, p->o_tok_stride, p->o_head_stride};
+        for (int64_t x : s)
+            if (x < 0 || x % 8) FAIL(TRIA_ERR_INVALID, "%s: q and out strides must be multiples of 8 elements, not negative", fn);
+        if (p->slopes && ((uintptr_t)p->slopes & 3)) FAIL(TRIA_ERR_INVALID, "%s: slopes misaligned", fn);
+        if (p->window > 0 || p->slopes) {
+            if ((rc = check_ints(fn, "tok_pos", p->tok_pos))) return rc;
+            if (p->tok_pos_stride < 0) FAIL(TRIA_ERR_INVALID, "%s: negative tok_pos_stride", fn);
+        }
+        if (p->tree) {
+            if ((uintptr_t)p->tree & 3) FAIL(TRIA_ERR_INVALID, "%s: tree misaligned", fn);
+            if (p->tree_words < (T + 31) / 32 || p->tree_stride < 0)
+                FAIL(TRIA_ERR_INVALID, "%s: tree_words %d < %d, or a negative tree_stride", fn, p->tree_words, (T + 31) / 32);
+        }
+    }
+    if ((rc = check_ctx(c, fn))) return rc;
+    const int H = KV * (int)c->G;
+    if ((int64_t)v->n_layer * H * T > INT32_MAX / 2)
+        FAIL(TRIA_ERR_UNSUPPORTED, "%s: %lld query rows in one call", fn, (long long)v->n_layer * H * T);
+    if (T == 0 && !mass_out) return TRIA_OK;
+    DeviceGuard g(c->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    const size_t lse_b = mass_out && !lse ? align256((size_t)v->n_layer * H * std::max(T, 1) * 4) : 0;
+    if ((rc = ensure_attend(c, lse_b, st))) return rc;
+    return for_cache_chunks(v, [&](int l0, int nl) -> int {
+        AttendArgs a;
+        memset(&a, 0, sizeof a);
+        const int64_t u0 = (int64_t)l0 * KV;
+        for (int l = 0; l < nl; l++) { a.k[l] = (const uint8_t *)v->k[l0 + l]; a.v[l] = (const uint8_t *)v->v[l0 + l]; }
+        a.cell_stride = v->cell_stride;
+        a.head_stride = v->head_stride;
+        a.pos = v->pos_shared ? v->pos : v->pos + u0 * v->n_cells;
+        a.pos_shared = v->pos_shared ? 1 : 0;
+        a.n_cells = v->n_cells;
+        a.n_layer = nl;
+        a.n_head_kv = KV;
+        a.G = (int32_t)c->G;
+        a.T = T;
+        a.n_rows = n_rows + u0;
+        a.q = (const __half *)q + l0 * p->q_cache_stride;
+        a.out = (__half *)out + l0 * p->o_cache_stride;
+        a.q_cache = p->q_cache_stride; a.q_tok = p->q_tok_stride; a.q_head = p->q_head_stride;
+        a.o_cache = p->o_cache_stride; a.o_tok = p->o_tok_stride; a.o_head = p->o_head_stride;
+        float *ls = lse ? lse : lse_b ? (float *)c->d_attend : nullptr;
+        a.lse = ls ? ls + (int64_t)l0 * T * H : nullptr;
+        a.mass_in = mass_in ? mass_in + u0 * v->n_cells : nullptr;
+        a.mass_out = mass_out ? mass_out + u0 * v->n_cells : nullptr;
+        a.mass_decay = p->mass_decay;
+        a.scale = p->scale;
+        a.softcap = p->softcap;
+        a.window = p->window;
+        a.sink = p->sink;
+        a.slopes = p->slopes;
+        a.tok_pos = p->window > 0 || p->slopes ? p->tok_pos + l0 * p->tok_pos_stride : nullptr;
+        a.tok_pos_stride = p->tok_pos_stride;
+        a.tree = p->tree ? p->tree + l0 * p->tree_stride : nullptr;
+        a.tree_stride = p->tree_stride;
+        a.tree_words = p->tree_words;
+        a.status = c->d_status;
+        if (v->type == TRIA_TYPE_F16)
+            return c->hd == 128 ? run_attend<KT_F16, 128>(c, a, st) : run_attend<KT_F16, 64>(c, a, st);
+        return c->hd == 128 ? run_attend<KT_Q8_0, 128>(c, a, st) : run_attend<KT_Q8_0, 64>(c, a, st);
+    });
+}

@@ -43,6 +43,7 @@ ERR_UNSUPPORTED = -5
 ERR_NO_DEVICE = -6
 ERR_TIMEOUT = -7
 ERR_BOUNDS = -8
+ERR_ROWS = -9
 
 
 class TriaError(RuntimeError):
@@ -127,6 +128,64 @@ class EvictParams(C.Structure):
     """struct tria_evict_params."""
     _fields_ = [("cur_pos", C.c_int32), ("budget", C.c_int32), ("ramp_pct", C.c_int32),
                 ("window", C.c_int32), ("sink", C.c_int32), ("reserved", C.c_int32)]
+
+
+class AttendParams(C.Structure):
+    """struct tria_attend_params; attend_params() fills one from tensors."""
+    _fields_ = [("n_tok", C.c_int32), ("window", C.c_int32), ("sink", C.c_int32), ("tree_words", C.c_int32),
+                ("scale", C.c_float), ("softcap", C.c_float), ("mass_decay", C.c_float), ("reserved", C.c_int32),
+                ("slopes", C.c_void_p), ("tok_pos", C.c_void_p), ("tree", C.c_void_p),
+                ("tok_pos_stride", C.c_int64), ("tree_stride", C.c_int64),
+                ("q_cache_stride", C.c_int64), ("q_tok_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("o_cache_stride", C.c_int64), ("o_tok_stride", C.c_int64), ("o_head_stride", C.c_int64)]
+
+
+class AppendParams(C.Structure):
+    """struct tria_append_params."""
+    _fields_ = [("n_tok", C.c_int32), ("src_type", C.c_int32), ("cache_stride", C.c_int64), ("tok_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("tok_pos", C.c_void_p), ("tok_pos_stride", C.c_int64)]
+
+
+SRC_F32 = 0
+SRC_F16 = 1
+
+
+def attend_params(scale, softcap=0.0, window=0, sink=0, slopes=None, tok_pos=None, tree=None, mass_decay=1.0):
+    """Options of Context.attend that stay the same from call to call (the
+    token count and the strides come from the call's q and out).  Device
+    tensors: slopes fp32 [heads]; tok_pos int32 [n_tok], or [caches][n_tok]
+    for positions of each cache's own; tree int32 [n_tok][words] or
+    [caches][n_tok][words], bit j % 32 of word j / 32 of row t set when token t
+    sees token j."""
+    p = AttendParams()
+    p.scale, p.softcap, p.window, p.sink, p.mass_decay = scale, softcap, int(window), int(sink), mass_decay
+    p.slopes = _ptr(_ints_or_floats(slopes, "slopes", 1, "float32"))
+    p.tok_pos = _ptr(_ints_or_floats(tok_pos, "tok_pos", 2, "int32"))
+    p.tree = _ptr(_ints_or_floats(tree, "tree", 3, "int32"))
+    if tok_pos is not None and tok_pos.dim() == 2:
+        p.tok_pos_stride = tok_pos.stride(0)
+    if tree is not None:
+        p.tree_words = tree.shape[-1]
+        if tree.dim() == 3:
+            p.tree_stride = tree.stride(0)
+    p._keep = (slopes, tok_pos, tree)
+    return p
+
+
+def _ints_or_floats(x, name, most_dims, dtype):
+    if x is None:
+        return None
+    if str(x.dtype) != "torch." + dtype or not 1 <= x.dim() <= most_dims or (x.shape[-1] > 1 and x.stride(-1) != 1):
+        raise ValueError(f"{name}: a {dtype} tensor of at most {most_dims} dimensions with a contiguous last one is wanted")
+    if x.dim() >= 2 and name == "tree" and x.shape[-2] > 1 and x.stride(-2) != x.shape[-1]:
+        raise ValueError("tree: rows must follow one another")
+    return x
+
+
+def _tensor(x, name, dtypes, dims):
+    if str(x.dtype).replace("torch.", "") not in dtypes or x.dim() != dims:
+        raise ValueError(f"{name}: a tensor of {' or '.join(dtypes)} with {dims} dimensions is wanted, got {x.dtype} {tuple(x.shape)}")
+    return x
 
 
 class Policy(C.Structure):
@@ -220,6 +279,12 @@ def lib() -> C.CDLL:
                                      C.c_void_p]
         L.tria_select_key.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_uint32, C.c_void_p,
                                       C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
+        L.tria_attend.argtypes = [C.c_void_p, C.POINTER(KvView), C.c_void_p, C.POINTER(AttendParams)] + [C.c_void_p] * 6
+        L.tria_append.argtypes = [C.c_void_p, C.POINTER(KvView), C.c_void_p, C.POINTER(AppendParams)] + [C.c_void_p] * 5
+        L.tria_accept.argtypes = [C.c_void_p, C.POINTER(KvView), C.c_void_p, C.c_int32, C.c_void_p, C.c_int64] + \
+            [C.c_void_p] * 4
+        L.tria_evict_mass.argtypes = [C.c_void_p, C.POINTER(KvView), C.POINTER(KvView), C.c_void_p, C.c_void_p, C.c_void_p,
+                                      C.POINTER(EvictParams), C.c_void_p, C.c_void_p]
         L.tria_score_kv_head_dev.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                              C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
         _lib = L
@@ -380,6 +445,8 @@ class Context:
         check(lib().tria_ctx_create(stats, device, C.byref(h)))
         self.h = h
         self.stats = stats
+        s = stats.contents
+        self.head_dim, self.gqa, self.device = int(s.head_dim), int(s.num_heads // s.num_kv_heads), int(device)
 
     def close(self):
         if self.h:
@@ -465,3 +532,111 @@ class Context:
     def score_kv_head_dev(self, k_re, k_im, key_pos, cur_pos, n, layer, kv_head, out, stream=None):
         check(lib().tria_score_kv_head_dev(self.h, _ptr(k_re), _ptr(k_im), _ptr(key_pos), int(cur_pos),
                                            int(n), int(layer), int(kv_head), _ptr(out), _stream(stream)))
+
+    # ---- serving from an evicted cache ----
+
+    def append(self, view, n_rows, k, v, tok_pos, n_rows_out=None, mass=None, stream=None):
+        """tria_append: device tensors k, v [caches][n_tok][kv heads][head_dim]
+        (f16 or fp32, contiguous last dimension) behind each unit's n_rows (device
+        int32); n_rows_out defaults to n_rows, updated in place."""
+        for x, name in ((k, "k"), (v, "v")):
+            _tensor(x, name, ("float16", "float32"), 4)
+            if x.stride(3) != 1 and x.shape[3] > 1 or x.shape != k.shape or x.dtype != k.dtype or x.stride() != k.stride():
+                raise ValueError("k and v must have the same shape, type and strides, the last dimension contiguous")
+        if tuple(k.shape) != (view.n_layer, k.shape[1], view.n_head_kv, self.head_dim):
+            raise ValueError(f"k of shape {tuple(k.shape)} for {view.n_layer} caches of {view.n_head_kv} heads of {self.head_dim}")
+        self._shared_or_own(tok_pos, "tok_pos", (k.shape[1],), view.n_layer)
+        _ints_or_floats(tok_pos, "tok_pos", 2, "int32")
+        self._mass(mass, view)
+        self._here(k, v, tok_pos, mass)
+        self._counts(view, n_rows, *(() if n_rows_out is None else (n_rows_out,)))
+        p = AppendParams()
+        p.n_tok, p.src_type = k.shape[1], SRC_F32 if str(k.dtype) == "torch.float32" else SRC_F16
+        p.cache_stride, p.tok_stride, p.head_stride = k.stride(0), k.stride(1), k.stride(2)
+        p.tok_pos, p.tok_pos_stride = _ptr(tok_pos), tok_pos.stride(0) if tok_pos.dim() == 2 else 0
+        check(lib().tria_append(self.h, C.byref(view), _ptr(n_rows), C.byref(p), _ptr(k), _ptr(v), _ptr(mass),
+                                _ptr(n_rows if n_rows_out is None else n_rows_out), _stream(stream)))
+
+    def attend(self, view, n_rows, q, out, params, lse=None, mass_in=None, mass_out=None, stream=None):
+        """tria_attend: device f16 tensors q, out [caches][n_tok][heads][head_dim]
+        (any strides that are multiples of 8, the last dimension contiguous)."""
+        for x, name in ((q, "q"), (out, "out")):
+            _tensor(x, name, ("float16",), 4)
+            if x.stride(3) != 1 or x.shape != q.shape:
+                raise ValueError("q and out must have the same shape and a contiguous last dimension")
+        if q.shape[0] != view.n_layer or q.shape[2] != view.n_head_kv * self.gqa or q.shape[3] != self.head_dim:
+            raise ValueError(f"q of shape {tuple(q.shape)} for {view.n_layer} caches of {view.n_head_kv} x {self.gqa} heads "
+                             f"of {self.head_dim}")
+        T = q.shape[1]
+        slopes, tok_pos, tree = getattr(params, "_keep", (None, None, None))
+        if slopes is not None and slopes.shape[0] != q.shape[2]:
+            raise ValueError(f"{slopes.shape[0]} slopes for {q.shape[2]} heads")
+        self._shared_or_own(tok_pos, "tok_pos", (T,), view.n_layer)
+        self._shared_or_own(tree, "tree", (T, params.tree_words), view.n_layer)
+        if lse is not None:
+            _tensor(lse, "lse", ("float32",), 3)
+            if tuple(lse.shape) != (view.n_layer, T, q.shape[2]) or not lse.is_contiguous():
+                raise ValueError("lse must be a contiguous [caches][n_tok][heads]")
+        for m in (mass_in, mass_out):
+            self._mass(m, view)
+        self._here(q, out, lse, mass_in, mass_out, slopes, tok_pos, tree)
+        self._counts(view, n_rows)
+        params.n_tok = T
+        params.q_cache_stride, params.q_tok_stride, params.q_head_stride = q.stride(0), q.stride(1), q.stride(2)
+        params.o_cache_stride, params.o_tok_stride, params.o_head_stride = out.stride(0), out.stride(1), out.stride(2)
+        check(lib().tria_attend(self.h, C.byref(view), _ptr(n_rows), C.byref(params), _ptr(q), _ptr(out), _ptr(lse),
+                                _ptr(mass_in), _ptr(mass_out), _stream(stream)))
+
+    def accept(self, view, n_rows, n_tok, path, n_path, n_rows_out=None, mass=None, stream=None):
+        """tria_accept: device int32 path [caches or 1][entries] and n_path [caches or 1]."""
+        _tensor(path, "path", ("int32",), 2)
+        own = path.shape[0] > 1 or view.n_layer == 1
+        if path.shape[0] not in (1, view.n_layer) or n_path.numel() != path.shape[0] or path.stride(1) != 1 and path.shape[1] > 1:
+            raise ValueError("path must be [caches or 1][entries], n_path [caches or 1]")
+        if path.shape[1] < n_tok:
+            raise ValueError(f"path holds {path.shape[1]} entries a cache: room for n_tok = {n_tok} is wanted")
+        self._mass(mass, view)
+        self._here(path, n_path, mass)
+        self._counts(view, n_rows, *(() if n_rows_out is None else (n_rows_out,)))
+        if str(n_path.dtype) != "torch.int32" or not n_path.is_contiguous():
+            raise ValueError("n_path must be a contiguous int32 tensor")
+        check(lib().tria_accept(self.h, C.byref(view), _ptr(n_rows), int(n_tok), _ptr(path),
+                                path.stride(0) if own and view.n_layer > 1 else 0, _ptr(n_path), _ptr(mass),
+                                _ptr(n_rows if n_rows_out is None else n_rows_out), _stream(stream)))
+
+    def evict_mass(self, src, dst, n_rows, mass, mass_dst, params, n_kept_out=None, stream=None):
+        """tria_evict_mass: one eviction step ranked by device `mass`
+        [layers][kv heads][n_cells]; n_rows is a host array."""
+        a, p = self._rows(n_rows)
+        self._mass(mass, src)
+        self._mass(mass_dst, dst)
+        self._here(mass, mass_dst)
+        if a.shape[0] != src.n_layer * src.n_head_kv:
+            raise ValueError(f"{a.shape[0]} row counts for {src.n_layer} x {src.n_head_kv} units")
+        if n_kept_out is not None:
+            self._counts(src, n_kept_out)
+        check(lib().tria_evict_mass(self.h, C.byref(src), C.byref(dst), p, _ptr(mass), _ptr(mass_dst), C.byref(params),
+                                    _ptr(n_kept_out), _stream(stream)))
+
+    def _here(self, *tensors):
+        """Tensors that kernels read or write must live on the context's device."""
+        for x in tensors:
+            if x is not None and (not x.is_cuda or x.get_device() != self.device):
+                raise ValueError(f"a tensor on {x.device} was given to a context of cuda:{self.device}")
+
+    def _counts(self, view, *counts):
+        for x in counts:
+            if str(x.dtype) != "torch.int32" or not x.is_contiguous() or x.numel() != view.n_layer * view.n_head_kv:
+                raise ValueError(f"row counts must be a contiguous int32 tensor of {view.n_layer} x {view.n_head_kv}")
+        self._here(*counts)
+
+    @staticmethod
+    def _shared_or_own(x, name, shape, caches):
+        if x is not None and tuple(x.shape) not in (shape, (caches,) + shape):
+            raise ValueError(f"{name} of shape {tuple(x.shape)}: {shape} or {(caches,) + shape} is wanted")
+
+    @staticmethod
+    def _mass(x, view):
+        if x is not None and (str(x.dtype) != "torch.float32" or not x.is_contiguous()
+                              or tuple(x.shape) != (view.n_layer, view.n_head_kv, view.n_cells)):
+            raise ValueError(f"mass must be a contiguous fp32 [{view.n_layer}][{view.n_head_kv}][{view.n_cells}] tensor")
