@@ -485,7 +485,7 @@ TRIA_API int tria_attend(tria_ctx *ctx, const struct tria_kv_view *kv, const int
 #define TRIA_SRC_F16 1
 
 /* Writes n_tok tokens' keys and values behind each unit's rows (row n of the
- * unit first), rounded to f16 or quantised to q8_0 (d = max|x| / 127, q =
+ * unit first), rounded to f16 or quantised to q8_0 (d = max|x| * (1/127), q =
  * round-half-even(x * (1 / d)), in fp32), their positions, and 0 as their mass
  * (mass may be NULL); n_rows_out = n_rows + n_tok (it may be n_rows).  k, v:
  * device [n_layer][n_tok][n_head_kv][head_dim] of src_type; the strides are

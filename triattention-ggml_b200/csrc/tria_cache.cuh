@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_append(const AppendArgs a) {
                     for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[kv][i]));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                    const float d = __fdiv_rn(m, 127.0f);
+                    const float d = __fmul_rn(m, 1.0f / 127.0f);
                     const float inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
                     uint8_t *blk = &s_row[w][sub][(c >> 2) * 34];
                     if ((c & 3) == 0) *reinterpret_cast<__half *>(blk) = __float2half_rn(d);

@@ -296,16 +296,97 @@ static int ensure_attend(tria_ctx *c, size_t need, cudaStream_t st) {
     return TRIA_OK;
 }
 
+/* Launch plan of one chunk of caches. */
+struct AttendPlan {
+    int mt = 1;                 /* 16-row tiles of query rows per group */
+    int groups = 0, items = 0, grid = 0;
+    bool plan_kernel = false, keep_scores = false;
+    size_t steps = 0, span = 0, done = 0, arrived = 0, part_o = 0, part_ml = 0, norm = 0, scores = 0, lse = 0, bytes = 0;
+    int64_t score_stride = 0;
+};
+
+/* Most blocks of an attention kernel (the workspace's counters). */
+constexpr int ATTEND_MAX_GRID = 1024;
+
+/* Most bytes of scores that a call with masses keeps instead of scoring twice. */
+constexpr size_t SCORES_MAX = (size_t)1 << 30;
+
+static int plan_attend(const tria_ctx *c, const tria_kv_view *v, int nl, int T, bool window, bool mass, AttendPlan &pl) {
+    const int64_t units = (int64_t)nl * v->n_head_kv, R = (int64_t)T * c->G;
+    pl = AttendPlan{};
+    pl.mt = R <= 16 ? 1 : 2;
+    const int rows = 16 * pl.mt;
+    const int64_t groups = (R + rows - 1) / rows, items = units * groups;
+    if (items * ((v->n_cells + ATT_STEP - 1) / ATT_STEP + 1) > INT32_MAX)
+        FAIL(TRIA_ERR_UNSUPPORTED, "tria_attend: %lld query rows over %d cells in one call", (long long)(units * R), v->n_cells);
+    pl.groups = (int)groups;
+    pl.items = (int)items;
+    pl.grid = std::min(2 * c->sm_count, ATTEND_MAX_GRID);
+    pl.plan_kernel = window || items > 512;
+    pl.score_stride = ((int64_t)v->n_cells + ATT_STEP - 1) / ATT_STEP * ATT_STEP;
+    const size_t sb = (size_t)(units * R * pl.score_stride) * 4;
+    pl.keep_scores = mass && R <= 16 && sb <= SCORES_MAX;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at += align256(bytes); return o; };
+    /* the counters come first and keep their place: they are zero between calls, whatever a call lays out behind them */
+    pl.done = take(4);
+    pl.arrived = take(ATTEND_MAX_GRID * 4);
+    if (pl.plan_kernel) {
+        pl.steps = take((size_t)items * 4);
+        if (window) pl.span = take((size_t)items * 8);
+    }
+    pl.part_o = take((size_t)2 * pl.grid * rows * c->hd * 4);
+    pl.part_ml = take((size_t)2 * pl.grid * rows * 8);
+    if (mass) pl.norm = take((size_t)(units * R) * 8);
+    if (pl.keep_scores) pl.scores = take(sb);
+    pl.bytes = at;
+    return TRIA_OK;
+}
+
+template <int KT, int HD, int MT>
+static int launch_few(tria_ctx *c, const AttendArgs &a, const AttendPlan &pl, cudaStream_t st) {
+    auto fn = k_attend_few<KT, HD, MT>;
+    constexpr int smem = few_smem<KT, HD, MT>();
+    CUDA_TRY(raise_smem_limit((const void *)fn, smem));
+    fn<<<pl.grid, FEW_THREADS, smem, st>>>(a);
+    CUDA_TRY(cudaGetLastError());
+    c->launches++;
+    return TRIA_OK;
+}
+
 template <int KT, int HD>
-static int run_attend(tria_ctx *c, const AttendArgs &a, cudaStream_t st) {
+static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStream_t st) {
     const int units = a.n_layer * a.n_head_kv;
+    uint8_t *ws = c->d_attend;
+    a.groups = pl.groups;
+    a.arrived = (int32_t *)(ws + pl.arrived);
+    a.part_o = (float *)(ws + pl.part_o);
+    a.part_ml = (float2 *)(ws + pl.part_ml);
+    a.norm = a.mass_out ? (float2 *)(ws + pl.norm) : nullptr;
+    a.scores = pl.keep_scores ? (float *)(ws + pl.scores) : nullptr;
+    a.score_stride = pl.score_stride;
     if (a.T > 0) {
-        k_attend_rows<KT, HD><<<(unsigned)(units * a.G * a.T), ROW_THREADS, 0, st>>>(a);
-        CUDA_TRY(cudaGetLastError());
-        c->launches++;
+        if (pl.plan_kernel) {
+            int32_t *steps = (int32_t *)(ws + pl.steps);
+            int2 *span = a.window > 0 ? (int2 *)(ws + pl.span) : nullptr;
+            k_attend_plan<<<span ? pl.items : 1, PLAN_THREADS, 0, st>>>(a, 16 * pl.mt, pl.items, span, steps,
+                                                                       (int32_t *)(ws + pl.done));
+            CUDA_TRY(cudaGetLastError());
+            c->launches++;
+            a.steps = steps;
+            a.span = span;
+        }
+        const int rc = pl.mt == 1 ? launch_few<KT, HD, 1>(c, a, pl, st) : launch_few<KT, HD, 2>(c, a, pl, st);
+        if (rc) return rc;
     }
     if (a.mass_out) {
-        k_mass_rows<KT, HD><<<dim3((unsigned)std::max(1, std::min((a.n_cells + 127) / 128, 1024)), (unsigned)units), 128, 0, st>>>(a);
+        if (pl.keep_scores && a.T > 0) {
+            const int gx = std::max(1, std::min((a.n_cells + 255) / 256, 8 * c->sm_count / std::min(units, 8 * c->sm_count)));
+            k_mass_scores<<<dim3((unsigned)gx, (unsigned)units), 256, 0, st>>>(a);
+        } else {
+            const int gx = std::max(1, std::min((a.n_cells + MASS_KEYS - 1) / MASS_KEYS, 65535));
+            k_mass_tiles<KT, HD><<<dim3((unsigned)gx, (unsigned)units), MASS_THREADS, 0, st>>>(a);
+        }
         CUDA_TRY(cudaGetLastError());
         c->launches++;
     }
@@ -355,9 +436,22 @@ extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const in
     if (T == 0 && !mass_out) return TRIA_OK;
     DeviceGuard g(c->device);
     cudaStream_t st = (cudaStream_t)stream;
-    const size_t lse_b = mass_out && !lse ? align256((size_t)v->n_layer * H * std::max(T, 1) * 4) : 0;
-    if ((rc = ensure_attend(c, lse_b, st))) return rc;
+    bool copy16 = true;                       /* rows on 16-byte (q8_0: 8-byte) boundaries */
+    const int align = v->type == TRIA_TYPE_F16 ? 15 : 7;
+    copy16 = !(v->cell_stride & align) && !(v->head_stride & align);
+    size_t need = 0;
+    rc = for_cache_chunks(v, [&](int, int nl) -> int {
+        AttendPlan pl;
+        const int r = plan_attend(c, v, nl, T, p->window > 0, mass_out != nullptr, pl);
+        need = std::max(need, pl.bytes);
+        return r;
+    });
+    if (rc) return rc;
+    if ((rc = ensure_attend(c, need, st))) return rc;
     return for_cache_chunks(v, [&](int l0, int nl) -> int {
+        AttendPlan pl;
+        const int r = plan_attend(c, v, nl, T, p->window > 0, mass_out != nullptr, pl);
+        if (r) return r;
         AttendArgs a;
         memset(&a, 0, sizeof a);
         const int64_t u0 = (int64_t)l0 * KV;
@@ -376,8 +470,8 @@ extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const in
         a.out = (__half *)out + l0 * p->o_cache_stride;
         a.q_cache = p->q_cache_stride; a.q_tok = p->q_tok_stride; a.q_head = p->q_head_stride;
         a.o_cache = p->o_cache_stride; a.o_tok = p->o_tok_stride; a.o_head = p->o_head_stride;
-        float *ls = lse ? lse : lse_b ? (float *)c->d_attend : nullptr;
-        a.lse = ls ? ls + (int64_t)l0 * T * H : nullptr;
+        a.lse = lse ? lse + (int64_t)l0 * T * H : nullptr;
+        a.copy16 = copy16;
         a.mass_in = mass_in ? mass_in + u0 * v->n_cells : nullptr;
         a.mass_out = mass_out ? mass_out + u0 * v->n_cells : nullptr;
         a.mass_decay = p->mass_decay;
@@ -393,7 +487,7 @@ extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const in
         a.tree_words = p->tree_words;
         a.status = c->d_status;
         if (v->type == TRIA_TYPE_F16)
-            return c->hd == 128 ? run_attend<KT_F16, 128>(c, a, st) : run_attend<KT_F16, 64>(c, a, st);
-        return c->hd == 128 ? run_attend<KT_Q8_0, 128>(c, a, st) : run_attend<KT_Q8_0, 64>(c, a, st);
+            return c->hd == 128 ? run_attend<KT_F16, 128>(c, a, pl, st) : run_attend<KT_F16, 64>(c, a, pl, st);
+        return c->hd == 128 ? run_attend<KT_Q8_0, 128>(c, a, pl, st) : run_attend<KT_Q8_0, 64>(c, a, pl, st);
     });
 }
