@@ -386,17 +386,23 @@ static_assert(FEW_SLICE == 16 && FEW_THREADS == ROW_THREADS, "warp tile");
 template <int KT, int HD>
 struct FewStage {
     static constexpr int KS = KT == KT_F16 ? 2 * HD : (HD == 128 ? 160 : 96);
-    static constexpr int VS = KT == KT_F16 ? 2 * HD : (HD == 128 ? 144 : 80);
+    static constexpr int VS = KT == KT_F16 ? 2 * HD : (HD == 128 ? 144 : 80);      /* 8 + 136, 68 */
     static constexpr int K = 0, V = 16 * KS, P = V + 16 * VS, BYTES = P + 64;
 };
 
-/* Stages a warp keeps in flight: as many as two blocks an SM leave room for. */
-template <int KT, int HD>
-__host__ __device__ constexpr int few_stages() { return KT == KT_F16 ? (HD == 128 ? 3 : 6) : (HD == 128 ? 5 : 8); }
-template <int KT, int HD, int MT>
+/* Blocks an SM holds, by registers (value sums and queries are 48 of them per
+ * 8 query rows), and the stages that their warps' rings leave room for. */
+template <int KT, int NT>
+__host__ __device__ constexpr int few_blocks() { return NT > 1 ? 2 : KT == KT_F16 ? 3 : 4; }
+template <int KT, int HD, int NT>
+__host__ __device__ constexpr int few_stages() {
+    const int fit = 200 * 1024 / few_blocks<KT, NT>() / FEW_WARPS / FewStage<KT, HD>::BYTES;
+    return fit < 4 ? fit : 4;
+}
+template <int KT, int HD, int NT>
 __host__ __device__ constexpr int few_smem() {
-    const int ring = FEW_WARPS * few_stages<KT, HD>() * FewStage<KT, HD>::BYTES;
-    const int merge = FEW_WARPS * 16 * MT * (HD + 8) * 4 + FEW_WARPS * 16 * MT * 8;
+    const int ring = FEW_WARPS * few_stages<KT, HD, NT>() * FewStage<KT, HD>::BYTES;
+    const int merge = FEW_WARPS * 8 * NT * (HD + 4) * 4 + FEW_WARPS * 8 * NT * 8;
     return ring > merge ? ring : merge;
 }
 
@@ -406,108 +412,102 @@ __host__ __device__ constexpr int few_smem() {
  * rescaled: 2^(FEW_LIFT + FEW_SLACK) is still finite in f16. */
 constexpr float FEW_LIFT = 6.0f, FEW_SLACK = 8.0f;
 
-/* Copies the warp's slice: rows [r0, r0 + 16) below n; rows at and behind n
- * become zeros. */
-template <int KT, int HD>
-__device__ __forceinline__ void few_load(const AttendArgs &a, const uint8_t *k, const uint8_t *v, const int32_t *pos,
-                                         bool want_pos, int r0, int n, uint32_t st, int lane) {
-    using S = FewStage<KT, HD>;
-    if constexpr (KT == KT_F16) {
-        constexpr int CH = HD / 8, PER = 16 * CH / 32;
-        if (a.copy16) {
+/* Copies one side of the warp's slice: rows [r0, r0 + 16) from p to `st`, row
+ * stride RS; rows at and behind n become zeros.  A full slice of aligned rows
+ * takes 16-byte copies with addresses stepped from one to the next: f16 a row
+ * by HD / 8 lanes, q8_0 rows of 136 bytes (8 bytes off a 16-byte boundary in
+ * every other head) by eight lanes and one 8-byte piece, on the side `lead`. */
+template <int KT, int HD, int RS>
+__device__ __forceinline__ void few_load(const AttendArgs &a, const uint8_t *p, int lead, int r0, int n, uint32_t st, int lane) {
+    const bool full = r0 + 16 <= n;
+    if (KT == KT_F16 && full && a.copy16) {
+        constexpr int CH = HD / 8, RPI = 32 / CH;
+        const int r = lane / CH, c = lane % CH;
+        const int64_t step = RPI * a.cell_stride;
+        p += (int64_t)(r0 + r) * a.cell_stride + 16 * c;
+        const uint32_t d = st + r * RS, cx = 16 * (c ^ r);
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                const int x = lane + 32 * i, r = x / CH, c = x % CH;
-                const bool in = r0 + r < n;
-                const int64_t off = in ? (int64_t)(r0 + r) * a.cell_stride + 16 * c : 0;
-                const uint32_t d = st + r * S::KS + 16 * (c ^ (r & 7));
-                cp_async16(d + S::K, k + off, in ? 16u : 0u);
-                cp_async16(d + S::V, v + off, in ? 16u : 0u);
-            }
-        } else {
-            for (int x = lane; x < 16 * CH * 4; x += 32) {
-                const int r = x / (CH * 4), c = x / 4 % CH, q = x & 3;
-                const bool in = r0 + r < n;
-                const int64_t off = in ? (int64_t)(r0 + r) * a.cell_stride + 16 * c + 4 * q : 0;
-                const uint32_t d = st + r * S::KS + 16 * (c ^ (r & 7)) + 4 * q;
-                cp_async4(d + S::K, k + off, in ? 4u : 0u);
-                cp_async4(d + S::V, v + off, in ? 4u : 0u);
-            }
+        for (int i = 0; i < 16 / RPI; i++) {
+            cp_async16(d + RPI * i * RS + (cx ^ (16 * ((RPI * i) & 7))), p, 16u);
+            p += step;
         }
+    } else if (KT == KT_Q8_0 && HD == 128 && full && a.copy16) {
+        const int r = lane >> 3, c = lane & 7;
+        const int64_t step = 4 * a.cell_stride;
+        const uint8_t *q = p + (int64_t)(r0 + r) * a.cell_stride + lead + 16 * c;
+        const uint32_t d = st + r * RS + 2 * lead + 16 * c;     /* a row starts lead bytes in, its chunks on 16 */
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            cp_async16(d + 4 * i * RS, q, 16u);
+            q += step;
+        }
+        if (lane < 16)
+            cp_async8(st + lane * RS + (lead ? lead : 128), p + (int64_t)(r0 + lane) * a.cell_stride + (lead ? 0 : 128), 8u);
     } else {
-        constexpr int RB = HD / 32 * 34;
-        if (a.copy16 && RB % 8 == 0) {
-            constexpr int CH = RB / 8;
-            for (int x = lane; x < 16 * CH; x += 32) {
-                const int r = x / CH, c = x - r * CH;
-                const bool in = r0 + r < n;
-                const int64_t off = in ? (int64_t)(r0 + r) * a.cell_stride + 8 * c : 0;
-                cp_async8(st + S::K + r * S::KS + 8 * c, k + off, in ? 8u : 0u);
-                cp_async8(st + S::V + r * S::VS + 8 * c, v + off, in ? 8u : 0u);
-            }
-        } else {
-            constexpr int CH = RB / 4;
-            for (int x = lane; x < 16 * CH; x += 32) {
-                const int r = x / CH, c = x - r * CH;
-                const bool in = r0 + r < n;
-                const int64_t off = in ? (int64_t)(r0 + r) * a.cell_stride + 4 * c : 0;
-                cp_async4(st + S::K + r * S::KS + 4 * c, k + off, in ? 4u : 0u);
-                cp_async4(st + S::V + r * S::VS + 4 * c, v + off, in ? 4u : 0u);
-            }
+        constexpr int W = KT == KT_F16 ? HD / 2 : HD / 32 * 34 / 4;
+        for (int x = lane; x < 16 * W; x += 32) {
+            const int r = x / W, c = x - r * W;
+            const bool in = r0 + r < n;
+            const uint32_t at = KT == KT_F16 ? 16 * ((c >> 2) ^ (r & 7)) + 4 * (c & 3) : lead + 4 * c;
+            cp_async4(st + r * RS + at, p + (in ? (int64_t)(r0 + r) * a.cell_stride + 4 * c : 0), in ? 4u : 0u);
         }
     }
-    if (want_pos && lane < 16) {
+}
+__device__ __forceinline__ void few_load_pos(const int32_t *pos, int r0, int n, uint32_t st, int lane) {
+    if (lane < 16) {
         const bool in = r0 + lane < n;
-        cp_async4(st + S::P + 4 * lane, pos + (in ? r0 + lane : 0), in ? 4u : 0u);
+        cp_async4(st + 4 * lane, pos + (in ? r0 + lane : 0), in ? 4u : 0u);
     }
 }
 
-/* The dims of a row that k-step s takes, for lane column c: f16 16 s + 2 c,
- * +1 and those 8 on; q8_0 the bytes 8 c + 4 (s & 1) .. +3 of block s / 2, so that
- * a lane's share of a block is 8 bytes in a row. */
+/* The dims that k-step s takes of a row, for lane column c: f16 16 s + 2 c, +1
+ * and those 8 on; q8_0 the bytes 8 c + 4 (s & 1) .. +3 of block s / 2, so that a
+ * lane's share of a block is 8 bytes in a row. */
 template <int KT>
 __device__ __forceinline__ int few_qdim(int s, int c, int hi) {
     return KT == KT_F16 ? 16 * s + 2 * c + 8 * hi : 32 * (s >> 1) + 8 * c + 4 * (s & 1) + 2 * hi;
 }
-/* The dim of accumulator tile j, column n: q8_0 tiles stay within a block and
- * give lane row n the bytes 4 n .. 4 n + 3 of it over its four tiles. */
+/* The dim of row r8 (+ 8 hi) of value tile j: q8_0 tiles stay within a block and
+ * give a lane row the bytes 4 r8 .. 4 r8 + 3 of it over the block's two tiles. */
 template <int KT>
-__device__ __forceinline__ int few_odim(int j, int n) {
-    return KT == KT_F16 ? 8 * j + n : 32 * (j >> 2) + 4 * n + (j & 3);
+__device__ __forceinline__ int few_odim(int j, int r8, int hi) {
+    return KT == KT_F16 ? 16 * j + r8 + 8 * hi : 32 * (j >> 1) + 4 * r8 + 2 * (j & 1) + hi;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
-/* The products of the slice's 16 keys with MT x 16 query rows: s[m][t][.] in
- * the accumulator layout, tile t keys 8 t .. 8 t + 7. */
-template <int KT, int HD, int MT>
-__device__ __forceinline__ void few_qk(const uint32_t (&qf)[MT][HD / 16][4], uint32_t st, int lane, float (&s)[MT][2][4]) {
-    using S = FewStage<KT, HD>;
+/* The products of 16 cache rows with 8 NT query rows, rows of the cache as the
+ * matrix rows: s[t][e] is cache row r8 + 8 (e >> 1) with query row 8 t + 2 c + (e & 1). */
+template <int KT, int HD, int NT>
+__device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], uint32_t st, int lead, int lane, float (&s)[NT][4]) {
+    constexpr int KS = FewStage<KT, HD>::KS;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[m][t][i] = 0.0f;
+        for (int i = 0; i < 4; i++) s[t][i] = 0.0f;
     if constexpr (KT == KT_F16) {
-        const int row = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
+        const int row = lane & 15, hi = lane >> 4;
 #pragma unroll
         for (int x = 0; x < HD / 16; x++) {
-            uint32_t b[4];
-            ldsm4(b, st + S::K + row * S::KS + 16 * ((2 * x + hi) ^ (row & 7)));
+            uint32_t k[4];
+            ldsm4(k, st + row * KS + 16 * ((2 * x + hi) ^ (row & 7)));
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                mma16816(s[m][0], qf[m][x], b[0], b[1]);
-                mma16816(s[m][1], qf[m][x], b[2], b[3]);
-            }
+            for (int t = 0; t < NT; t++) mma16816(s[t], k, qf[t][x][0], qf[t][x][1]);
         }
     } else {
-        const int r = lane >> 2, c = lane & 3;
+        const int r8 = lane >> 2, c = lane & 3;
+        st += lead + r8 * KS;
 #pragma unroll
         for (int blk = 0; blk < HD / 32; blk++) {
-            constexpr int KS = S::KS;
             const int sh = (2 * blk + 2) & 7;                        /* bytes into the aligned 8-byte word */
+            uint32_t k[2][4];
+            float d[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint32_t at = st + S::K + (8 * t + r) * KS + 34 * blk + 2 + 8 * c - sh;
+            for (int hi = 0; hi < 2; hi++) {
+                const uint32_t at = st + 8 * hi * KS + 34 * blk + 2 + 8 * c - sh;
                 const uint2 x = lds64(at);
                 uint32_t w0, w1;
                 if (sh == 0) {
@@ -518,96 +518,93 @@ __device__ __forceinline__ void few_qk(const uint32_t (&qf)[MT][HD / 16][4], uin
                     w0 = sh == 2 ? __funnelshift_r(x.x, x.y, 16) : sh == 4 ? x.y : __funnelshift_r(x.y, y.x, 16);
                     w1 = sh == 2 ? __funnelshift_r(x.y, y.x, 16) : sh == 4 ? y.x : __funnelshift_r(y.x, y.y, 16);
                 }
-                uint32_t b0, b1, b2, b3;
-                int8x4_half(w0, b0, b1);
-                int8x4_half(w1, b2, b3);
-                /* the block's scale belongs to the key, so it multiplies the block's sum: the f16 operands
-                 * stay the stored integers and the scores keep fp32 */
-                const float d0 = lds_half(st + S::K + (8 * t + 2 * c) * KS + 34 * blk);
-                const float d1 = lds_half(st + S::K + (8 * t + 2 * c + 1) * KS + 34 * blk);
+                int8x4_half(w0, k[0][hi], k[0][hi + 2]);
+                int8x4_half(w1, k[1][hi], k[1][hi + 2]);
+                d[hi] = lds_half(st + 8 * hi * KS + 34 * blk);
+            }
+            /* the block's scale belongs to the cache row, so it multiplies the block's sum: the f16 operands stay the
+             * stored integers and the scores keep fp32 */
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma16816(p, qf[m][2 * blk], b0, b1);
-                    mma16816(p, qf[m][2 * blk + 1], b2, b3);
-                    s[m][t][0] = fmaf(p[0], d0, s[m][t][0]);
-                    s[m][t][1] = fmaf(p[1], d1, s[m][t][1]);
-                    s[m][t][2] = fmaf(p[2], d0, s[m][t][2]);
-                    s[m][t][3] = fmaf(p[3], d1, s[m][t][3]);
-                }
+            for (int t = 0; t < NT; t++) {
+                float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma16816(p, k[0], qf[t][2 * blk][0], qf[t][2 * blk][1]);
+                mma16816(p, k[1], qf[t][2 * blk + 1][0], qf[t][2 * blk + 1][1]);
+                s[t][0] = fmaf(p[0], d[0], s[t][0]);
+                s[t][1] = fmaf(p[1], d[0], s[t][1]);
+                s[t][2] = fmaf(p[2], d[1], s[t][2]);
+                s[t][3] = fmaf(p[3], d[1], s[t][3]);
             }
         }
     }
 }
 
-/* o += p v over the slice's 16 rows; keep0, keep1: 0xffff for each f16 of a V
- * pair whose row some query row sees (a row that none sees may hold NaN). */
-template <int KT, int HD, int MT>
-__device__ __forceinline__ void few_pv(const float (&p)[MT][2][4], uint32_t st, int lane, uint32_t keep0, uint32_t keep1,
-                                       float (&o)[MT][HD / 8][4]) {
-    using S = FewStage<KT, HD>;
+/* o += v^T p over the slice's 16 rows.  FULL: every query row sees them all.
+ * Otherwise a weight of 0 meets 0: keep0, keep1 (f16) have the bits of a V pair
+ * whose row some query row sees, and a q8_0 scale only enters where p is not 0
+ * (a row that is not seen may hold NaN). */
+template <int KT, int HD, int NT, bool FULL>
+__device__ __forceinline__ void few_pv(const float (&p)[NT][4], uint32_t st, int lead, int lane, uint32_t keep0, uint32_t keep1,
+                                       float (&o)[NT][HD / 16][4]) {
+    constexpr int VS = FewStage<KT, HD>::VS;
     if constexpr (KT == KT_F16) {
-        uint32_t pf[MT][4];
+        uint32_t pf[NT][2];
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            pf[m][0] = pack_half2(p[m][0][0], p[m][0][1]);
-            pf[m][1] = pack_half2(p[m][0][2], p[m][0][3]);
-            pf[m][2] = pack_half2(p[m][1][0], p[m][1][1]);
-            pf[m][3] = pack_half2(p[m][1][2], p[m][1][3]);
+        for (int t = 0; t < NT; t++) {
+            pf[t][0] = transpose8(pack_half2(p[t][0], p[t][1]));
+            pf[t][1] = transpose8(pack_half2(p[t][2], p[t][3]));
         }
-        const int row = lane & 15, hi = lane >> 4;
+        const int row = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
 #pragma unroll
-        for (int j = 0; j < HD / 8; j += 2) {
-            uint32_t b[4];
-            ldsm4t(b, st + S::V + row * S::VS + 16 * ((j + hi) ^ (row & 7)));
-            b[0] &= keep0;
-            b[1] &= keep1;
-            b[2] &= keep0;
-            b[3] &= keep1;
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                mma16816(o[m][j], pf[m], b[0], b[1]);
-                mma16816(o[m][j + 1], pf[m], b[2], b[3]);
+        for (int j = 0; j < HD / 16; j++) {
+            uint32_t v[4];
+            ldsm4t(v, st + row * VS + 16 * ((2 * j + hi) ^ (row & 7)));
+            if (!FULL) {
+                v[0] &= keep0;
+                v[1] &= keep0;
+                v[2] &= keep1;
+                v[3] &= keep1;
             }
+#pragma unroll
+            for (int t = 0; t < NT; t++) mma16816(o[t][j], v, pf[t][0], pf[t][1]);
         }
     } else {
-        const int r = lane >> 2, c = lane & 3;
-        constexpr int VS = S::VS;
-        const uint32_t v0 = st + S::V + 2 * c * VS;                  /* rows 2c, 2c+1, 2c+8, 2c+9 */
+        const int r8 = lane >> 2, c = lane & 3;
+        st += lead;
+        const uint32_t v0 = st + 2 * c * VS + 4 * r8, d0 = st + r8 * VS;      /* rows 2c, 2c+1, 2c+8, 2c+9; scales of r8, r8+8 */
 #pragma unroll
         for (int blk = 0; blk < HD / 32; blk++) {
             const int sh = (2 * blk + 2) & 3;
             uint32_t w[4];
-            float d[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t at = v0 + ((i & 1) + (i >> 1) * 8) * VS + 34 * blk;
-                d[i] = lds_half(at);
-                if (sh == 0) w[i] = lds32(at + 2 + 4 * r);
-                else w[i] = __funnelshift_r(lds32(at + 4 * r), lds32(at + 4 + 4 * r), 16);
-                /* a row that no query row sees: its scale may be anything */
-                if (!((i >> 1 ? keep1 : keep0) >> (16 * (i & 1)) & 1u)) d[i] = 0.0f;
+                if (sh == 0) w[i] = lds32(at + 2);
+                else w[i] = __funnelshift_r(lds32(at), lds32(at + 4), 16);
             }
+            const float da = lds_half(d0 + 34 * blk), db = lds_half(d0 + 8 * VS + 34 * blk);
             /* the scales go into the weights before their one rounding to f16; the V operands are the stored integers */
-            uint32_t pf[MT][4];
+            uint32_t pf[NT][2];
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                pf[m][0] = pack_half2(p[m][0][0] * d[0], p[m][0][1] * d[1]);
-                pf[m][1] = pack_half2(p[m][0][2] * d[0], p[m][0][3] * d[1]);
-                pf[m][2] = pack_half2(p[m][1][0] * d[2], p[m][1][1] * d[3]);
-                pf[m][3] = pack_half2(p[m][1][2] * d[2], p[m][1][3] * d[3]);
+            for (int t = 0; t < NT; t++) {
+                float x[4] = {p[t][0] * da, p[t][1] * da, p[t][2] * db, p[t][3] * db};
+                if (!FULL) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = p[t][i] == 0.0f ? 0.0f : x[i];
+                }
+                pf[t][0] = transpose8(pack_half2(x[0], x[1]));
+                pf[t][1] = transpose8(pack_half2(x[2], x[3]));
             }
-            const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
-            const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
             uint32_t x[4], y[4];
-            int8x4_half(a01, x[0], x[1]);
-            int8x4_half(a23, x[2], x[3]);
-            int8x4_half(b01, y[0], y[1]);
-            int8x4_half(b23, y[2], y[3]);
+            int8x4_half(__byte_perm(w[0], w[1], 0x5140), x[0], x[1]);
+            int8x4_half(__byte_perm(w[0], w[1], 0x7362), x[2], x[3]);
+            int8x4_half(__byte_perm(w[2], w[3], 0x5140), y[0], y[1]);
+            int8x4_half(__byte_perm(w[2], w[3], 0x7362), y[2], y[3]);
+            const uint32_t lo[4] = {x[0], x[1], y[0], y[1]}, hi[4] = {x[2], x[3], y[2], y[3]};
 #pragma unroll
-            for (int jj = 0; jj < 4; jj++)
-#pragma unroll
-                for (int m = 0; m < MT; m++) mma16816(o[m][4 * blk + jj], pf[m], x[jj], y[jj]);
+            for (int t = 0; t < NT; t++) {
+                mma16816(o[t][2 * blk], lo, pf[t][0], pf[t][1]);
+                mma16816(o[t][2 * blk + 1], hi, pf[t][0], pf[t][1]);
+            }
         }
     }
 }
@@ -629,28 +626,34 @@ __device__ __forceinline__ float merge_row(int S, Ml &&ml, O &&o, float &m, floa
     return v;
 }
 
-/* Attention of the items' query rows (up to 16 * MT) over their steps.  The
+/* Attention of the items' query rows (8 NT a group) over their steps.  The
  * steps of all items are shared out evenly: block b takes steps
- * [b * total / grid, (b + 1) * total / grid) (grid: at most `total`), whatever units they fall in, so
- * ragged counts read from the device keep every SM busy without the host
- * knowing them.  Within a step each warp takes 16 cache rows of its own and
- * keeps its own running maximum, sum and value sums: the loop has no block
- * barrier, and a warp's copies run `stages` slices ahead.  An item that ends
- * in several blocks leaves partial results; the block that arrives last
- * merges them in block order, so the result does not depend on timing.
+ * [b * total / grid, (b + 1) * total / grid) (grid: at most `total`), whatever
+ * units they fall in, so ragged counts read from the device keep every SM busy
+ * without the host knowing them.  Within a step each warp takes 16 cache rows
+ * of its own and keeps its own running maximum, sum and value sums: the loop
+ * has no block barrier.  A warp's ring is refilled side by side, K as soon as
+ * the scores are made and V after the sums, so a stage is in flight but for the
+ * half being read.  An item that ends in several blocks leaves partial
+ * results; the block that arrives last merges them in block order, so the
+ * result does not depend on timing.
  *
- * Bound by the cache's bytes up to a few tens of query rows: 16 rows cost 32
- * mma (f16, head_dim 128) for 8 KB. */
-template <int KT, int HD, int MT>
-__global__ void __launch_bounds__(FEW_THREADS, 2) k_attend_few(const AttendArgs a) {
+ * Cache rows are the matrix rows and query rows its columns, so few query rows
+ * waste little: 16 cache rows cost 16 mma per 8 query rows (head_dim 128), and
+ * the weights turn around in registers (movmatrix) for the value product.
+ * EXTRA: the call caps, biases or windows its scores. */
+template <int KT, int HD, int NT, bool EXTRA>
+__global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_few(const AttendArgs a) {
     using S = FewStage<KT, HD>;
-    constexpr int ROWS = 16 * MT, ST = few_stages<KT, HD>(), OS = HD + 8;
+    constexpr int ROWS = 8 * NT, ST = few_stages<KT, HD, NT>(), OS = HD + 4;
+    static_assert(ST >= 2, "ring");
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int s_steps[512];
     __shared__ int s_warp[FEW_WARPS];
     __shared__ int s_flag;
     __shared__ RowShared<HD> s_row;
     __shared__ int s_redo[ROWS];
+    __shared__ float s_inv[ROWS];
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, r8 = lane >> 2, c = lane & 3;
     const int units = a.n_layer * a.n_head_kv, items = units * a.groups, R = a.T * a.G;
     const int *steps = a.steps;
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) k_attend_few(const AttendArgs 
     const int64_t total = steps[items - 1];
     const int b = blockIdx.x, grid = (int)min((int64_t)gridDim.x, total);     /* no block between an item's first and last is idle */
     const ScoreMap map(a);
-    const bool want_pos = a.window > 0 || a.slopes != nullptr;
+    const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
     const uint32_t ring = smem_u32(smem) + w * ST * S::BYTES;
 
     /* items without a row to see */
@@ -713,139 +716,173 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) k_attend_few(const AttendArgs 
         const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
         const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
 
+        const int lead = KT == KT_Q8_0 && HD == 128 ? (int)((h * a.head_stride) & 8) : 0;
+
+        auto load_k = [&](int i) {
+            if (i < i1) {
+                const int row = slice_row(i);
+                const uint32_t st = ring + ((i - i0) % ST) * S::BYTES;
+                few_load<KT, HD, S::KS>(a, k, lead, row, n, st + S::K, lane);
+                if (want_pos) few_load_pos(pos, row, n, st + S::P, lane);
+            }
+            cp_async_commit();
+        };
+        auto load_v = [&](int i) {
+            if (i < i1) few_load<KT, HD, S::VS>(a, v, lead, slice_row(i), n, ring + ((i - i0) % ST) * S::BYTES + S::V, lane);
+            cp_async_commit();
+        };
         /* prologue: copies first, then the queries while they fly */
 #pragma unroll
-        for (int p = 0; p < ST - 1; p++) {
-            if (i0 + p < i1) few_load<KT, HD>(a, k, v, pos, want_pos, slice_row(i0 + p), n, ring + p * S::BYTES, lane);
-            cp_async_commit();
+        for (int p = 0; p < ST; p++) {
+            load_k(i0 + p);
+            load_v(i0 + p);
         }
-        uint32_t qf[MT][HD / 16][4];
-        int tok[MT][2], tp[MT][2];
-        float slope2[MT][2];
+        uint32_t qf[NT][HD / 16][2];
+        int tok[NT][2], tp[NT][2];
+        float slope2[NT][2];
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int hi = 0; hi < 2; hi++) {
-                const int r = grp * ROWS + 16 * m + r8 + 8 * hi, t = r / a.G, head = h * a.G + r % a.G;
+        for (int t = 0; t < NT; t++) {
+            {
+                const int r = grp * ROWS + 8 * t + r8;
                 const bool in = r < R;
-                tok[m][hi] = in ? t : -1;
-                tp[m][hi] = in && want_pos ? a.tok_pos[l * a.tok_pos_stride + t] : 0;
-                slope2[m][hi] = in && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
-                const __half *q = a.q + l * a.q_cache + (in ? t * a.q_tok + head * a.q_head : 0);
+                const __half *q = a.q + l * a.q_cache + (in ? (r / a.G) * a.q_tok + (h * a.G + r % a.G) * a.q_head : 0);
 #pragma unroll
                 for (int s = 0; s < HD / 16; s++)
 #pragma unroll
                     for (int e = 0; e < 2; e++)
-                        qf[m][s][hi + 2 * e] = in ? *reinterpret_cast<const uint32_t *>(q + few_qdim<KT>(s, c, e)) : 0u;
+                        qf[t][s][e] = in ? *reinterpret_cast<const uint32_t *>(q + few_qdim<KT>(s, c, e)) : 0u;
             }
-        float o[MT][HD / 8][4], mx[MT][2], sum[MT][2];
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            mx[m][0] = mx[m][1] = -INFINITY;
-            sum[m][0] = sum[m][1] = 0.0f;
+            for (int e = 0; e < 2; e++) {
+                const int r = grp * ROWS + 8 * t + 2 * c + e;
+                const bool in = r < R;
+                tok[t][e] = in ? r / a.G : -1;
+                tp[t][e] = in && want_pos ? a.tok_pos[l * a.tok_pos_stride + r / a.G] : 0;
+                slope2[t][e] = EXTRA && in && a.slopes ? a.slopes[h * a.G + r % a.G] * LOG2E : 0.0f;
+            }
+        }
+        float o[NT][HD / 16][4], mx[NT][2], sum[NT][2];
 #pragma unroll
-            for (int j = 0; j < HD / 8; j++)
+        for (int t = 0; t < NT; t++) {
+            mx[t][0] = mx[t][1] = -INFINITY;
+            sum[t][0] = sum[t][1] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[m][j][i] = 0.0f;
+            for (int x = 0; x < HD / 16; x++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[t][x][i] = 0.0f;
         }
 
         for (int i = i0; i < i1; i++) {
-            const int nx = i + ST - 1;
-            cp_async_wait<ST - 2>();
-            __syncwarp();
-            if (nx < i1) few_load<KT, HD>(a, k, v, pos, want_pos, slice_row(nx), n, ring + ((nx - i0) % ST) * S::BYTES, lane);
-            cp_async_commit();
             const uint32_t st = ring + ((i - i0) % ST) * S::BYTES;
             const int row0 = slice_row(i);
-            if (row0 >= n) continue;
-            float s[MT][2][4];
-            few_qk<KT, HD, MT>(qf, st, lane, s);
+            const bool live = row0 < n;
+            float s[NT][4];
             uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-            const bool all = row0 + FEW_SLICE <= n - a.T && a.window <= 0;       /* every row is seen by every token */
-            uint32_t seen = 0;
+            const bool all = row0 + FEW_SLICE <= n - a.T && (!EXTRA || a.window <= 0);   /* every token sees every row */
+            cp_async_wait<2 * ST - 1>();
+            __syncwarp();
+            if (live) {
+                few_qk<KT, HD, NT>(qf, st + S::K, lead, lane, s);
+                if (EXTRA && map.cap > 0.0f) {
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int t = 0; t < 2; t++)
+                        for (int e = 0; e < 4; e++) s[t][e] = map.cap * tanh_both(s[t][e] * map.scale);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int hi = e >> 1, key = 8 * t + 2 * c + (e & 1);
-                        float x = map(s[m][t][e]);
-                        int pk = 0;
-                        if (want_pos) {
-                            pk = (int)lds32(st + S::P + 4 * key);
-                            x = fmaf(-slope2[m][hi], (float)(tp[m][hi] - pk), x);
-                        }
-                        if (!all) {
-                            const bool see = tok[m][hi] >= 0 &&
-                                             attend_sees(a, l, tok[m][hi], row0 + key, n, pk, (int64_t)tp[m][hi] - a.window);
-                            x = see ? x : -INFINITY;
-                            seen |= see ? 1u << (2 * t + (e & 1)) : 0u;
-                        }
-                        s[m][t][e] = x;
-                    }
-            if (!all) {
-                seen |= __shfl_xor_sync(0xffffffffu, seen, 4);
-                seen |= __shfl_xor_sync(0xffffffffu, seen, 8);
-                seen |= __shfl_xor_sync(0xffffffffu, seen, 16);
-                keep0 = (seen & 1u ? 0xffffu : 0u) | (seen & 2u ? 0xffff0000u : 0u);
-                keep1 = (seen & 4u ? 0xffffu : 0u) | (seen & 8u ? 0xffff0000u : 0u);
-            }
-            if (a.scores) {
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int hi = 0; hi < 2; hi++) {
-                        const int r = grp * ROWS + 16 * m + r8 + 8 * hi;
-                        if (r >= R) continue;
-                        float *d = a.scores + ((int64_t)u * R + r) * a.score_stride + row0 + 2 * c;
-                        *reinterpret_cast<float2 *>(d) = make_float2(s[m][0][2 * hi], s[m][0][2 * hi + 1]);
-                        *reinterpret_cast<float2 *>(d + 8) = make_float2(s[m][1][2 * hi], s[m][1][2 * hi + 1]);
-                    }
-            }
-            float top[MT][2];
-            bool up = false;
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int hi = 0; hi < 2; hi++) {
-                    float x = fmaxf(fmaxf(s[m][0][2 * hi], s[m][0][2 * hi + 1]), fmaxf(s[m][1][2 * hi], s[m][1][2 * hi + 1]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                    top[m][hi] = x;
-                    up |= x > mx[m][hi] + FEW_SLACK;
+                        for (int e = 0; e < 4; e++) s[t][e] *= map.scale;
                 }
-            if (__any_sync(0xffffffffu, up)) {
+                int pk[2] = {0, 0};
+                if (want_pos) {
+                    pk[0] = (int)lds32(st + S::P + 4 * r8);
+                    pk[1] = (int)lds32(st + S::P + 4 * (r8 + 8));
 #pragma unroll
-                for (int m = 0; m < MT; m++)
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int hi = 0; hi < 2; hi++) {
-                        const float to = fmaxf(mx[m][hi], top[m][hi]);
-                        const float f = to == mx[m][hi] ? 1.0f : ex2(mx[m][hi] - to);
-                        mx[m][hi] = to;
-                        sum[m][hi] *= f;
+                        for (int e = 0; e < 4; e++)
+                            s[t][e] = fmaf(-slope2[t][e & 1], (float)(tp[t][e & 1] - pk[e >> 1]), s[t][e]);
+                }
+                if (!all) {
+                    bool seen[2] = {false, false};
 #pragma unroll
-                        for (int j = 0; j < HD / 8; j++) {
-                            o[m][j][2 * hi] *= f;
-                            o[m][j][2 * hi + 1] *= f;
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const bool see = tok[t][e & 1] >= 0 &&
+                                             attend_sees(a, l, tok[t][e & 1], row0 + r8 + 8 * (e >> 1), n, pk[e >> 1],
+                                                         (int64_t)tp[t][e & 1] - a.window);
+                            s[t][e] = see ? s[t][e] : -INFINITY;
+                            seen[e >> 1] |= see;
                         }
-                    }
-            }
+                    /* rows 2c, 2c+1 (+ 8): four lanes each */
+                    const uint32_t b0 = __ballot_sync(0xffffffffu, seen[0]) >> (8 * c), b1 = __ballot_sync(0xffffffffu, seen[1]) >> (8 * c);
+                    keep0 = (b0 & 0xfu ? 0xffffu : 0u) | (b0 & 0xf0u ? 0xffff0000u : 0u);
+                    keep1 = (b1 & 0xfu ? 0xffffu : 0u) | (b1 & 0xf0u ? 0xffff0000u : 0u);
+                }
+                if (a.scores) {
 #pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int hi = 0; hi < 2; hi++) {
-                    const float from = mx[m][hi] == -INFINITY ? 0.0f : mx[m][hi] - FEW_LIFT;
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const float p = ex2(s[m][t][2 * hi + e] - from);
-                            s[m][t][2 * hi + e] = p;
-                            sum[m][hi] += p;
+                            const int r = grp * ROWS + 8 * t + 2 * c + e;
+                            if (r >= R) continue;
+                            float *d = a.scores + ((int64_t)u * R + r) * a.score_stride + row0 + r8;
+                            d[0] = s[t][e];
+                            d[8] = s[t][e + 2];
                         }
                 }
-            few_pv<KT, HD, MT>(s, st, lane, keep0, keep1, o);
+            }
+            __syncwarp();
+            load_k(i + ST);
+            if (live) {
+                float top[NT][2];
+                bool up = false;
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float x = fmaxf(s[t][e], s[t][e + 2]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        top[t][e] = x;
+                        up |= x > mx[t][e] + FEW_SLACK;
+                    }
+                if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float to = fmaxf(mx[t][e], top[t][e]);
+                            const float f = to == mx[t][e] ? 1.0f : ex2(mx[t][e] - to);
+                            mx[t][e] = to;
+                            sum[t][e] *= f;
+#pragma unroll
+                            for (int x = 0; x < HD / 16; x++) {
+                                o[t][x][e] *= f;
+                                o[t][x][e + 2] *= f;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float from = mx[t][e & 1] == -INFINITY ? 0.0f : mx[t][e & 1] - FEW_LIFT;
+                        s[t][e] = ex2(s[t][e] - from);
+                        sum[t][e & 1] += s[t][e];
+                    }
+            }
+            cp_async_wait<2 * ST - 1>();
+            __syncwarp();
+            if (live) {
+                if (all) few_pv<KT, HD, NT, true>(s, st + S::V, lead, lane, keep0, keep1, o);
+                else few_pv<KT, HD, NT, false>(s, st + S::V, lead, lane, keep0, keep1, o);
+            }
+            __syncwarp();
+            load_v(i + ST);
         }
         cp_async_wait<0>();
         __syncthreads();                                      /* the ring becomes the merge buffer */
@@ -853,19 +890,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) k_attend_few(const AttendArgs 
         float *mo = reinterpret_cast<float *>(smem);          /* [warp][ROWS][OS] */
         float2 *mml = reinterpret_cast<float2 *>(mo + FEW_WARPS * ROWS * OS);     /* [warp][ROWS] */
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int hi = 0; hi < 2; hi++) {
-                const int r = 16 * m + r8 + 8 * hi;
-                float x = sum[m][hi];
-                x += __shfl_xor_sync(0xffffffffu, x, 1);
-                x += __shfl_xor_sync(0xffffffffu, x, 2);
-                if (c == 0) mml[w * ROWS + r] = make_float2(mx[m][hi], x);
+            for (int e = 0; e < 2; e++) {
+                const int r = 8 * t + 2 * c + e;
+                float x = sum[t][e];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (r8 == 0) mml[w * ROWS + r] = make_float2(mx[t][e], x);
                 float *d = mo + (w * ROWS + r) * OS;
 #pragma unroll
-                for (int j = 0; j < HD / 8; j++) {
-                    d[few_odim<KT>(j, 2 * c)] = o[m][j][2 * hi];
-                    d[few_odim<KT>(j, 2 * c + 1)] = o[m][j][2 * hi + 1];
+                for (int j = 0; j < HD / 16; j++) {
+                    d[few_odim<KT>(j, r8, 0)] = o[t][j][e];
+                    d[few_odim<KT>(j, r8, 1)] = o[t][j][e + 2];
                 }
             }
         __syncthreads();
@@ -892,41 +930,98 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) k_attend_few(const AttendArgs 
             last = s_flag != 0;
         }
         if (last) {
+            for (int r = tid; r < ROWS; r += FEW_THREADS) s_redo[r] = 0;
             if (c0 != c1) {
                 __threadfence();
                 if (tid == 0) a.arrived[c0] = 0;
             }
-            const int s0 = 2 * c0 + (c0 * total / grid >= base ? 0 : 1);     /* block c0's slot; the others' first */
-            auto slot_of = [&](int s) { return s == 0 ? s0 : 2 * (c0 + s); };
-            int bad = 0;
-            for (int r = dr; r < rows; r += DPT) {
-                float m, sm, val;
-                if (c0 == c1)
-                    val = merge_row(FEW_WARPS, [&](int s) { return mml[s * ROWS + r]; },
-                                    [&](int s) { return mo[(s * ROWS + r) * OS + d]; }, m, sm);
-                else
-                    val = merge_row(c1 - c0 + 1, [&](int s) { return __ldcg(&a.part_ml[(int64_t)slot_of(s) * ROWS + r]); },
-                                    [&](int s) { return __ldcg(&a.part_o[((int64_t)slot_of(s) * ROWS + r) * HD + d]); }, m, sm);
-                const int q = grp * ROWS + r, t = q / a.G, hq = h * a.G + q % a.G;
+            auto put = [&](int r, int dim, float x) {
+                const int q = grp * ROWS + r;
+                if (!(fabsf(x) < INFINITY)) s_redo[r] = 1;
+                return a.out + l * a.o_cache + (q / a.G) * a.o_tok + (h * a.G + q % a.G) * a.o_head + dim;
+            };
+            auto put_sums = [&](int r, float m, float sm) {
+                const int q = grp * ROWS + r;
                 const bool none = sm == 0.0f;
-                val = none ? 0.0f : val / sm;
-                a.out[l * a.o_cache + t * a.o_tok + hq * a.o_head + d] = __float2half_rn(val);
-                if (!(fabsf(val) < INFINITY)) bad = 1;
-                if (d == 0) {
-                    if (a.lse) a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + hq] =
-                        none ? -INFINITY : (m - FEW_LIFT + log2f(sm)) * LN2;
-                    if (a.norm) a.norm[(int64_t)u * R + q] = none ? make_float2(0.0f, 0.0f) : make_float2(m - FEW_LIFT, 1.0f / sm);
+                if (a.lse) a.lse[((int64_t)l * a.T + q / a.G) * a.n_head_kv * a.G + h * a.G + q % a.G] =
+                    none ? -INFINITY : (m - FEW_LIFT + log2f(sm)) * LN2;
+                if (a.norm) a.norm[(int64_t)u * R + q] = none ? make_float2(0.0f, 0.0f) : make_float2(m - FEW_LIFT, 1.0f / sm);
+            };
+            __syncthreads();
+            if (c0 == c1) {
+                for (int r = dr; r < rows; r += DPT) {
+                    float m, sm;
+                    float val = merge_row(FEW_WARPS, [&](int s) { return mml[s * ROWS + r]; },
+                                          [&](int s) { return mo[(s * ROWS + r) * OS + d]; }, m, sm);
+                    val = sm == 0.0f ? 0.0f : val / sm;
+                    *put(r, d, val) = __float2half_rn(val);
+                    if (d == 0) put_sums(r, m, sm);
+                }
+            } else {
+                /* the factor of every partial result first (a warp per row), then the value sums, four dims a thread and
+                 * several results in flight */
+                const int nS = c1 - c0 + 1, s0 = 2 * c0 + (c0 * total / grid >= base ? 0 : 1);   /* c0's slot; the others' first */
+                float2 *f = reinterpret_cast<float2 *>(smem);                /* [nS][rows] */
+                for (int x = tid; x < nS * rows; x += FEW_THREADS) {
+                    const int s = x / rows, r = x - s * rows;
+                    f[x] = __ldcg(&a.part_ml[(int64_t)(s == 0 ? s0 : 2 * (c0 + s)) * ROWS + r]);
+                }
+                __syncthreads();
+                for (int r = w; r < rows; r += FEW_WARPS) {
+                    float m = -INFINITY, sm = 0.0f;
+                    for (int s = lane; s < nS; s += 32) m = fmaxf(m, f[s * rows + r].x);
+#pragma unroll
+                    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                    for (int s = lane; s < nS; s += 32) {
+                        const float2 y = f[s * rows + r];
+                        const float g = y.x == -INFINITY ? 0.0f : ex2(y.x - m);
+                        sm = fmaf(y.y, g, sm);
+                        f[s * rows + r].x = g;
+                    }
+#pragma unroll
+                    for (int x = 16; x; x >>= 1) sm += __shfl_xor_sync(0xffffffffu, sm, x);
+                    if (lane == 0) {
+                        put_sums(r, m, sm);
+                        s_inv[r] = sm == 0.0f ? 0.0f : 1.0f / sm;
+                    }
+                }
+                __syncthreads();
+                constexpr int RPP = FEW_THREADS / (HD / 4);
+                const int dim = tid % (HD / 4) * 4;
+                for (int r = tid / (HD / 4); r < rows; r += RPP) {
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int sb = 0; sb < nS; sb += 8) {
+                        float4 x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const int s = sb + i;
+                            if (s < nS)
+                                x[i] = __ldcg(reinterpret_cast<const float4 *>(
+                                    a.part_o + ((int64_t)(s == 0 ? s0 : 2 * (c0 + s)) * ROWS + r) * HD + dim));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float g = sb + i < nS ? f[(sb + i) * rows + r].x : 0.0f;
+                            if (g != 0.0f) {             /* not 0 times what may be infinite */
+                                acc.x = fmaf(x[i].x, g, acc.x);
+                                acc.y = fmaf(x[i].y, g, acc.y);
+                                acc.z = fmaf(x[i].z, g, acc.z);
+                                acc.w = fmaf(x[i].w, g, acc.w);
+                            }
+                        }
+                    }
+                    const float inv = s_inv[r];
+                    if (inv == 0.0f) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    acc.x *= inv;
+                    acc.y *= inv;
+                    acc.z *= inv;
+                    acc.w *= inv;
+                    __half *dst = put(r, dim, acc.x + acc.y + acc.z + acc.w);
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_half2(acc.x, acc.y), pack_half2(acc.z, acc.w));
                 }
             }
             /* a value that is not finite may be 0 times another token's row: those query rows again, one by one */
-            if (a.T > 1 && __syncthreads_or(bad)) {
-                for (int r = tid; r < ROWS; r += FEW_THREADS) s_redo[r] = 0;
-                __syncthreads();
-                for (int r = dr; r < rows; r += DPT) {
-                    const int q = grp * ROWS + r;
-                    const float x = __half2float(a.out[l * a.o_cache + (q / a.G) * a.o_tok + (h * a.G + q % a.G) * a.o_head + d]);
-                    if (!(fabsf(x) < INFINITY)) s_redo[r] = 1;
-                }
+            if (a.T > 1) {
                 __syncthreads();
                 for (int r = 0; r < rows; r++)
                     if (s_redo[r]) attend_row<KT, HD>(a, u, (grp * ROWS + r) % a.G, (grp * ROWS + r) / a.G, s_row);
@@ -971,7 +1066,8 @@ constexpr int MASS_THREADS = 128, MASS_KEYS = 64;
 template <int KT, int HD>
 __global__ void __launch_bounds__(MASS_THREADS) k_mass_tiles(const AttendArgs a) {
     using S = FewStage<KT, HD>;
-    __shared__ __align__(16) uint8_t s_keys[MASS_THREADS / 32][S::BYTES];
+    constexpr int NT = 2;
+    __shared__ __align__(16) uint8_t s_keys[MASS_THREADS / 32][16 * S::KS + 64];
     const int u = blockIdx.y, l = u / a.n_head_kv, h = u - l * a.n_head_kv, R = a.T * a.G;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, r8 = lane >> 2, c = lane & 3;
     const int n = attend_rows(a, u);
@@ -980,66 +1076,66 @@ __global__ void __launch_bounds__(MASS_THREADS) k_mass_tiles(const AttendArgs a)
     const bool want_pos = a.window > 0 || a.slopes != nullptr;
     const ScoreMap map(a);
     const uint32_t st = smem_u32(s_keys[w]);
+    const int lead = KT == KT_Q8_0 && HD == 128 ? (int)((h * a.head_stride) & 8) : 0;
     for (int row0 = (blockIdx.x * (MASS_THREADS / 32) + w) * 16; row0 < n; row0 += gridDim.x * MASS_KEYS) {
         __syncwarp();
-        few_load<KT, HD>(a, k, k, pos, want_pos, row0, n, st, lane);
+        few_load<KT, HD, S::KS>(a, k, lead, row0, n, st, lane);
+        if (want_pos) few_load_pos(pos, row0, n, st + 16 * S::KS, lane);
         cp_async_commit();
         cp_async_wait<0>();
         __syncwarp();
-        float mass[4] = {0.0f, 0.0f, 0.0f, 0.0f};               /* keys 2c, 2c+1, 2c+8, 2c+9 */
+        int pk[2] = {0, 0};
+        if (want_pos) {
+            pk[0] = (int)lds32(st + 16 * S::KS + 4 * r8);
+            pk[1] = (int)lds32(st + 16 * S::KS + 4 * (r8 + 8));
+        }
+        float mass[2] = {0.0f, 0.0f};                           /* cache rows r8, r8 + 8 */
         /* by order, token t sees row j only if j <= n - T + t: query rows before that see none of these 16 */
         int q0 = 0;
-        if (!a.tree) q0 = max(0, row0 - (n - a.T)) * a.G / 16 * 16;
-        for (; q0 < R; q0 += 16) {
-            uint32_t qf[1][HD / 16][4];
-            int tok[2], tp[2];
-            float slope2[2];
-            float2 nm[2];
+        if (!a.tree) q0 = max(0, row0 - (n - a.T)) * a.G / (8 * NT) * (8 * NT);
+        for (; q0 < R; q0 += 8 * NT) {
+            uint32_t qf[NT][HD / 16][2];
 #pragma unroll
-            for (int hi = 0; hi < 2; hi++) {
-                const int r = q0 + r8 + 8 * hi, t = r / a.G, head = h * a.G + r % a.G;
+            for (int t = 0; t < NT; t++) {
+                const int r = q0 + 8 * t + r8;
                 const bool in = r < R;
-                tok[hi] = in ? t : -1;
-                tp[hi] = in && want_pos ? a.tok_pos[l * a.tok_pos_stride + t] : 0;
-                slope2[hi] = in && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
-                nm[hi] = in ? a.norm[(int64_t)u * R + r] : make_float2(0.0f, 0.0f);
-                const __half *q = a.q + l * a.q_cache + (in ? t * a.q_tok + head * a.q_head : 0);
+                const __half *q = a.q + l * a.q_cache + (in ? (r / a.G) * a.q_tok + (h * a.G + r % a.G) * a.q_head : 0);
 #pragma unroll
                 for (int s = 0; s < HD / 16; s++)
 #pragma unroll
                     for (int e = 0; e < 2; e++)
-                        qf[0][s][hi + 2 * e] = in ? *reinterpret_cast<const uint32_t *>(q + few_qdim<KT>(s, c, e)) : 0u;
+                        qf[t][s][e] = in ? *reinterpret_cast<const uint32_t *>(q + few_qdim<KT>(s, c, e)) : 0u;
             }
-            float s[1][2][4];
-            few_qk<KT, HD, 1>(qf, st, lane, s);
-            const bool all = row0 + 16 <= n - a.T && a.window <= 0 && q0 + 16 <= R;
+            float s[NT][4];
+            few_qk<KT, HD, NT>(qf, st, lead, lane, s);
+            const bool all = row0 + 16 <= n - a.T && a.window <= 0 && q0 + 8 * NT <= R;
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int hi = e >> 1, key = 8 * t + 2 * c + (e & 1);
-                    float x = map(s[0][t][e]);
-                    int pk = 0;
-                    if (want_pos) {
-                        pk = (int)lds32(st + S::P + 4 * key);
-                        x = fmaf(-slope2[hi], (float)(tp[hi] - pk), x);
+                for (int e = 0; e < 2; e++) {
+                    const int r = q0 + 8 * t + 2 * c + e, tk = r / a.G;
+                    const bool in = r < R;
+                    const float2 nm = in ? a.norm[(int64_t)u * R + r] : make_float2(0.0f, 0.0f);
+                    const int tp = in && want_pos ? a.tok_pos[l * a.tok_pos_stride + tk] : 0;
+                    const float slope2 = in && a.slopes ? a.slopes[h * a.G + r % a.G] * LOG2E : 0.0f;
+#pragma unroll
+                    for (int hi = 0; hi < 2; hi++) {
+                        float x = map(s[t][e + 2 * hi]);
+                        if (want_pos) x = fmaf(-slope2, (float)(tp - pk[hi]), x);
+                        bool see = in;
+                        if (!all) see = in && attend_sees(a, l, tk, row0 + r8 + 8 * hi, n, pk[hi], (int64_t)tp - a.window);
+                        if (see) mass[hi] = fmaf(ex2(x - nm.x), nm.y, mass[hi]);
                     }
-                    bool see = true;
-                    if (!all) see = tok[hi] >= 0 && attend_sees(a, l, tok[hi], row0 + key, n, pk, (int64_t)tp[hi] - a.window);
-                    if (see) mass[2 * t + (e & 1)] = fmaf(ex2(x - nm[hi].x), nm[hi].y, mass[2 * t + (e & 1)]);
                 }
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int m = 4; m < 32; m <<= 1) mass[i] += __shfl_xor_sync(0xffffffffu, mass[i], m);
-        if (r8 == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int j = row0 + 2 * c + (i & 1) + 8 * (i >> 1);
-                if (j >= n) continue;
+        for (int hi = 0; hi < 2; hi++) {
+            mass[hi] += __shfl_xor_sync(0xffffffffu, mass[hi], 1);
+            mass[hi] += __shfl_xor_sync(0xffffffffu, mass[hi], 2);
+            const int j = row0 + r8 + 8 * hi;
+            if (c == 0 && j < n) {
                 const int64_t x = (int64_t)u * a.n_cells + j;
-                a.mass_out[x] = a.mass_in ? fmaf(a.mass_decay, a.mass_in[x], mass[i]) : mass[i];
+                a.mass_out[x] = a.mass_in ? fmaf(a.mass_decay, a.mass_in[x], mass[hi]) : mass[hi];
             }
         }
     }

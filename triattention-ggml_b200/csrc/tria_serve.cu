@@ -296,9 +296,14 @@ static int ensure_attend(tria_ctx *c, size_t need, cudaStream_t st) {
     return TRIA_OK;
 }
 
+template <int KT>
+static int few_blocks_of(int nt) {
+    return nt == 1 ? few_blocks<KT, 1>() : nt == 2 ? few_blocks<KT, 2>() : few_blocks<KT, 4>();
+}
+
 /* Launch plan of one chunk of caches. */
 struct AttendPlan {
-    int mt = 1;                 /* 16-row tiles of query rows per group */
+    int nt = 1;                 /* query rows per group, in eights */
     int groups = 0, items = 0, grid = 0;
     bool plan_kernel = false, keep_scores = false;
     size_t steps = 0, span = 0, done = 0, arrived = 0, part_o = 0, part_ml = 0, norm = 0, scores = 0, lse = 0, bytes = 0;
@@ -314,14 +319,15 @@ constexpr size_t SCORES_MAX = (size_t)1 << 30;
 static int plan_attend(const tria_ctx *c, const tria_kv_view *v, int nl, int T, bool window, bool mass, AttendPlan &pl) {
     const int64_t units = (int64_t)nl * v->n_head_kv, R = (int64_t)T * c->G;
     pl = AttendPlan{};
-    pl.mt = R <= 16 ? 1 : 2;
-    const int rows = 16 * pl.mt;
+    pl.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
+    const int rows = 8 * pl.nt;
     const int64_t groups = (R + rows - 1) / rows, items = units * groups;
     if (items * ((v->n_cells + ATT_STEP - 1) / ATT_STEP + 1) > INT32_MAX)
         FAIL(TRIA_ERR_UNSUPPORTED, "tria_attend: %lld query rows over %d cells in one call", (long long)(units * R), v->n_cells);
     pl.groups = (int)groups;
     pl.items = (int)items;
-    pl.grid = std::min(2 * c->sm_count, ATTEND_MAX_GRID);
+    pl.grid = std::min((v->type == TRIA_TYPE_F16 ? few_blocks_of<KT_F16>(pl.nt) : few_blocks_of<KT_Q8_0>(pl.nt)) * c->sm_count,
+                       ATTEND_MAX_GRID);
     pl.plan_kernel = window || items > 512;
     pl.score_stride = ((int64_t)v->n_cells + ATT_STEP - 1) / ATT_STEP * ATT_STEP;
     const size_t sb = (size_t)(units * R * pl.score_stride) * 4;
@@ -343,10 +349,11 @@ static int plan_attend(const tria_ctx *c, const tria_kv_view *v, int nl, int T, 
     return TRIA_OK;
 }
 
-template <int KT, int HD, int MT>
+template <int KT, int HD, int NT>
 static int launch_few(tria_ctx *c, const AttendArgs &a, const AttendPlan &pl, cudaStream_t st) {
-    auto fn = k_attend_few<KT, HD, MT>;
-    constexpr int smem = few_smem<KT, HD, MT>();
+    const bool extra = a.softcap > 0.0f || a.window > 0 || a.slopes;
+    auto fn = extra ? k_attend_few<KT, HD, NT, true> : k_attend_few<KT, HD, NT, false>;
+    constexpr int smem = few_smem<KT, HD, NT>();
     CUDA_TRY(raise_smem_limit((const void *)fn, smem));
     fn<<<pl.grid, FEW_THREADS, smem, st>>>(a);
     CUDA_TRY(cudaGetLastError());
@@ -369,14 +376,15 @@ static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStre
         if (pl.plan_kernel) {
             int32_t *steps = (int32_t *)(ws + pl.steps);
             int2 *span = a.window > 0 ? (int2 *)(ws + pl.span) : nullptr;
-            k_attend_plan<<<span ? pl.items : 1, PLAN_THREADS, 0, st>>>(a, 16 * pl.mt, pl.items, span, steps,
+            k_attend_plan<<<span ? pl.items : 1, PLAN_THREADS, 0, st>>>(a, 8 * pl.nt, pl.items, span, steps,
                                                                        (int32_t *)(ws + pl.done));
             CUDA_TRY(cudaGetLastError());
             c->launches++;
             a.steps = steps;
             a.span = span;
         }
-        const int rc = pl.mt == 1 ? launch_few<KT, HD, 1>(c, a, pl, st) : launch_few<KT, HD, 2>(c, a, pl, st);
+        const int rc = pl.nt == 1 ? launch_few<KT, HD, 1>(c, a, pl, st)
+                     : pl.nt == 2 ? launch_few<KT, HD, 2>(c, a, pl, st) : launch_few<KT, HD, 4>(c, a, pl, st);
         if (rc) return rc;
     }
     if (a.mass_out) {
@@ -436,9 +444,8 @@ extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const in
     if (T == 0 && !mass_out) return TRIA_OK;
     DeviceGuard g(c->device);
     cudaStream_t st = (cudaStream_t)stream;
-    bool copy16 = true;                       /* rows on 16-byte (q8_0: 8-byte) boundaries */
-    const int align = v->type == TRIA_TYPE_F16 ? 15 : 7;
-    copy16 = !(v->cell_stride & align) && !(v->head_stride & align);
+    /* rows on 16-byte boundaries (q8_0: 8 bytes off them, the same for every cell of a head) */
+    const bool copy16 = !(v->cell_stride & 15) && !(v->head_stride & (v->type == TRIA_TYPE_F16 ? 15 : 7));
     size_t need = 0;
     rc = for_cache_chunks(v, [&](int, int nl) -> int {
         AttendPlan pl;

@@ -159,9 +159,9 @@ def attend_params(scale, softcap=0.0, window=0, sink=0, slopes=None, tok_pos=Non
     sees token j."""
     p = AttendParams()
     p.scale, p.softcap, p.window, p.sink, p.mass_decay = scale, softcap, int(window), int(sink), mass_decay
-    p.slopes = _ptr(_ints_or_floats(slopes, "slopes", 1, "float32"))
-    p.tok_pos = _ptr(_ints_or_floats(tok_pos, "tok_pos", 2, "int32"))
-    p.tree = _ptr(_ints_or_floats(tree, "tree", 3, "int32"))
+    p.slopes = _ptr(_ints_or_floats(slopes, "slopes", 1, _torch().float32))
+    p.tok_pos = _ptr(_ints_or_floats(tok_pos, "tok_pos", 2, _torch().int32))
+    p.tree = _ptr(_ints_or_floats(tree, "tree", 3, _torch().int32))
     if tok_pos is not None and tok_pos.dim() == 2:
         p.tok_pos_stride = tok_pos.stride(0)
     if tree is not None:
@@ -172,19 +172,25 @@ def attend_params(scale, softcap=0.0, window=0, sink=0, slopes=None, tok_pos=Non
     return p
 
 
+def _torch():
+    """torch, imported by the callers that hand tensors in."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
+
+
+_torch_module = None
+
+
 def _ints_or_floats(x, name, most_dims, dtype):
     if x is None:
         return None
-    if str(x.dtype) != "torch." + dtype or not 1 <= x.dim() <= most_dims or (x.shape[-1] > 1 and x.stride(-1) != 1):
+    if x.dtype != dtype or not 1 <= x.dim() <= most_dims or (x.shape[-1] > 1 and x.stride(-1) != 1):
         raise ValueError(f"{name}: a {dtype} tensor of at most {most_dims} dimensions with a contiguous last one is wanted")
     if x.dim() >= 2 and name == "tree" and x.shape[-2] > 1 and x.stride(-2) != x.shape[-1]:
         raise ValueError("tree: rows must follow one another")
-    return x
-
-
-def _tensor(x, name, dtypes, dims):
-    if str(x.dtype).replace("torch.", "") not in dtypes or x.dim() != dims:
-        raise ValueError(f"{name}: a tensor of {' or '.join(dtypes)} with {dims} dimensions is wanted, got {x.dtype} {tuple(x.shape)}")
     return x
 
 
@@ -539,70 +545,77 @@ class Context:
         """tria_append: device tensors k, v [caches][n_tok][kv heads][head_dim]
         (f16 or fp32, contiguous last dimension) behind each unit's n_rows (device
         int32); n_rows_out defaults to n_rows, updated in place."""
-        for x, name in ((k, "k"), (v, "v")):
-            _tensor(x, name, ("float16", "float32"), 4)
-            if x.stride(3) != 1 and x.shape[3] > 1 or x.shape != k.shape or x.dtype != k.dtype or x.stride() != k.stride():
-                raise ValueError("k and v must have the same shape, type and strides, the last dimension contiguous")
-        if tuple(k.shape) != (view.n_layer, k.shape[1], view.n_head_kv, self.head_dim):
-            raise ValueError(f"k of shape {tuple(k.shape)} for {view.n_layer} caches of {view.n_head_kv} heads of {self.head_dim}")
-        self._shared_or_own(tok_pos, "tok_pos", (k.shape[1],), view.n_layer)
-        _ints_or_floats(tok_pos, "tok_pos", 2, "int32")
+        shape, stride, dtype = k.shape, k.stride(), k.dtype
+        if len(shape) != 4 or stride[3] != 1 or v.shape != shape or v.stride() != stride or v.dtype != dtype:
+            raise ValueError("k and v must have the same shape [caches][n_tok][kv heads][head_dim], type and strides, the last "
+                             "dimension contiguous")
+        f32 = dtype == _torch().float32
+        if not f32 and dtype != _torch().float16:
+            raise ValueError(f"k and v must be float16 or float32, not {dtype}")
+        if shape[0] != view.n_layer or shape[2] != view.n_head_kv or shape[3] != self.head_dim:
+            raise ValueError(f"k of shape {tuple(shape)} for {view.n_layer} caches of {view.n_head_kv} heads of {self.head_dim}")
+        self._shared_or_own(tok_pos, "tok_pos", (shape[1],), view.n_layer)
+        _ints_or_floats(tok_pos, "tok_pos", 2, _torch().int32)
         self._mass(mass, view)
         self._here(k, v, tok_pos, mass)
-        self._counts(view, n_rows, *(() if n_rows_out is None else (n_rows_out,)))
-        p = AppendParams()
-        p.n_tok, p.src_type = k.shape[1], SRC_F32 if str(k.dtype) == "torch.float32" else SRC_F16
-        p.cache_stride, p.tok_stride, p.head_stride = k.stride(0), k.stride(1), k.stride(2)
-        p.tok_pos, p.tok_pos_stride = _ptr(tok_pos), tok_pos.stride(0) if tok_pos.dim() == 2 else 0
-        check(lib().tria_append(self.h, C.byref(view), _ptr(n_rows), C.byref(p), _ptr(k), _ptr(v), _ptr(mass),
-                                _ptr(n_rows if n_rows_out is None else n_rows_out), _stream(stream)))
+        rows_out = n_rows if n_rows_out is None else n_rows_out
+        self._counts(view, n_rows, rows_out)
+        p = AppendParams(shape[1], SRC_F32 if f32 else SRC_F16, stride[0], stride[1], stride[2], tok_pos.data_ptr(),
+                         tok_pos.stride(0) if tok_pos.dim() == 2 else 0)
+        check(lib().tria_append(self.h, C.byref(view), n_rows.data_ptr(), C.byref(p), k.data_ptr(), v.data_ptr(), _ptr(mass),
+                                rows_out.data_ptr(), _stream(stream)))
 
     def attend(self, view, n_rows, q, out, params, lse=None, mass_in=None, mass_out=None, stream=None):
         """tria_attend: device f16 tensors q, out [caches][n_tok][heads][head_dim]
         (any strides that are multiples of 8, the last dimension contiguous)."""
-        for x, name in ((q, "q"), (out, "out")):
-            _tensor(x, name, ("float16",), 4)
-            if x.stride(3) != 1 or x.shape != q.shape:
-                raise ValueError("q and out must have the same shape and a contiguous last dimension")
+        sig = (view.n_layer, view.n_head_kv, self.gqa, self.head_dim, q.shape, q.stride(), out.shape, out.stride(), q.dtype, out.dtype)
+        if getattr(params, "_sig", None) != sig:
+            self._attend_shapes(view, q, out, params)
+            params._sig = sig
+        if lse is not None and (lse.dtype != _torch().float32 or tuple(lse.shape) != tuple(q.shape[:3]) or not lse.is_contiguous()):
+            raise ValueError("lse must be a contiguous fp32 [caches][n_tok][heads]")
+        self._mass(mass_in, view)
+        self._mass(mass_out, view)
+        self._here(q, out, lse, mass_in, mass_out, *params._keep)
+        self._counts(view, n_rows)
+        check(lib().tria_attend(self.h, C.byref(view), n_rows.data_ptr(), C.byref(params), q.data_ptr(), out.data_ptr(),
+                                _ptr(lse), _ptr(mass_in), _ptr(mass_out), _stream(stream)))
+
+    def _attend_shapes(self, view, q, out, params):
+        """Checks q and out against the view and the params, and puts their strides into the params."""
+        f16 = _torch().float16
+        if q.dtype != f16 or out.dtype != f16 or q.dim() != 4 or out.shape != q.shape or q.stride(3) != 1 or out.stride(3) != 1:
+            raise ValueError("q and out must be float16 of the same shape [caches][n_tok][heads][head_dim], the last dimension "
+                             "contiguous")
         if q.shape[0] != view.n_layer or q.shape[2] != view.n_head_kv * self.gqa or q.shape[3] != self.head_dim:
             raise ValueError(f"q of shape {tuple(q.shape)} for {view.n_layer} caches of {view.n_head_kv} x {self.gqa} heads "
                              f"of {self.head_dim}")
-        T = q.shape[1]
-        slopes, tok_pos, tree = getattr(params, "_keep", (None, None, None))
+        slopes, tok_pos, tree = params._keep
         if slopes is not None and slopes.shape[0] != q.shape[2]:
             raise ValueError(f"{slopes.shape[0]} slopes for {q.shape[2]} heads")
-        self._shared_or_own(tok_pos, "tok_pos", (T,), view.n_layer)
-        self._shared_or_own(tree, "tree", (T, params.tree_words), view.n_layer)
-        if lse is not None:
-            _tensor(lse, "lse", ("float32",), 3)
-            if tuple(lse.shape) != (view.n_layer, T, q.shape[2]) or not lse.is_contiguous():
-                raise ValueError("lse must be a contiguous [caches][n_tok][heads]")
-        for m in (mass_in, mass_out):
-            self._mass(m, view)
-        self._here(q, out, lse, mass_in, mass_out, slopes, tok_pos, tree)
-        self._counts(view, n_rows)
-        params.n_tok = T
-        params.q_cache_stride, params.q_tok_stride, params.q_head_stride = q.stride(0), q.stride(1), q.stride(2)
-        params.o_cache_stride, params.o_tok_stride, params.o_head_stride = out.stride(0), out.stride(1), out.stride(2)
-        check(lib().tria_attend(self.h, C.byref(view), _ptr(n_rows), C.byref(params), _ptr(q), _ptr(out), _ptr(lse),
-                                _ptr(mass_in), _ptr(mass_out), _stream(stream)))
+        self._shared_or_own(tok_pos, "tok_pos", (q.shape[1],), view.n_layer)
+        self._shared_or_own(tree, "tree", (q.shape[1], params.tree_words), view.n_layer)
+        params.n_tok = q.shape[1]
+        params.q_cache_stride, params.q_tok_stride, params.q_head_stride = q.stride()[:3]
+        params.o_cache_stride, params.o_tok_stride, params.o_head_stride = out.stride()[:3]
 
     def accept(self, view, n_rows, n_tok, path, n_path, n_rows_out=None, mass=None, stream=None):
         """tria_accept: device int32 path [caches or 1][entries] and n_path [caches or 1]."""
-        _tensor(path, "path", ("int32",), 2)
-        own = path.shape[0] > 1 or view.n_layer == 1
-        if path.shape[0] not in (1, view.n_layer) or n_path.numel() != path.shape[0] or path.stride(1) != 1 and path.shape[1] > 1:
-            raise ValueError("path must be [caches or 1][entries], n_path [caches or 1]")
-        if path.shape[1] < n_tok:
-            raise ValueError(f"path holds {path.shape[1]} entries a cache: room for n_tok = {n_tok} is wanted")
+        i32 = _torch().int32
+        if path.dtype != i32 or path.dim() != 2 or n_path.dtype != i32 or not n_path.is_contiguous():
+            raise ValueError("path must be an int32 [caches or 1][entries], n_path a contiguous int32 [caches or 1]")
+        lists, entries = path.shape
+        if lists not in (1, view.n_layer) or n_path.numel() != lists or (path.stride(1) != 1 and entries > 1):
+            raise ValueError("path must be [caches or 1][entries], its rows contiguous, n_path [caches or 1]")
+        if entries < n_tok:
+            raise ValueError(f"path holds {entries} entries a cache: room for n_tok = {n_tok} is wanted")
         self._mass(mass, view)
         self._here(path, n_path, mass)
-        self._counts(view, n_rows, *(() if n_rows_out is None else (n_rows_out,)))
-        if str(n_path.dtype) != "torch.int32" or not n_path.is_contiguous():
-            raise ValueError("n_path must be a contiguous int32 tensor")
-        check(lib().tria_accept(self.h, C.byref(view), _ptr(n_rows), int(n_tok), _ptr(path),
-                                path.stride(0) if own and view.n_layer > 1 else 0, _ptr(n_path), _ptr(mass),
-                                _ptr(n_rows if n_rows_out is None else n_rows_out), _stream(stream)))
+        rows_out = n_rows if n_rows_out is None else n_rows_out
+        self._counts(view, n_rows, rows_out)
+        check(lib().tria_accept(self.h, C.byref(view), n_rows.data_ptr(), n_tok, path.data_ptr(),
+                                path.stride(0) if lists > 1 else 0, n_path.data_ptr(), _ptr(mass), rows_out.data_ptr(),
+                                _stream(stream)))
 
     def evict_mass(self, src, dst, n_rows, mass, mass_dst, params, n_kept_out=None, stream=None):
         """tria_evict_mass: one eviction step ranked by device `mass`
@@ -621,14 +634,15 @@ class Context:
     def _here(self, *tensors):
         """Tensors that kernels read or write must live on the context's device."""
         for x in tensors:
-            if x is not None and (not x.is_cuda or x.get_device() != self.device):
+            if x is not None and x.get_device() != self.device:
                 raise ValueError(f"a tensor on {x.device} was given to a context of cuda:{self.device}")
 
     def _counts(self, view, *counts):
+        i32, units = _torch().int32, view.n_layer * view.n_head_kv
         for x in counts:
-            if str(x.dtype) != "torch.int32" or not x.is_contiguous() or x.numel() != view.n_layer * view.n_head_kv:
-                raise ValueError(f"row counts must be a contiguous int32 tensor of {view.n_layer} x {view.n_head_kv}")
-        self._here(*counts)
+            if x.dtype != i32 or x.numel() != units or not x.is_contiguous() or x.get_device() != self.device:
+                raise ValueError(f"row counts must be a contiguous int32 tensor of {view.n_layer} x {view.n_head_kv} on "
+                                 f"cuda:{self.device}")
 
     @staticmethod
     def _shared_or_own(x, name, shape, caches):
@@ -637,6 +651,6 @@ class Context:
 
     @staticmethod
     def _mass(x, view):
-        if x is not None and (str(x.dtype) != "torch.float32" or not x.is_contiguous()
-                              or tuple(x.shape) != (view.n_layer, view.n_head_kv, view.n_cells)):
+        if x is not None and (x.dtype != _torch().float32 or x.shape != (view.n_layer, view.n_head_kv, view.n_cells)
+                              or not x.is_contiguous()):
             raise ValueError(f"mass must be a contiguous fp32 [{view.n_layer}][{view.n_head_kv}][{view.n_cells}] tensor")
