@@ -46,6 +46,7 @@ struct AttendArgs {
     float2 *part_ml;                     /* [2 * grid][rows] */
     int32_t *arrived;                    /* [grid]: by the first block of an item (one such item a block); zero between calls */
     float2 *norm;                        /* [n_layer * n_head_kv][T * G]: (max, 1 / sum) of each query row, or NULL */
+    int32_t *redo;                       /* [0] how many, then query rows (unit * T * G + r) to do again one by one */
     float *scores;                       /* [n_layer * n_head_kv][T * G][score_stride], or NULL */
     int64_t score_stride;
 };
@@ -90,7 +91,7 @@ constexpr float LN2 = 0.6931471805599453f;
  * large arguments need and too little where tanh u is small; there the series
  * u (1 - z/3 + 2 z^2/15 - ...), z = u^2, whose first omitted term is below
  * 2^-27 at |u| = 0.4. */
-__device__ __forceinline__ float tanh_both(float u) {
+__device__ __forceinline__ float tanh_small(float u) {
     const float z = u * u;
     float s = 21844.0f / 6081075.0f;
     s = fmaf(s, z, -1382.0f / 155925.0f);
@@ -98,9 +99,11 @@ __device__ __forceinline__ float tanh_both(float u) {
     s = fmaf(s, z, -17.0f / 315.0f);
     s = fmaf(s, z, 2.0f / 15.0f);
     s = fmaf(s, z, -1.0f / 3.0f);
-    s = fmaf(s * z, u, u);
+    return fmaf(s * z, u, u);
+}
+__device__ __forceinline__ float tanh_both(float u) {
     const float b = fmaf(-2.0f, rcp(1.0f + ex2(2.0f * LOG2E * u)), 1.0f);
-    return fabsf(u) < 0.4f ? s : b;
+    return fabsf(u) < 0.4f ? tanh_small(u) : b;
 }
 
 /* The call's score transform in the base-2 exponent: x = log2(e) s. */
@@ -213,12 +216,13 @@ __device__ void attend_row(const AttendArgs &a, int u, int g, int t, RowShared<H
 /* ------------------------------------------------------------------ */
 
 /* Query rows r = t * G + g of a unit are taken in groups of `rows`; an item is
- * (unit, group).  An item walks steps of ATT_STEP cache rows: all rows up to
+ * (unit, group).  An item walks steps of `step` cache rows: all rows up to
  * the last that its tokens see by order, or, with a window, the rows before
  * `head` (where the sink ends) and those from `tail` on (where the window
  * begins).  Positions need not ascend: head and tail enclose every row that
  * the window admits. */
-constexpr int ATT_STEP = 64;
+constexpr int ATT_STEP = 64;           /* few query rows */
+constexpr int TILE_STEP = 128;         /* many */
 
 /* Rows of the unit that the group's last token can see by order. */
 __device__ __forceinline__ int item_rows(const AttendArgs &a, int u, int grp, int rows) {
@@ -227,9 +231,9 @@ __device__ __forceinline__ int item_rows(const AttendArgs &a, int u, int grp, in
     return max(0, a.tree ? n : min(n, n - a.T + r1 / a.G + 1));
 }
 
-__device__ __forceinline__ int span_steps(int n, int2 s) {
-    const int hs = (s.x + ATT_STEP - 1) / ATT_STEP;
-    return hs + (n > s.y ? (n - s.y + ATT_STEP - 1) / ATT_STEP : 0);
+__device__ __forceinline__ int span_steps(int n, int2 s, int step) {
+    const int hs = (s.x + step - 1) / step;
+    return hs + (n > s.y ? (n - s.y + step - 1) / step : 0);
 }
 
 constexpr int PLAN_THREADS = 512;
@@ -256,10 +260,11 @@ __device__ __forceinline__ int block_scan(int v, int *s_warp, int threads, int *
 
 /* With a window: block `it` finds its item's span.  The last block to finish
  * (the only one without a window) scans the items' steps. */
-__global__ void __launch_bounds__(PLAN_THREADS) k_attend_plan(const AttendArgs a, int rows, int items, int2 *span,
+__global__ void __launch_bounds__(PLAN_THREADS) k_attend_plan(const AttendArgs a, int rows, int step, int items, int2 *span,
                                                               int32_t *steps, int32_t *done) {
     __shared__ int s_min[PLAN_THREADS / 32], s_max[PLAN_THREADS / 32], s_last;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if (a.redo && blockIdx.x == 0 && threadIdx.x == 0) a.redo[0] = 0;
     if (span) {
         const int it = blockIdx.x, u = it / a.groups, grp = it - u * a.groups, l = u / a.n_head_kv;
         const int n = item_rows(a, u, grp, rows);
@@ -285,7 +290,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_attend_plan(const AttendArgs a
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int i = 1; i < PLAN_THREADS / 32; i++) { tail = min(tail, s_min[i]); head = max(head, s_max[i]); }
-            tail = tail / ATT_STEP * ATT_STEP;
+            tail = tail / step * step;
             if (head >= tail) { head = 0; tail = 0; }         /* one run of rows */
             span[it] = make_int2(head, tail);
             __threadfence();
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_attend_plan(const AttendArgs a
         if (it < items) {
             const int u = it / a.groups, grp = it - u * a.groups, n = item_rows(a, u, grp, rows);
             const int2 s = span ? __ldcg(&span[it]) : make_int2(0, 0);
-            st = span_steps(n, make_int2(min(s.x, n), s.y));
+            st = span_steps(n, make_int2(min(s.x, n), s.y), step);
         }
         const int incl = block_scan(st, s_min, PLAN_THREADS, &sum);
         if (it < items) steps[it] = base + incl;

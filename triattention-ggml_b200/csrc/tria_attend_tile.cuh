@@ -1,0 +1,705 @@
+/*
+ * tria_attend_tile.cuh - attention of many query rows over a ragged cache on
+ * the tcgen05 tensor cores.
+ *
+ * A block takes up to 256 query rows of a unit as two row tiles of 128 and
+ * walks 128 cache rows a step: S = Q K^T into tensor memory, one thread per
+ * query row turns its row of S into weights P (written over S as f16), and
+ * O += P V accumulates in tensor memory.  While one row tile is at its
+ * exponentials, the other one's products run.
+ */
+#pragma once
+
+#include "tria_attend.cuh"
+
+namespace tria {
+
+/* ------------------------------------------------------------------ */
+/* tcgen05 and its descriptors                                          */
+/* ------------------------------------------------------------------ */
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+/* The barrier completes when every product this thread issued so far has. */
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+/* Operand in shared memory as panels of 64 f16 columns: row r of a panel is the
+ * 128 bytes at 128 r, its 16-byte chunks XORed with r mod 8 (128-byte swizzle).
+ * `lead` is the byte step between panels where the columns are the operand's
+ * row dimension (V), unused otherwise; eight rows are 1024 bytes on. */
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+/* Instruction descriptor: fp32 sums, f16 operands, M = 128, B by rows (K) or by columns (V). */
+__host__ __device__ constexpr uint32_t tile_idesc(int n, bool b_by_column) {
+    return 1u << 4 | (b_by_column ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+#define TC_R8(x, o) "=r"(x[o]), "=r"(x[o + 1]), "=r"(x[o + 2]), "=r"(x[o + 3]), "=r"(x[o + 4]), "=r"(x[o + 5]), "=r"(x[o + 6]), "=r"(x[o + 7])
+#define TC_I8(x, o) "r"(x[o]), "r"(x[o + 1]), "r"(x[o + 2]), "r"(x[o + 3]), "r"(x[o + 4]), "r"(x[o + 5]), "r"(x[o + 6]), "r"(x[o + 7])
+/* 32 columns of the warp's 32 lanes: a thread gets (gives) its lane's. */
+__device__ __forceinline__ void tc_ld32(uint32_t (&x)[32], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : TC_R8(x, 0), TC_R8(x, 8), TC_R8(x, 16), TC_R8(x, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&x)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                 "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+                 ::TC_I8(x, 0), TC_I8(x, 8), TC_I8(x, 16), TC_I8(x, 24), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t (&x)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+                 ::TC_I8(x, 0), TC_I8(x, 8), "r"(addr) : "memory");
+}
+
+/* ------------------------------------------------------------------ */
+/* Layout                                                               */
+/* ------------------------------------------------------------------ */
+
+constexpr int TILE_Q = 128, TILE_ROWS = 2 * TILE_Q, TILE_K = 128;
+static_assert(TILE_K == TILE_STEP, "plan");
+constexpr int TILE_SOFT = 2 * TILE_Q;                    /* threads of the two weight groups */
+
+/* q8_0 rows become two f16 operands, the rounded value and what the rounding
+ * left, so a product keeps the stored value's 19 bits. */
+template <int KT, int HD>
+struct TileLayout {
+    static constexpr int PARTS = KT == KT_F16 ? 1 : 2;
+    static constexpr int STAGES = KT == KT_F16 ? 2 : 1;
+    static constexpr int LOADERS = KT == KT_F16 ? 128 : 224;
+    static constexpr int THREADS = TILE_SOFT + 32 + LOADERS;
+    static constexpr int PANEL = TILE_K * 128;           /* 128 rows of 64 f16 */
+    static constexpr int SIDE = HD / 64 * PANEL;         /* one operand of one tile */
+    static constexpr int Q = 0;
+    static constexpr int K = Q + 2 * SIDE, V = K + STAGES * PARTS * SIDE;
+    static constexpr int POS = V + STAGES * PARTS * SIDE;         /* int32 [STAGES][128] */
+    static constexpr int BYTES = POS + STAGES * TILE_K * 4 + 1024;    /* 1024: the panels start on a multiple of it */
+};
+
+/* ------------------------------------------------------------------ */
+/* Kernel                                                               */
+/* ------------------------------------------------------------------ */
+
+/* Where a block's walk stands: each role follows the same segments. */
+struct TileWalk {
+    int64_t at, end, base;
+    int it, i0, i1;
+    bool first;
+};
+__device__ __forceinline__ void tile_walk_start(TileWalk &w, const int32_t *steps, int items, int64_t total, int grid, int b) {
+    w.at = b * total / grid;
+    w.end = (b + 1) * total / grid;
+    w.it = 0;
+    w.first = true;
+    int lo = 0, hi = items;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (steps[mid] <= w.at) lo = mid + 1;
+        else hi = mid;
+    }
+    w.it = lo;
+}
+__device__ __forceinline__ bool tile_walk_segment(TileWalk &w, const int32_t *steps) {
+    if (w.at >= w.end) return false;
+    while (steps[w.it] <= w.at) w.it++;
+    w.base = w.it ? steps[w.it - 1] : 0;
+    w.i0 = (int)(w.at - w.base);
+    w.i1 = (int)(min(w.end, (int64_t)steps[w.it]) - w.base);
+    return true;
+}
+__device__ __forceinline__ void tile_walk_next(TileWalk &w) {
+    w.at = w.base + w.i1;
+    w.first = false;
+}
+
+/* One thread's wait on a pipeline barrier: false when it gave up or another
+ * role did, with the status set. */
+__device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volatile int *s_abort, int32_t *status) {
+    if (mbar_try(bar, parity)) return true;
+    if (*s_abort || !mbar_wait(bar, parity)) {
+        *s_abort = 1;
+        atomicOr(status, ST_TIMEOUT);
+        return false;
+    }
+    return true;
+}
+
+/* A q8_0 block's 32 values from p (2-byte aligned) as f16 pairs, the value
+ * rounded (hi) and its remainder (lo = q d - hi, exact in one f16 fma). */
+__device__ __forceinline__ void dequant_block(const uint8_t *p, uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+    uint32_t w[8];
+    __half d;
+    if (((uintptr_t)p & 2) == 0) {
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+        uint32_t x = __ldg(q);
+        d = __ushort_as_half((unsigned short)x);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t y = i < 7 ? __ldg(q + i + 1) : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(q + 8));
+            w[i] = __funnelshift_r(x, y, 16);
+            x = y;
+        }
+    } else {
+        d = __ushort_as_half(__ldg(reinterpret_cast<const uint16_t *>(p)));
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(p + 2);
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = __ldg(q + i);
+    }
+    const __half2 dd = __half2half2(d);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        uint32_t x[2];
+        int8x4_half(w[i], x[0], x[1]);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const __half2 q = *reinterpret_cast<const __half2 *>(&x[j]);
+            const __half2 h = __hmul2(q, dd), r = __hfma2(q, dd, __hneg2(h));
+            hi[2 * i + j] = *reinterpret_cast<const uint32_t *>(&h);
+            lo[2 * i + j] = *reinterpret_cast<const uint32_t *>(&r);
+        }
+    }
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+/* Byte offset of 16-byte chunk c (of a row's HD / 8) of row r in an operand. */
+__device__ __forceinline__ uint32_t tile_chunk(int r, int c) { return (c >> 3) * (TILE_K * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+
+/* Starts (f16) or does (q8_0) the copy of rows [r0, r0 + 128) of one side;
+ * rows at and behind n become zeros. */
+template <int KT, int HD>
+__device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p, int r0, int n, uint32_t st, int x) {
+    using L = TileLayout<KT, HD>;
+    if constexpr (KT == KT_F16) {
+        constexpr int CH = HD / 8, RPI = L::LOADERS / CH;
+        if (a.copy16) {
+            const int r = x / CH, c = x % CH;
+            const uint32_t d = st + tile_chunk(r, c);           /* RPI is a multiple of 8: the swizzle stays */
+            const uint8_t *s = p + (int64_t)(r0 + r) * a.cell_stride + 16 * c;
+            const int64_t step = (int64_t)RPI * a.cell_stride;
+            if (r0 + TILE_K <= n) {
+#pragma unroll
+                for (int i = 0; i < TILE_K / RPI; i++) {
+                    cp_async16(d + i * RPI * 128, s, 16u);
+                    s += step;
+                }
+            } else {
+                for (int i = 0; i < TILE_K / RPI; i++) {
+                    const bool in = r0 + r + i * RPI < n;
+                    cp_async16(d + i * RPI * 128, in ? s + i * step : p, in ? 16u : 0u);
+                }
+            }
+        } else {
+            for (int y = x; y < TILE_K * CH * 4; y += L::LOADERS) {
+                const int r = y / (CH * 4), c = y / 4 % CH, q = y & 3;
+                const bool in = r0 + r < n;
+                cp_async4(st + tile_chunk(r, c) + 4 * q, p + (in ? (int64_t)(r0 + r) * a.cell_stride + 16 * c + 4 * q : 0), in ? 4u : 0u);
+            }
+        }
+    } else {
+        constexpr int NB = HD / 32;
+#pragma unroll 1
+        for (int y = x; y < TILE_K * NB; y += L::LOADERS) {
+            const int r = y / NB, b = y % NB;
+            uint32_t hi[16], lo[16];
+            if (r0 + r < n) {
+                dequant_block(p + (int64_t)(r0 + r) * a.cell_stride + 34 * b, hi, lo);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) hi[i] = lo[i] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t d = st + tile_chunk(r, 4 * b + i);
+                sts128(d, hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+                sts128(d + L::SIDE, lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+            }
+        }
+    }
+}
+
+template <int KT, int HD, bool EXTRA>
+__global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(const AttendArgs a) {
+    using L = TileLayout<KT, HD>;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t b_q_full, b_q_free, b_o_full, b_s_full[2], b_p_ready[2];
+    __shared__ __align__(8) uint64_t b_k_full[L::STAGES], b_k_free[L::STAGES], b_v_full[L::STAGES], b_v_free[L::STAGES];
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_abort;
+    __shared__ int s_last;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int32_t *s_pos = reinterpret_cast<const int32_t *>(smem_raw + (smem - smem_u32(smem_raw)) + L::POS);
+    const int units = a.n_layer * a.n_head_kv, items = units * a.groups, R = a.T * a.G;
+    const int32_t *steps = a.steps;
+    const int64_t total = steps[items - 1];
+    const int b = blockIdx.x, grid = (int)min((int64_t)gridDim.x, total);
+    const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
+
+    if (tid == 0) {
+        mbar_init(&b_q_full, L::LOADERS);
+        mbar_init(&b_q_free, 1);
+        mbar_init(&b_o_full, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&b_s_full[i], 1);
+            mbar_init(&b_p_ready[i], TILE_Q);
+        }
+        for (int i = 0; i < L::STAGES; i++) {
+            mbar_init(&b_k_full[i], L::LOADERS);
+            mbar_init(&b_v_full[i], L::LOADERS);
+            mbar_init(&b_k_free[i], 1);
+            mbar_init(&b_v_free[i], 1);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (w == TILE_SOFT / 32) {                                /* the product warp owns the tensor memory */
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    /* columns: S (and P) of tile x at 128 x, O at 256 + 128 x */
+
+    TileWalk wk;
+    if (b < grid) tile_walk_start(wk, steps, items, total, grid, b);
+    else wk.at = wk.end = 0;
+
+    if (w > TILE_SOFT / 32) {
+        /* ---------------- loaders ---------------- */
+        const int x = tid - TILE_SOFT - 32;
+        uint32_t kc = 0, vc = 0;
+        uint64_t *pending = nullptr;                          /* the copy still to be announced */
+        auto announce = [&]() {
+            fence_async_smem();
+            mbar_arrive(pending);
+            pending = nullptr;
+        };
+        auto wait_free = [&](uint64_t *bar, uint32_t parity) -> bool {
+            if (mbar_try(bar, parity)) return true;
+            if (pending) {                                    /* nobody may wait for it while we wait */
+                cp_async_wait<0>();
+                announce();
+            }
+            return tile_wait(bar, parity, &s_abort, a.status);
+        };
+        auto issued = [&](uint64_t *bar) {
+            cp_async_commit();
+            if (KT != KT_F16) {                               /* the rows were converted, not copied */
+                cp_async_wait<0>();
+                if (pending) announce();
+                pending = bar;
+                announce();
+            } else {
+                if (pending) {
+                    cp_async_wait<1>();
+                    announce();
+                }
+                pending = bar;
+            }
+        };
+        bool ok = true;
+        for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+            const int u = wk.it / a.groups, grp = wk.it - u * a.groups, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
+            const int n = attend_rows(a, u);
+            const int2 span = a.span ? a.span[wk.it] : make_int2(0, 0);
+            const int hs = (min(span.x, n) + TILE_K - 1) / TILE_K;
+            const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
+            const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
+            if (seg && !wait_free(&b_q_free, (seg - 1) & 1)) break;
+            for (int y = x; y < TILE_ROWS * (HD / 8); y += L::LOADERS) {
+                const int q = y / (HD / 8), c = y % (HD / 8), r = grp * TILE_ROWS + q;
+                const __half *s = a.q + l * a.q_cache;
+                if (r < R) s += (r / a.G) * a.q_tok + (h * a.G + r % a.G) * a.q_head + 8 * c;
+                cp_async16(smem + L::Q + (q / TILE_Q) * L::SIDE + tile_chunk(q % TILE_Q, c), s, r < R ? 16u : 0u);
+            }
+            issued(&b_q_full);
+            for (int i = wk.i0; i < wk.i1; i++) {
+                const int row0 = i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K;
+                const int ks = kc % L::STAGES, vs = vc % L::STAGES;
+                if (kc >= L::STAGES && !wait_free(&b_k_free[ks], (kc / L::STAGES - 1) & 1)) { ok = false; break; }
+                tile_load<KT, HD>(a, k, row0, n, smem + L::K + ks * L::PARTS * L::SIDE, x);
+                issued(&b_k_full[ks]);
+                kc++;
+                if (vc >= L::STAGES && !wait_free(&b_v_free[vs], (vc / L::STAGES - 1) & 1)) { ok = false; break; }
+                tile_load<KT, HD>(a, v, row0, n, smem + L::V + vs * L::PARTS * L::SIDE, x);
+                if (want_pos && x < TILE_K) {                 /* with V: free once the weights are made */
+                    const bool in = row0 + x < n;
+                    cp_async4(smem + L::POS + (vs * TILE_K + x) * 4, pos + (in ? row0 + x : 0), in ? 4u : 0u);
+                }
+                issued(&b_v_full[vs]);
+                vc++;
+            }
+        }
+        cp_async_wait<0>();
+        if (pending) announce();
+    } else if (w == TILE_SOFT / 32) {
+        /* ---------------- products ---------------- */
+        if (lane == 0) {
+            constexpr uint32_t qk = tile_idesc(TILE_K, false), pv = tile_idesc(HD, true);
+            uint32_t kc = 0, vc = 0, pc[2] = {0, 0};
+            bool ok = true;
+            for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+                const int grp = wk.it % a.groups, N = wk.i1 - wk.i0;
+                const int tiles = R - grp * TILE_ROWS > TILE_Q ? 2 : 1;
+                if (!tile_wait(&b_q_full, seg & 1, &s_abort, a.status)) break;
+                for (int i = 0; ok && i <= N; i++) {
+                    if (i < N && !tile_wait(&b_k_full[kc % L::STAGES], (kc / L::STAGES) & 1, &s_abort, a.status)) { ok = false; break; }
+                    if (i > 0 && !tile_wait(&b_v_full[vc % L::STAGES], (vc / L::STAGES) & 1, &s_abort, a.status)) { ok = false; break; }
+                    for (int x = 0; x < tiles; x++) {
+                        if (i > 0) {
+                            if (!tile_wait(&b_p_ready[x], pc[x] & 1, &s_abort, a.status)) { ok = false; break; }
+                            pc[x]++;
+                            tc_fence_after();
+                            const uint32_t vb = smem + L::V + (vc % L::STAGES) * L::PARTS * L::SIDE;
+#pragma unroll
+                            for (int part = 0; part < L::PARTS; part++)
+#pragma unroll
+                                for (int s = 0; s < TILE_K / 16; s++)
+                                    tc_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * s, tile_desc(vb + part * L::SIDE + s * 2048, L::PANEL),
+                                              pv, i > 1 || part > 0 || s > 0);
+                        }
+                        if (i < N) {
+                            const uint32_t qb = smem + L::Q + x * L::SIDE, kb = smem + L::K + (kc % L::STAGES) * L::PARTS * L::SIDE;
+#pragma unroll
+                            for (int part = 0; part < L::PARTS; part++)
+#pragma unroll
+                                for (int s = 0; s < HD / 16; s++) {
+                                    const uint32_t off = (s / 4) * L::PANEL + (s % 4) * 32;
+                                    tc_mma_ss(tmem + 128 * x, tile_desc(qb + off, 16), tile_desc(kb + part * L::SIDE + off, 16), qk,
+                                              part > 0 || s > 0);
+                                }
+                            tc_commit(&b_s_full[x]);
+                        }
+                    }
+                    if (!ok) break;
+                    if (i > 0) tc_commit(&b_v_free[vc++ % L::STAGES]);
+                    if (i < N) tc_commit(&b_k_free[kc++ % L::STAGES]);
+                }
+                if (!ok) break;
+                tc_commit(&b_o_full);
+                tc_commit(&b_q_free);
+            }
+        }
+        __syncwarp();
+    } else {
+        /* ---------------- weights ---------------- */
+        const int x = w >> 2, row = tid & (TILE_Q - 1);       /* row tile, query row in it */
+        const uint32_t mine = tmem + ((uint32_t)(w & 3) << 21);      /* lanes 32 (w mod 4) on */
+        const uint32_t S = mine + 128 * x, O = mine + 256 + 128 * x;
+        const ScoreMap map(a);
+        uint32_t sc = 0, tiles = 0;                           /* scores seen, tiles of the segments before */
+        bool ok = true;
+
+        /* items without a row to see */
+        for (int it = b; it < items; it += gridDim.x) {
+            if (steps[it] != (it ? steps[it - 1] : 0)) continue;
+            const int u = it / a.groups, grp = it - u * a.groups, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
+            for (int y = tid; y < TILE_ROWS * HD / 8; y += TILE_SOFT) {
+                const int r = grp * TILE_ROWS + y / (HD / 8);
+                if (r >= R) break;
+                *reinterpret_cast<uint4 *>(a.out + l * a.o_cache + (r / a.G) * a.o_tok + (h * a.G + r % a.G) * a.o_head +
+                                           y % (HD / 8) * 8) = make_uint4(0, 0, 0, 0);
+            }
+            const int r = grp * TILE_ROWS + tid;
+            if (r < R) {
+                if (a.lse) a.lse[((int64_t)l * a.T + r / a.G) * a.n_head_kv * a.G + h * a.G + r % a.G] = -INFINITY;
+                if (a.norm) a.norm[(int64_t)u * R + r] = make_float2(0.0f, 0.0f);
+            }
+        }
+
+        for (uint32_t seg = 0; tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+            const int u = wk.it / a.groups, grp = wk.it - u * a.groups, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
+            const int n = attend_rows(a, u);
+            const int rows = min(TILE_ROWS, R - grp * TILE_ROWS);
+            const bool active = x == 0 || rows > TILE_Q;
+            const int2 span = a.span ? a.span[wk.it] : make_int2(0, 0);
+            const int hs = (min(span.x, n) + TILE_K - 1) / TILE_K;
+            const int r = grp * TILE_ROWS + x * TILE_Q + row;
+            const bool in = r < R;
+            const int t = in ? r / a.G : -1, head = h * a.G + r % a.G;
+            const int tp = in && want_pos ? a.tok_pos[l * a.tok_pos_stride + t] : 0;
+            const float slope2 = EXTRA && in && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
+            const int64_t lo = (int64_t)tp - a.window;
+            const int seen_end = in ? n - a.T + t + 1 : 0;    /* causal: rows before it are seen */
+            float m = -INFINITY, sum = 0.0f;
+            for (int i = wk.i0; active && i < wk.i1; i++) {
+                const int j0 = i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K;
+                const uint32_t tc = tiles + (i - wk.i0);
+                if (!tile_wait(&b_s_full[x], sc & 1, &s_abort, a.status)) ok = false;
+                if (want_pos && ok && !tile_wait(&b_v_full[tc % L::STAGES], (tc / L::STAGES) & 1, &s_abort, a.status)) ok = false;
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                sc++;
+                tc_fence_after();
+                const bool all = j0 + TILE_K <= n - a.T && (!EXTRA || a.window <= 0);
+                const bool rewrite = EXTRA || !all;           /* the scores are made final in tensor memory first */
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < TILE_K / 32; c++) {
+                    uint32_t v[32];
+                    tc_ld32(v, S + 32 * c);
+                    tc_wait_ld();
+                    if (!rewrite) {
+                        float hi = -INFINITY;
+                        if (map.scale >= 0.0f) {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) hi = fmaxf(hi, __uint_as_float(v[e]));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) hi = fmaxf(hi, -__uint_as_float(v[e]));
+                        }
+                        top = fmaxf(top, hi);
+                    } else {
+                        if (EXTRA && map.cap > 0.0f) {
+                            float far = 0.0f;
+#pragma unroll
+                            for (int e = 0; e < 32; e++) {
+                                const float y = __uint_as_float(v[e]) * map.scale;
+                                v[e] = __float_as_uint(y);
+                                far = fmaxf(far, fabsf(y));
+                            }
+                            if (__any_sync(0xffffffffu, !(far < 0.4f))) {
+#pragma unroll
+                                for (int e = 0; e < 32; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; e++) v[e] = __float_as_uint(map.cap * tanh_small(__uint_as_float(v[e])));
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
+                        }
+                        if (want_pos) {
+                            const int32_t *ps = s_pos + (tc % L::STAGES) * TILE_K + 32 * c;
+#pragma unroll
+                            for (int e = 0; e < 32; e++) {
+                                const int pj = ps[e];
+                                float y = fmaf(-slope2, (float)(tp - pj), __uint_as_float(v[e]));
+                                if (a.window > 0 && !(pj >= lo || pj < a.sink)) y = -INFINITY;
+                                v[e] = __float_as_uint(y);
+                            }
+                        }
+                        const int e0 = j0 + 32 * c;
+                        if (e0 + 32 > n - a.T) {
+                            if (!a.tree) {
+#pragma unroll
+                                for (int e = 0; e < 32; e++)
+                                    if (e0 + e >= seen_end) v[e] = 0xff800000u;
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; e++) {
+                                    const int own = e0 + e - (n - a.T);
+                                    bool see = in && e0 + e < n;
+                                    if (see && own >= 0)
+                                        see = a.tree[l * a.tree_stride + (int64_t)t * a.tree_words + (own >> 5)] >> (own & 31) & 1u;
+                                    if (!see) v[e] = 0xff800000u;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(v[e]));
+                        tc_st32(S + 32 * c, v);
+                    }
+                }
+                if (rewrite) tc_wait_st();
+                else top *= fabsf(map.scale);
+                const bool up = top > m + FEW_SLACK;
+                if (__any_sync(0xffffffffu, up)) {
+                    const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
+                    m = to;
+                    sum *= f;
+                    if (i > wk.i0) {                          /* the sums so far: their products are done when S is */
+#pragma unroll 1
+                        for (int c = 0; c < HD / 32; c++) {
+                            uint32_t v[32];
+                            tc_ld32(v, O + 32 * c);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            tc_st32(O + 32 * c, v);
+                        }
+                    }
+                }
+                const float from = m == -INFINITY ? 0.0f : m - FEW_LIFT, mul = rewrite ? 1.0f : map.scale;
+#pragma unroll
+                for (int c = 0; c < TILE_K / 32; c++) {
+                    uint32_t v[32], p[16];
+                    tc_ld32(v, S + 32 * c);
+                    tc_wait_ld();
+                    float part[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float p0 = ex2(fmaf(__uint_as_float(v[2 * e]), mul, -from));
+                        const float p1 = ex2(fmaf(__uint_as_float(v[2 * e + 1]), mul, -from));
+                        part[0] += p0;
+                        part[1] += p1;
+                        p[e] = pack_half2(p0, p1);
+                    }
+                    sum += part[0] + part[1];
+                    tc_st16(S + 16 * c, p);                   /* over scores already read */
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&b_p_ready[x]);
+            }
+            if (!ok) break;
+            if (!tile_wait(&b_o_full, seg & 1, &s_abort, a.status)) ok = false;
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+
+            const int64_t base = wk.base;
+            const int c0 = (int)(((base + 1) * grid - 1) / total), c1 = (int)(((int64_t)steps[wk.it] * grid - 1) / total);
+            if (c0 == c1) {
+                const bool none = sum == 0.0f;
+                const float inv = none ? 0.0f : 1.0f / sum;
+                bool bad = false;
+                if (active) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t v[32];
+                        tc_ld32(v, O + 32 * c);
+                        tc_wait_ld();
+                        float fin = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            const float y = none ? 0.0f : __uint_as_float(v[e]) * inv;
+                            fin += y * 0.0f;
+                            v[e] = __float_as_uint(y);
+                        }
+                        bad |= fin != 0.0f;                   /* NaN: some value is not finite */
+                        if (in) {
+                            uint4 *d = reinterpret_cast<uint4 *>(a.out + l * a.o_cache + t * a.o_tok + head * a.o_head + 32 * c);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                d[e] = make_uint4(pack_half2(__uint_as_float(v[8 * e]), __uint_as_float(v[8 * e + 1])),
+                                                  pack_half2(__uint_as_float(v[8 * e + 2]), __uint_as_float(v[8 * e + 3])),
+                                                  pack_half2(__uint_as_float(v[8 * e + 4]), __uint_as_float(v[8 * e + 5])),
+                                                  pack_half2(__uint_as_float(v[8 * e + 6]), __uint_as_float(v[8 * e + 7])));
+                        }
+                    }
+                    if (in) {
+                        if (a.lse) a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + head] = none ? -INFINITY : (m - FEW_LIFT + log2f(sum)) * LN2;
+                        if (a.norm) a.norm[(int64_t)u * R + r] = none ? make_float2(0.0f, 0.0f) : make_float2(m - FEW_LIFT, inv);
+                        if (bad) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + r;
+                    }
+                }
+            } else {
+                const int slot = 2 * b + (wk.first ? 0 : 1);
+                if (active) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t v[32];
+                        tc_ld32(v, O + 32 * c);
+                        tc_wait_ld();
+                        if (in) {
+                            uint4 *d = reinterpret_cast<uint4 *>(a.part_o + ((int64_t)slot * TILE_ROWS + x * TILE_Q + row) * HD + 32 * c);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) d[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                        }
+                    }
+                    if (in) a.part_ml[(int64_t)slot * TILE_ROWS + x * TILE_Q + row] = make_float2(m, sum);
+                }
+                __threadfence();
+                asm volatile("bar.sync 1, %0;" ::"n"(TILE_SOFT) : "memory");
+                if (tid == 0) s_last = atomicAdd(&a.arrived[c0], 1) == c1 - c0;
+                asm volatile("bar.sync 1, %0;" ::"n"(TILE_SOFT) : "memory");
+                if (s_last) {
+                    __threadfence();
+                    if (tid == 0) a.arrived[c0] = 0;
+                    const int s0 = 2 * c0 + (c0 * total / grid >= base ? 0 : 1);
+                    constexpr int LPR = HD / 4, RPP = TILE_SOFT / LPR;
+                    const int dim = tid % LPR * 4;
+                    for (int q = tid / LPR; q < rows; q += RPP) {
+                        auto slot_of = [&](int s) { return ((int64_t)(s == 0 ? s0 : 2 * (c0 + s)) * TILE_ROWS + q); };
+                        float mm = -INFINITY, ss = 0.0f;
+                        for (int s = 0; s <= c1 - c0; s++) mm = fmaxf(mm, __ldcg(&a.part_ml[slot_of(s)]).x);
+                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                        for (int s = 0; s <= c1 - c0; s++) {
+                            const float2 y = __ldcg(&a.part_ml[slot_of(s)]);
+                            const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part_o + slot_of(s) * HD + dim));
+                            const float g = y.x == -INFINITY ? 0.0f : ex2(y.x - mm);
+                            ss = fmaf(y.y, g, ss);
+                            if (g != 0.0f) {
+                                acc.x = fmaf(o.x, g, acc.x);
+                                acc.y = fmaf(o.y, g, acc.y);
+                                acc.z = fmaf(o.z, g, acc.z);
+                                acc.w = fmaf(o.w, g, acc.w);
+                            }
+                        }
+                        const bool none = ss == 0.0f;
+                        const float inv = none ? 0.0f : 1.0f / ss;
+                        if (none) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        acc.x *= inv;
+                        acc.y *= inv;
+                        acc.z *= inv;
+                        acc.w *= inv;
+                        const int rq = grp * TILE_ROWS + q, tq = rq / a.G, hq = h * a.G + rq % a.G;
+                        *reinterpret_cast<uint2 *>(a.out + l * a.o_cache + tq * a.o_tok + hq * a.o_head + dim) =
+                            make_uint2(pack_half2(acc.x, acc.y), pack_half2(acc.z, acc.w));
+                        const bool bad = (acc.x + acc.y + acc.z + acc.w) * 0.0f != 0.0f;
+                        /* one entry a row: the first of its lanes that saw it */
+                        const unsigned group = LPR == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
+                        const unsigned who = __ballot_sync(group, bad) & group;
+                        if (bad && lane == __ffs(who) - 1) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + rq;
+                        if (dim == 0) {
+                            if (a.lse) a.lse[((int64_t)l * a.T + tq) * a.n_head_kv * a.G + hq] = none ? -INFINITY : (mm - FEW_LIFT + log2f(ss)) * LN2;
+                            if (a.norm) a.norm[(int64_t)u * R + rq] = none ? make_float2(0.0f, 0.0f) : make_float2(mm - FEW_LIFT, inv);
+                        }
+                    }
+                }
+            }
+            tiles += wk.i1 - wk.i0;
+            /* s_last is read before it is set again, and a group without rows stays with the other */
+            asm volatile("bar.sync 1, %0;" ::"n"(TILE_SOFT) : "memory");
+        }
+        tc_fence_before();
+    }
+
+    __syncthreads();
+    if (w == TILE_SOFT / 32) {
+        tc_fence_after();
+        if (s_abort) {                                        /* products may still run: wait for them, within a bound */
+            if (lane == 0) {
+                mbar_init(&b_q_full, 1);
+                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+                tc_commit(&b_q_full);
+                mbar_wait(&b_q_full, 0);
+            }
+            __syncwarp();
+        }
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+/* Query rows whose result was not finite, one block each (see attend_row). */
+template <int KT, int HD>
+__global__ void __launch_bounds__(ROW_THREADS) k_attend_redo(const AttendArgs a) {
+    __shared__ RowShared<HD> sm;
+    const int R = a.T * a.G, many = a.redo[0];
+    for (int i = blockIdx.x; i < many; i += gridDim.x) {
+        const int q = a.redo[1 + i], u = q / R, r = q - u * R;
+        attend_row<KT, HD>(a, u, r % a.G, r / a.G, sm);
+    }
+}
+
+}  // namespace tria

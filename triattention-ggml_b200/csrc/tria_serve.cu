@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "tria_attend.cuh"
+#include "tria_attend_tile.cuh"
 #include "tria_cache.cuh"
 #include "tria_ctx.cuh"
 
@@ -303,15 +304,20 @@ static int few_blocks_of(int nt) {
 
 /* Launch plan of one chunk of caches. */
 struct AttendPlan {
-    int nt = 1;                 /* query rows per group, in eights */
+    bool tile = false;          /* k_attend_tile, else k_attend_few */
+    int nt = 1;                 /* k_attend_few: query rows per group, in eights */
+    int rows = 8;               /* query rows per group */
     int groups = 0, items = 0, grid = 0;
     bool plan_kernel = false, keep_scores = false;
-    size_t steps = 0, span = 0, done = 0, arrived = 0, part_o = 0, part_ml = 0, norm = 0, scores = 0, lse = 0, bytes = 0;
+    size_t steps = 0, span = 0, done = 0, arrived = 0, part_o = 0, part_ml = 0, norm = 0, scores = 0, redo = 0, bytes = 0;
     int64_t score_stride = 0;
 };
 
 /* Most blocks of an attention kernel (the workspace's counters). */
 constexpr int ATTEND_MAX_GRID = 1024;
+
+/* Query rows of a unit from which the tensor-core tiles are taken. */
+constexpr int TILE_FROM = 16;
 
 /* Most bytes of scores that a call with masses keeps instead of scoring twice. */
 constexpr size_t SCORES_MAX = (size_t)1 << 30;
@@ -319,16 +325,19 @@ constexpr size_t SCORES_MAX = (size_t)1 << 30;
 static int plan_attend(const tria_ctx *c, const tria_kv_view *v, int nl, int T, bool window, bool mass, AttendPlan &pl) {
     const int64_t units = (int64_t)nl * v->n_head_kv, R = (int64_t)T * c->G;
     pl = AttendPlan{};
+    pl.tile = R > TILE_FROM;
     pl.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
-    const int rows = 8 * pl.nt;
+    const int rows = pl.rows = pl.tile ? TILE_ROWS : 8 * pl.nt;
+    const int step = pl.tile ? TILE_STEP : ATT_STEP;
     const int64_t groups = (R + rows - 1) / rows, items = units * groups;
-    if (items * ((v->n_cells + ATT_STEP - 1) / ATT_STEP + 1) > INT32_MAX)
+    if (items * ((v->n_cells + step - 1) / step + 1) > INT32_MAX)
         FAIL(TRIA_ERR_UNSUPPORTED, "tria_attend: %lld query rows over %d cells in one call", (long long)(units * R), v->n_cells);
     pl.groups = (int)groups;
     pl.items = (int)items;
     pl.grid = std::min((v->type == TRIA_TYPE_F16 ? few_blocks_of<KT_F16>(pl.nt) : few_blocks_of<KT_Q8_0>(pl.nt)) * c->sm_count,
                        ATTEND_MAX_GRID);
-    pl.plan_kernel = window || items > 512;
+    if (pl.tile) pl.grid = std::min(c->sm_count, ATTEND_MAX_GRID);
+    pl.plan_kernel = pl.tile || window || items > 512;
     pl.score_stride = ((int64_t)v->n_cells + ATT_STEP - 1) / ATT_STEP * ATT_STEP;
     const size_t sb = (size_t)(units * R * pl.score_stride) * 4;
     pl.keep_scores = mass && R <= 16 && sb <= SCORES_MAX;
@@ -343,6 +352,7 @@ static int plan_attend(const tria_ctx *c, const tria_kv_view *v, int nl, int T, 
     }
     pl.part_o = take((size_t)2 * pl.grid * rows * c->hd * 4);
     pl.part_ml = take((size_t)2 * pl.grid * rows * 8);
+    if (pl.tile) pl.redo = take((size_t)(units * R + 1) * 4);
     if (mass) pl.norm = take((size_t)(units * R) * 8);
     if (pl.keep_scores) pl.scores = take(sb);
     pl.bytes = at;
@@ -362,6 +372,20 @@ static int launch_few(tria_ctx *c, const AttendArgs &a, const AttendPlan &pl, cu
 }
 
 template <int KT, int HD>
+static int launch_tile(tria_ctx *c, const AttendArgs &a, const AttendPlan &pl, cudaStream_t st) {
+    using L = TileLayout<KT, HD>;
+    const bool extra = a.softcap > 0.0f || a.window > 0 || a.slopes;
+    auto fn = extra ? k_attend_tile<KT, HD, true> : k_attend_tile<KT, HD, false>;
+    CUDA_TRY(raise_smem_limit((const void *)fn, L::BYTES));
+    fn<<<pl.grid, L::THREADS, L::BYTES, st>>>(a);
+    CUDA_TRY(cudaGetLastError());
+    k_attend_redo<KT, HD><<<c->sm_count, ROW_THREADS, 0, st>>>(a);
+    CUDA_TRY(cudaGetLastError());
+    c->launches += 2;
+    return TRIA_OK;
+}
+
+template <int KT, int HD>
 static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStream_t st) {
     const int units = a.n_layer * a.n_head_kv;
     uint8_t *ws = c->d_attend;
@@ -372,18 +396,20 @@ static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStre
     a.norm = a.mass_out ? (float2 *)(ws + pl.norm) : nullptr;
     a.scores = pl.keep_scores ? (float *)(ws + pl.scores) : nullptr;
     a.score_stride = pl.score_stride;
+    a.redo = pl.tile ? (int32_t *)(ws + pl.redo) : nullptr;
     if (a.T > 0) {
         if (pl.plan_kernel) {
             int32_t *steps = (int32_t *)(ws + pl.steps);
             int2 *span = a.window > 0 ? (int2 *)(ws + pl.span) : nullptr;
-            k_attend_plan<<<span ? pl.items : 1, PLAN_THREADS, 0, st>>>(a, 8 * pl.nt, pl.items, span, steps,
+            k_attend_plan<<<span ? pl.items : 1, PLAN_THREADS, 0, st>>>(a, pl.rows, pl.tile ? TILE_STEP : ATT_STEP, pl.items, span, steps,
                                                                        (int32_t *)(ws + pl.done));
             CUDA_TRY(cudaGetLastError());
             c->launches++;
             a.steps = steps;
             a.span = span;
         }
-        const int rc = pl.nt == 1 ? launch_few<KT, HD, 1>(c, a, pl, st)
+        const int rc = pl.tile ? launch_tile<KT, HD>(c, a, pl, st)
+                     : pl.nt == 1 ? launch_few<KT, HD, 1>(c, a, pl, st)
                      : pl.nt == 2 ? launch_few<KT, HD, 2>(c, a, pl, st) : launch_few<KT, HD, 4>(c, a, pl, st);
         if (rc) return rc;
     }
