@@ -57,6 +57,13 @@ __device__ __forceinline__ void tc_ld32(uint32_t (&x)[32], uint32_t addr) {
                  "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                  : TC_R8(x, 0), TC_R8(x, 8), TC_R8(x, 16), TC_R8(x, 24) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void tc_ld64(uint32_t (&x)[64], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+                 : TC_R8(x, 0), TC_R8(x, 8), TC_R8(x, 16), TC_R8(x, 24), 
+                   TC_R8(x, 32), TC_R8(x, 40), TC_R8(x, 48), TC_R8(x, 56)
+                 : "r"(addr) : "memory");
+}
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&x)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
                  "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
@@ -65,6 +72,84 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&x)[32]) 
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t (&x)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
                  ::TC_I8(x, 0), TC_I8(x, 8), "r"(addr) : "memory");
+}
+
+/* Two fp32 at a time (one instruction for both). */
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+/* tanh_small of both. */
+__device__ __forceinline__ uint64_t tanh_small2(uint64_t u) {
+    const uint64_t z = mul2(u, u);
+    uint64_t s = pair(21844.0f / 6081075.0f, 21844.0f / 6081075.0f);
+    s = fma2(s, z, pair(-1382.0f / 155925.0f, -1382.0f / 155925.0f));
+    s = fma2(s, z, pair(62.0f / 2835.0f, 62.0f / 2835.0f));
+    s = fma2(s, z, pair(-17.0f / 315.0f, -17.0f / 315.0f));
+    s = fma2(s, z, pair(2.0f / 15.0f, 2.0f / 15.0f));
+    s = fma2(s, z, pair(-1.0f / 3.0f, -1.0f / 3.0f));
+    return fma2(mul2(s, z), u, u);
+}
+/* N scores x (as bits) to weights 2^(x mul - from) in f16 pairs; their fp32 sums go to `sum`. */
+template <int N>
+__device__ __forceinline__ void tile_weights(const uint32_t (&v)[N], uint64_t mul, uint64_t from, uint32_t (&p)[N / 2], uint64_t &sum) {
+    uint64_t s[2] = {0ull, 0ull};
+#pragma unroll
+    for (int e = 0; e < N / 2; e++) {
+        const float2 x = unpair(fma2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), mul, from));
+        const float p0 = ex2(x.x), p1 = ex2(x.y);
+        s[e & 1] = add2(s[e & 1], pair(p0, p1));
+        p[e] = pack_half2(p0, p1);
+    }
+    sum = add2(sum, add2(s[0], s[1]));
+}
+template <int N>
+__device__ __forceinline__ float tile_max(const uint32_t (&v)[N]) {
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < N; e += 8)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            m[i] = fmaxf(m[i], fmaxf(__uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1])));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+/* Bits of the cache rows [e0, e0 + 32) that a query row sees by order: token t
+ * of the last T rows of n, causal or by its row of the tree; t < 0: none. */
+__device__ __forceinline__ uint32_t order_bits(const AttendArgs &a, int l, int t, int e0, int n) {
+    if (t < 0 || e0 >= n) return 0u;
+    const int own = e0 - (n - a.T);                       /* of the first row, among the tokens' own */
+    if (own + 32 <= 0) return 0xffffffffu;
+    const int live = a.tree ? n - e0 : t + 1 - own;       /* rows from e0 on that can be seen */
+    uint32_t bits = live <= 0 ? 0u : live >= 32 ? 0xffffffffu : (1u << live) - 1u;
+    if (a.tree && bits) {
+        const uint32_t *row = a.tree + l * a.tree_stride + (int64_t)t * a.tree_words;
+        const int w0 = own >> 5, sh = own & 31;            /* own >= -31: word -1 stands for rows before the tokens' */
+        const uint32_t x = w0 < 0 ? 0xffffffffu : w0 < a.tree_words ? row[w0] : 0u;
+        const uint32_t y = sh && w0 + 1 < a.tree_words ? row[w0 + 1] : 0u;
+        bits &= __funnelshift_r(x, y, sh);
+    }
+    return bits;
 }
 
 /* ------------------------------------------------------------------ */
@@ -81,7 +166,7 @@ template <int KT, int HD>
 struct TileLayout {
     static constexpr int PARTS = KT == KT_F16 ? 1 : 2;
     static constexpr int STAGES = KT == KT_F16 ? 2 : 1;
-    static constexpr int LOADERS = KT == KT_F16 ? 128 : 224;
+    static constexpr int LOADERS = KT == KT_F16 ? 96 : 224;
     static constexpr int THREADS = TILE_SOFT + 32 + LOADERS;
     static constexpr int PANEL = TILE_K * 128;           /* 128 rows of 64 f16 */
     static constexpr int SIDE = HD / 64 * PANEL;         /* one operand of one tile */
@@ -188,22 +273,22 @@ template <int KT, int HD>
 __device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p, int r0, int n, uint32_t st, int x) {
     using L = TileLayout<KT, HD>;
     if constexpr (KT == KT_F16) {
-        constexpr int CH = HD / 8, RPI = L::LOADERS / CH;
+        constexpr int CH = HD / 8, RPW = 32 / CH, NW = L::LOADERS / 32;      /* rows a warp copies at a time */
         if (a.copy16) {
-            const int r = x / CH, c = x % CH;
-            const uint32_t d = st + tile_chunk(r, c);           /* RPI is a multiple of 8: the swizzle stays */
-            const uint8_t *s = p + (int64_t)(r0 + r) * a.cell_stride + 16 * c;
-            const int64_t step = (int64_t)RPI * a.cell_stride;
+            const int w = x >> 5, r = (x & 31) / CH, c = x % CH;
+            const uint8_t *s = p + (int64_t)(r0 + r + RPW * w) * a.cell_stride + 16 * c;
+            const int64_t step = (int64_t)RPW * NW * a.cell_stride;
             if (r0 + TILE_K <= n) {
-#pragma unroll
-                for (int i = 0; i < TILE_K / RPI; i++) {
-                    cp_async16(d + i * RPI * 128, s, 16u);
+#pragma unroll 4
+                for (int y = r + RPW * w; y < TILE_K; y += RPW * NW) {
+                    cp_async16(st + tile_chunk(y, c), s, 16u);
                     s += step;
                 }
             } else {
-                for (int i = 0; i < TILE_K / RPI; i++) {
-                    const bool in = r0 + r + i * RPI < n;
-                    cp_async16(d + i * RPI * 128, in ? s + i * step : p, in ? 16u : 0u);
+                for (int y = r + RPW * w; y < TILE_K; y += RPW * NW) {
+                    const bool in = r0 + y < n;
+                    cp_async16(st + tile_chunk(y, c), in ? s : p, in ? 16u : 0u);
+                    s += step;
                 }
             }
         } else {
@@ -342,9 +427,9 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                 kc++;
                 if (vc >= L::STAGES && !wait_free(&b_v_free[vs], (vc / L::STAGES - 1) & 1)) { ok = false; break; }
                 tile_load<KT, HD>(a, v, row0, n, smem + L::V + vs * L::PARTS * L::SIDE, x);
-                if (want_pos && x < TILE_K) {                 /* with V: free once the weights are made */
-                    const bool in = row0 + x < n;
-                    cp_async4(smem + L::POS + (vs * TILE_K + x) * 4, pos + (in ? row0 + x : 0), in ? 4u : 0u);
+                for (int y = x; want_pos && y < TILE_K; y += L::LOADERS) {      /* with V: free once the weights are made */
+                    const bool in = row0 + y < n;
+                    cp_async4(smem + L::POS + (vs * TILE_K + y) * 4, pos + (in ? row0 + y : 0), in ? 4u : 0u);
                 }
                 issued(&b_v_full[vs]);
                 vc++;
@@ -440,8 +525,8 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const int tp = in && want_pos ? a.tok_pos[l * a.tok_pos_stride + t] : 0;
             const float slope2 = EXTRA && in && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
             const int64_t lo = (int64_t)tp - a.window;
-            const int seen_end = in ? n - a.T + t + 1 : 0;    /* causal: rows before it are seen */
-            float m = -INFINITY, sum = 0.0f;
+            float m = -INFINITY;
+            uint64_t sum = 0ull;                              /* two partial sums */
             for (int i = wk.i0; active && i < wk.i1; i++) {
                 const int j0 = i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K;
                 const uint32_t tc = tiles + (i - wk.i0);
@@ -451,111 +536,106 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                 sc++;
                 tc_fence_after();
                 const bool all = j0 + TILE_K <= n - a.T && (!EXTRA || a.window <= 0);
-                const bool rewrite = EXTRA || !all;           /* the scores are made final in tensor memory first */
-                float top = -INFINITY;
+                /* rescales what is there when the maximum has outrun it; the sums so far are complete when S is */
+                auto raise = [&](float top) {
+                    if (!__any_sync(0xffffffffu, top > m + FEW_SLACK)) return;
+                    const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
+                    m = to;
+                    sum = mul2(sum, pair(f, f));
+                    if (i == wk.i0) return;
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t v[32];
+                        tc_ld32(v, O + 32 * c);
+                        tc_wait_ld();
 #pragma unroll
-                for (int c = 0; c < TILE_K / 32; c++) {
-                    uint32_t v[32];
-                    tc_ld32(v, S + 32 * c);
+                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                        tc_st32(O + 32 * c, v);
+                    }
+                };
+                if (!EXTRA && all && map.scale >= 0.0f) {
+                    /* straight: the second half's scores stay in registers between the two passes */
+                    uint32_t v[64], p[32];
+                    tc_ld64(v, S);
                     tc_wait_ld();
-                    if (!rewrite) {
-                        float hi = -INFINITY;
-                        if (map.scale >= 0.0f) {
+                    float top = tile_max<64>(v);
+                    tc_ld64(v, S + 64);
+                    tc_wait_ld();
+                    top = fmaxf(top, tile_max<64>(v));
+                    raise(top * map.scale);
+                    const float from = m == -INFINITY ? 0.0f : FEW_LIFT - m;
+                    const uint64_t mul = pair(map.scale, map.scale), off = pair(from, from);
+                    tile_weights<64>(v, mul, off, p, sum);
+                    tc_ld64(v, S);
+                    tc_wait_ld();
+                    tc_st32(S + 32, p);                       /* over scores already read */
+                    tile_weights<64>(v, mul, off, p, sum);
+                    tc_st32(S, p);
+                } else {
+                    /* the scores are made final in tensor memory first */
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < TILE_K / 32; c++) {
+                        uint32_t v[32];
+                        tc_ld32(v, S + 32 * c);
+                        tc_wait_ld();
+                        const uint64_t ms = pair(map.scale, map.scale);
+                        float far = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < 32; e++) hi = fmaxf(hi, __uint_as_float(v[e]));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; e++) hi = fmaxf(hi, -__uint_as_float(v[e]));
+                        for (int e = 0; e < 16; e++) {
+                            const float2 y = unpair(mul2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), ms));
+                            v[2 * e] = __float_as_uint(y.x);
+                            v[2 * e + 1] = __float_as_uint(y.y);
+                            if (EXTRA) far = fmaxf(far, fmaxf(fabsf(y.x), fabsf(y.y)));
                         }
-                        top = fmaxf(top, hi);
-                    } else {
                         if (EXTRA && map.cap > 0.0f) {
-                            float far = 0.0f;
-#pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                const float y = __uint_as_float(v[e]) * map.scale;
-                                v[e] = __float_as_uint(y);
-                                far = fmaxf(far, fabsf(y));
-                            }
+                            const uint64_t cap = pair(map.cap, map.cap);
                             if (__any_sync(0xffffffffu, !(far < 0.4f))) {
 #pragma unroll
                                 for (int e = 0; e < 32; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 32; e++) v[e] = __float_as_uint(map.cap * tanh_small(__uint_as_float(v[e])));
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
-                        }
-                        if (want_pos) {
-                            const int32_t *ps = s_pos + (tc % L::STAGES) * TILE_K + 32 * c;
-#pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                const int pj = ps[e];
-                                float y = fmaf(-slope2, (float)(tp - pj), __uint_as_float(v[e]));
-                                if (a.window > 0 && !(pj >= lo || pj < a.sink)) y = -INFINITY;
-                                v[e] = __float_as_uint(y);
-                            }
-                        }
-                        const int e0 = j0 + 32 * c;
-                        if (e0 + 32 > n - a.T) {
-                            if (!a.tree) {
-#pragma unroll
-                                for (int e = 0; e < 32; e++)
-                                    if (e0 + e >= seen_end) v[e] = 0xff800000u;
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 32; e++) {
-                                    const int own = e0 + e - (n - a.T);
-                                    bool see = in && e0 + e < n;
-                                    if (see && own >= 0)
-                                        see = a.tree[l * a.tree_stride + (int64_t)t * a.tree_words + (own >> 5)] >> (own & 31) & 1u;
-                                    if (!see) v[e] = 0xff800000u;
+                                for (int e = 0; e < 16; e++) {
+                                    const float2 y = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
+                                    v[2 * e] = __float_as_uint(y.x);
+                                    v[2 * e + 1] = __float_as_uint(y.y);
                                 }
                             }
                         }
+                        uint32_t bits = all ? 0xffffffffu : order_bits(a, l, t, j0 + 32 * c, n);
+                        if (want_pos) {
+                            const int4 *ps = reinterpret_cast<const int4 *>(s_pos + (tc % L::STAGES) * TILE_K + 32 * c);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(v[e]));
+                            for (int e = 0; e < 8; e++) {
+                                const int4 q = ps[e];
+                                const int pj[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                                for (int f = 0; f < 4; f++) {
+                                    v[4 * e + f] = __float_as_uint(fmaf(-slope2, (float)(tp - pj[f]), __uint_as_float(v[4 * e + f])));
+                                    if (a.window > 0 && !(pj[f] >= lo || pj[f] < a.sink)) bits &= ~(1u << (4 * e + f));
+                                }
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, bits != 0xffffffffu)) {
+#pragma unroll
+                            for (int e = 0; e < 32; e++)
+                                if (!(bits >> e & 1u)) v[e] = 0xff800000u;
+                        }
+                        top = fmaxf(top, tile_max<32>(v));
                         tc_st32(S + 32 * c, v);
                     }
-                }
-                if (rewrite) tc_wait_st();
-                else top *= fabsf(map.scale);
-                const bool up = top > m + FEW_SLACK;
-                if (__any_sync(0xffffffffu, up)) {
-                    const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
-                    m = to;
-                    sum *= f;
-                    if (i > wk.i0) {                          /* the sums so far: their products are done when S is */
+                    tc_wait_st();
+                    raise(top);
+                    const float from = m == -INFINITY ? 0.0f : FEW_LIFT - m;
+                    const uint64_t one = pair(1.0f, 1.0f), off = pair(from, from);
 #pragma unroll 1
-                        for (int c = 0; c < HD / 32; c++) {
-                            uint32_t v[32];
-                            tc_ld32(v, O + 32 * c);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                            tc_st32(O + 32 * c, v);
-                        }
+                    for (int c = 0; c < TILE_K / 32; c++) {
+                        uint32_t v[32], p[16];
+                        tc_ld32(v, S + 32 * c);
+                        tc_wait_ld();
+                        tile_weights<32>(v, one, off, p, sum);
+                        tc_st16(S + 16 * c, p);
                     }
-                }
-                const float from = m == -INFINITY ? 0.0f : m - FEW_LIFT, mul = rewrite ? 1.0f : map.scale;
-#pragma unroll
-                for (int c = 0; c < TILE_K / 32; c++) {
-                    uint32_t v[32], p[16];
-                    tc_ld32(v, S + 32 * c);
-                    tc_wait_ld();
-                    float part[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float p0 = ex2(fmaf(__uint_as_float(v[2 * e]), mul, -from));
-                        const float p1 = ex2(fmaf(__uint_as_float(v[2 * e + 1]), mul, -from));
-                        part[0] += p0;
-                        part[1] += p1;
-                        p[e] = pack_half2(p0, p1);
-                    }
-                    sum += part[0] + part[1];
-                    tc_st16(S + 16 * c, p);                   /* over scores already read */
                 }
                 tc_wait_st();
                 tc_fence_before();
@@ -566,11 +646,13 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc_fence_after();
 
+            const float2 halves = unpair(sum);
+            const float total_w = halves.x + halves.y;
             const int64_t base = wk.base;
             const int c0 = (int)(((base + 1) * grid - 1) / total), c1 = (int)(((int64_t)steps[wk.it] * grid - 1) / total);
             if (c0 == c1) {
-                const bool none = sum == 0.0f;
-                const float inv = none ? 0.0f : 1.0f / sum;
+                const bool none = total_w == 0.0f;
+                const float inv = none ? 0.0f : 1.0f / total_w;
                 bool bad = false;
                 if (active) {
 #pragma unroll 1
@@ -597,7 +679,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                         }
                     }
                     if (in) {
-                        if (a.lse) a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + head] = none ? -INFINITY : (m - FEW_LIFT + log2f(sum)) * LN2;
+                        if (a.lse) a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + head] = none ? -INFINITY : (m - FEW_LIFT + log2f(total_w)) * LN2;
                         if (a.norm) a.norm[(int64_t)u * R + r] = none ? make_float2(0.0f, 0.0f) : make_float2(m - FEW_LIFT, inv);
                         if (bad) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + r;
                     }
@@ -616,7 +698,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                             for (int e = 0; e < 8; e++) d[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                         }
                     }
-                    if (in) a.part_ml[(int64_t)slot * TILE_ROWS + x * TILE_Q + row] = make_float2(m, sum);
+                    if (in) a.part_ml[(int64_t)slot * TILE_ROWS + x * TILE_Q + row] = make_float2(m, total_w);
                 }
                 __threadfence();
                 asm volatile("bar.sync 1, %0;" ::"n"(TILE_SOFT) : "memory");
