@@ -339,16 +339,16 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
     const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
 
     if (tid == 0) {
-        mbar_init(&b_q_full, L::LOADERS);
+        mbar_init(&b_q_full, L::LOADERS / 32);
         mbar_init(&b_q_free, 1);
         mbar_init(&b_o_full, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&b_s_full[i], 1);
-            mbar_init(&b_p_ready[i], TILE_Q);
+            mbar_init(&b_p_ready[i], TILE_Q / 32);
         }
         for (int i = 0; i < L::STAGES; i++) {
-            mbar_init(&b_k_full[i], L::LOADERS);
-            mbar_init(&b_v_full[i], L::LOADERS);
+            mbar_init(&b_k_full[i], L::LOADERS / 32);
+            mbar_init(&b_v_full[i], L::LOADERS / 32);
             mbar_init(&b_k_free[i], 1);
             mbar_init(&b_v_free[i], 1);
         }
@@ -375,17 +375,18 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
         uint32_t kc = 0, vc = 0;
         uint64_t *pending = nullptr;                          /* the copy still to be announced */
         auto announce = [&]() {
-            fence_async_smem();
-            mbar_arrive(pending);
+            fence_async_smem();                               /* every lane's own writes, then one arrival a warp */
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pending);
             pending = nullptr;
         };
         auto wait_free = [&](uint64_t *bar, uint32_t parity) -> bool {
-            if (mbar_try(bar, parity)) return true;
+            if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
             if (pending) {                                    /* nobody may wait for it while we wait */
                 cp_async_wait<0>();
                 announce();
             }
-            return tile_wait(bar, parity, &s_abort, a.status);
+            return __all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a.status));
         };
         auto issued = [&](uint64_t *bar) {
             cp_async_commit();
@@ -439,48 +440,64 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
         if (pending) announce();
     } else if (w == TILE_SOFT / 32) {
         /* ---------------- products ---------------- */
-        if (lane == 0) {
-            constexpr uint32_t qk = tile_idesc(TILE_K, false), pv = tile_idesc(HD, true);
-            uint32_t kc = 0, vc = 0, pc[2] = {0, 0};
-            bool ok = true;
-            for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
-                const int grp = wk.it % a.groups, N = wk.i1 - wk.i0;
-                const int tiles = R - grp * TILE_ROWS > TILE_Q ? 2 : 1;
-                if (!tile_wait(&b_q_full, seg & 1, &s_abort, a.status)) break;
-                for (int i = 0; ok && i <= N; i++) {
-                    if (i < N && !tile_wait(&b_k_full[kc % L::STAGES], (kc / L::STAGES) & 1, &s_abort, a.status)) { ok = false; break; }
-                    if (i > 0 && !tile_wait(&b_v_full[vc % L::STAGES], (vc / L::STAGES) & 1, &s_abort, a.status)) { ok = false; break; }
-                    for (int x = 0; x < tiles; x++) {
-                        if (i > 0) {
-                            if (!tile_wait(&b_p_ready[x], pc[x] & 1, &s_abort, a.status)) { ok = false; break; }
-                            pc[x]++;
-                            tc_fence_after();
-                            const uint32_t vb = smem + L::V + (vc % L::STAGES) * L::PARTS * L::SIDE;
+        /* the warp walks together, one lane issues */
+        constexpr uint32_t qk = tile_idesc(TILE_K, false), pv = tile_idesc(HD, true);
+        /* operand descriptors: the address is in the low bits, so a step is an addition */
+        const uint64_t d_q = tile_desc(smem + L::Q, 16), d_k = tile_desc(smem + L::K, 16), d_v = tile_desc(smem + L::V, L::PANEL);
+        uint32_t kc = 0, vc = 0, pc0 = 0, pc1 = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a.status)); };
+        auto values = [&](int x, bool add) {                  /* O += P V */
+            if (lane == 0) {
+                const uint64_t vd = d_v + (uint64_t)((vc % L::STAGES) * (L::PARTS * L::SIDE >> 4));
+                const uint32_t o = tmem + 256 + 128 * x, p = tmem + 128 * x;
+                tc_mma_ts(o, p, vd, pv, add);
 #pragma unroll
-                            for (int part = 0; part < L::PARTS; part++)
-#pragma unroll
-                                for (int s = 0; s < TILE_K / 16; s++)
-                                    tc_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * s, tile_desc(vb + part * L::SIDE + s * 2048, L::PANEL),
-                                              pv, i > 1 || part > 0 || s > 0);
-                        }
-                        if (i < N) {
-                            const uint32_t qb = smem + L::Q + x * L::SIDE, kb = smem + L::K + (kc % L::STAGES) * L::PARTS * L::SIDE;
-#pragma unroll
-                            for (int part = 0; part < L::PARTS; part++)
-#pragma unroll
-                                for (int s = 0; s < HD / 16; s++) {
-                                    const uint32_t off = (s / 4) * L::PANEL + (s % 4) * 32;
-                                    tc_mma_ss(tmem + 128 * x, tile_desc(qb + off, 16), tile_desc(kb + part * L::SIDE + off, 16), qk,
-                                              part > 0 || s > 0);
-                                }
-                            tc_commit(&b_s_full[x]);
-                        }
-                    }
-                    if (!ok) break;
-                    if (i > 0) tc_commit(&b_v_free[vc++ % L::STAGES]);
-                    if (i < N) tc_commit(&b_k_free[kc++ % L::STAGES]);
+                for (int s = 1; s < L::PARTS * (TILE_K / 16); s++) {
+                    constexpr int PER = TILE_K / 16;
+                    tc_mma_ts(o, p + 8 * (s % PER), vd + ((s / PER) * (L::SIDE >> 4) + (s % PER) * (2048 >> 4)), pv, true);
                 }
-                if (!ok) break;
+            }
+        };
+        auto scores = [&](int x) {                            /* S = Q K^T */
+            if (lane == 0) {
+                const uint64_t qd = d_q + (uint64_t)(x * (L::SIDE >> 4)), kd = d_k + (uint64_t)((kc % L::STAGES) * (L::PARTS * L::SIDE >> 4));
+#pragma unroll
+                for (int s = 0; s < L::PARTS * (HD / 16); s++) {
+                    constexpr int PER = HD / 16;
+                    const int off = ((s % PER) / 4) * (L::PANEL >> 4) + (s % 4) * (32 >> 4);
+                    tc_mma_ss(tmem + 128 * x, qd + off, kd + ((s / PER) * (L::SIDE >> 4) + off), qk, s > 0);
+                }
+                tc_commit(&b_s_full[x]);
+            }
+        };
+        for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+            const int grp = wk.it % a.groups, N = wk.i1 - wk.i0;
+            const bool two = R - grp * TILE_ROWS > TILE_Q;
+            if (!wait(&b_q_full, seg & 1)) break;
+            for (int i = 0; i <= N; i++) {
+                if (i < N && !(ok = wait(&b_k_full[kc % L::STAGES], (kc / L::STAGES) & 1))) break;
+                if (i > 0) {
+                    if (!(ok = wait(&b_v_full[vc % L::STAGES], (vc / L::STAGES) & 1) && wait(&b_p_ready[0], pc0++ & 1))) break;
+                    tc_fence_after();
+                    values(0, i > 1);
+                }
+                if (i < N) scores(0);
+                if (two) {
+                    if (i > 0) {
+                        if (!(ok = wait(&b_p_ready[1], pc1++ & 1))) break;
+                        tc_fence_after();
+                        values(1, i > 1);
+                    }
+                    if (i < N) scores(1);
+                }
+                if (i > 0 && lane == 0) tc_commit(&b_v_free[vc % L::STAGES]);
+                if (i > 0) vc++;
+                if (i < N && lane == 0) tc_commit(&b_k_free[kc % L::STAGES]);
+                if (i < N) kc++;
+            }
+            if (!ok) break;
+            if (lane == 0) {
                 tc_commit(&b_o_full);
                 tc_commit(&b_q_free);
             }
@@ -639,7 +656,8 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                 }
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&b_p_ready[x]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b_p_ready[x]);
             }
             if (!ok) break;
             if (!tile_wait(&b_o_full, seg & 1, &s_abort, a.status)) ok = false;
@@ -693,9 +711,10 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                         tc_ld32(v, O + 32 * c);
                         tc_wait_ld();
                         if (in) {
-                            uint4 *d = reinterpret_cast<uint4 *>(a.part_o + ((int64_t)slot * TILE_ROWS + x * TILE_Q + row) * HD + 32 * c);
+                            /* [slot][dim / 4][row][4]: a warp's rows side by side */
+                            uint4 *d = reinterpret_cast<uint4 *>(a.part_o) + ((int64_t)slot * (HD / 4) + 8 * c) * TILE_ROWS + x * TILE_Q + row;
 #pragma unroll
-                            for (int e = 0; e < 8; e++) d[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                            for (int e = 0; e < 8; e++) d[e * TILE_ROWS] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                         }
                     }
                     if (in) a.part_ml[(int64_t)slot * TILE_ROWS + x * TILE_Q + row] = make_float2(m, total_w);
@@ -708,45 +727,58 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                     __threadfence();
                     if (tid == 0) a.arrived[c0] = 0;
                     const int s0 = 2 * c0 + (c0 * total / grid >= base ? 0 : 1);
-                    constexpr int LPR = HD / 4, RPP = TILE_SOFT / LPR;
-                    const int dim = tid % LPR * 4;
-                    for (int q = tid / LPR; q < rows; q += RPP) {
-                        auto slot_of = [&](int s) { return ((int64_t)(s == 0 ? s0 : 2 * (c0 + s)) * TILE_ROWS + q); };
+                    if (tid < rows) {                         /* a thread a row */
+                        auto slot_of = [&](int s) { return (int64_t)(s == 0 ? s0 : 2 * (c0 + s)); };
+                        const int rq = grp * TILE_ROWS + tid, tq = rq / a.G, hq = h * a.G + rq % a.G, nS = c1 - c0 + 1;
                         float mm = -INFINITY, ss = 0.0f;
-                        for (int s = 0; s <= c1 - c0; s++) mm = fmaxf(mm, __ldcg(&a.part_ml[slot_of(s)]).x);
-                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-                        for (int s = 0; s <= c1 - c0; s++) {
-                            const float2 y = __ldcg(&a.part_ml[slot_of(s)]);
-                            const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part_o + slot_of(s) * HD + dim));
-                            const float g = y.x == -INFINITY ? 0.0f : ex2(y.x - mm);
-                            ss = fmaf(y.y, g, ss);
-                            if (g != 0.0f) {
-                                acc.x = fmaf(o.x, g, acc.x);
-                                acc.y = fmaf(o.y, g, acc.y);
-                                acc.z = fmaf(o.z, g, acc.z);
-                                acc.w = fmaf(o.w, g, acc.w);
-                            }
+                        for (int s = 0; s < nS; s++) mm = fmaxf(mm, __ldcg(&a.part_ml[slot_of(s) * TILE_ROWS + tid]).x);
+#pragma unroll 4
+                        for (int s = 0; s < nS; s++) {
+                            const float2 y = __ldcg(&a.part_ml[slot_of(s) * TILE_ROWS + tid]);
+                            ss = fmaf(y.y, y.x == -INFINITY ? 0.0f : ex2(y.x - mm), ss);
                         }
                         const bool none = ss == 0.0f;
                         const float inv = none ? 0.0f : 1.0f / ss;
-                        if (none) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        acc.x *= inv;
-                        acc.y *= inv;
-                        acc.z *= inv;
-                        acc.w *= inv;
-                        const int rq = grp * TILE_ROWS + q, tq = rq / a.G, hq = h * a.G + rq % a.G;
-                        *reinterpret_cast<uint2 *>(a.out + l * a.o_cache + tq * a.o_tok + hq * a.o_head + dim) =
-                            make_uint2(pack_half2(acc.x, acc.y), pack_half2(acc.z, acc.w));
-                        const bool bad = (acc.x + acc.y + acc.z + acc.w) * 0.0f != 0.0f;
-                        /* one entry a row: the first of its lanes that saw it */
-                        const unsigned group = LPR == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
-                        const unsigned who = __ballot_sync(group, bad) & group;
-                        if (bad && lane == __ffs(who) - 1) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + rq;
-                        if (dim == 0) {
-                            if (a.lse) a.lse[((int64_t)l * a.T + tq) * a.n_head_kv * a.G + hq] = none ? -INFINITY : (mm - FEW_LIFT + log2f(ss)) * LN2;
-                            if (a.norm) a.norm[(int64_t)u * R + rq] = none ? make_float2(0.0f, 0.0f) : make_float2(mm - FEW_LIFT, inv);
+                        float fin = 0.0f;
+                        __half *dst = a.out + l * a.o_cache + tq * a.o_tok + hq * a.o_head;
+#pragma unroll 1
+                        for (int c = 0; c < HD / 16; c++) {
+                            float4 acc[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+                            for (int s = 0; s < nS; s++) {
+                                const float2 y = __ldcg(&a.part_ml[slot_of(s) * TILE_ROWS + tid]);
+                                const float g = y.x == -INFINITY ? 0.0f : ex2(y.x - mm);
+                                float4 o[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    o[e] = __ldcg(reinterpret_cast<const float4 *>(a.part_o) + (slot_of(s) * (HD / 4) + 4 * c + e) * TILE_ROWS + tid);
+                                if (g != 0.0f) {
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) {
+                                        acc[e].x = fmaf(o[e].x, g, acc[e].x);
+                                        acc[e].y = fmaf(o[e].y, g, acc[e].y);
+                                        acc[e].z = fmaf(o[e].z, g, acc[e].z);
+                                        acc[e].w = fmaf(o[e].w, g, acc[e].w);
+                                    }
+                                }
+                            }
+                            uint2 h2[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float x0 = none ? 0.0f : acc[e].x * inv, x1 = none ? 0.0f : acc[e].y * inv;
+                                const float x2 = none ? 0.0f : acc[e].z * inv, x3 = none ? 0.0f : acc[e].w * inv;
+                                fin += x0 * 0.0f + x1 * 0.0f + x2 * 0.0f + x3 * 0.0f;
+                                h2[e] = make_uint2(pack_half2(x0, x1), pack_half2(x2, x3));
+                            }
+                            reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(h2[0].x, h2[0].y, h2[1].x, h2[1].y);
+                            reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(h2[2].x, h2[2].y, h2[3].x, h2[3].y);
                         }
+                        if (fin != 0.0f) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + rq;
+                        if (a.lse) a.lse[((int64_t)l * a.T + tq) * a.n_head_kv * a.G + hq] = none ? -INFINITY : (mm - FEW_LIFT + log2f(ss)) * LN2;
+                        if (a.norm) a.norm[(int64_t)u * R + rq] = none ? make_float2(0.0f, 0.0f) : make_float2(mm - FEW_LIFT, inv);
                     }
                 }
             }
