@@ -3,10 +3,11 @@
  * the tcgen05 tensor cores.
  *
  * A block takes up to 256 query rows of a unit as two row tiles of 128 and
- * walks 128 cache rows a step: S = Q K^T into tensor memory, one thread per
- * query row turns its row of S into weights P (written over S as f16), and
- * O += P V accumulates in tensor memory.  While one row tile is at its
- * exponentials, the other one's products run.
+ * walks 128 cache rows a step, 64 at a time: S = Q K^T into tensor memory, one
+ * thread per query row turns its row of S into weights P (written over S as
+ * f16), and O += P V accumulates in tensor memory.  Each row tile has two S
+ * buffers, so the next scores are made while the weights of the last ones are:
+ * no role waits for the round trip through the others.
  */
 #pragma once
 
@@ -23,31 +24,35 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-/* The barrier completes when every product this thread issued so far has. */
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 /* Operand in shared memory as panels of 64 f16 columns: row r of a panel is the
- * 128 bytes at 128 r, its 16-byte chunks XORed with r mod 8 (128-byte swizzle).
- * `lead` is the byte step between panels where the columns are the operand's
- * row dimension (V), unused otherwise; eight rows are 1024 bytes on. */
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+ * 128 bytes at 128 r, its 16-byte chunks XORed with r mod 8 (128-byte swizzle);
+ * eight rows are 1024 bytes on.  Where the columns are the operand's row
+ * dimension (V), panels are `lead` bytes apart.  The low word of a descriptor
+ * holds the address (in 16 bytes) and lead, the high word is the same for all. */
+__device__ __forceinline__ uint32_t tile_desc(uint32_t addr, uint32_t lead) { return (addr & 0x3ffff) >> 4 | (lead >> 4) << 16; }
+constexpr uint32_t TILE_DESC_HI = (1024 >> 4) | 1u << 14 | 2u << 29;
 /* Instruction descriptor: fp32 sums, f16 operands, M = 128, B by rows (K) or by columns (V). */
 __host__ __device__ constexpr uint32_t tile_idesc(int n, bool b_by_column) {
     return 1u << 4 | (b_by_column ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+/* Products are issued by the one lane whose `lead` is not 0, predicated within
+ * the instruction: the warp stays converged and its operands uniform. */
+__device__ __forceinline__ void tc_mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %6, 0;\n\t"
+                 "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "n"(TILE_DESC_HI), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void tc_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %6, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "n"(TILE_DESC_HI), "r"(lead) : "memory");
+}
+/* The barrier completes when every product this thread issued so far has. */
+__device__ __forceinline__ void tc_commit(uint32_t lead, uint64_t *bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 ::"r"(smem_u32(bar)), "r"(lead) : "memory");
 }
 #define TC_R8(x, o) "=r"(x[o]), "=r"(x[o + 1]), "=r"(x[o + 2]), "=r"(x[o + 3]), "=r"(x[o + 4]), "=r"(x[o + 5]), "=r"(x[o + 6]), "=r"(x[o + 7])
 #define TC_I8(x, o) "r"(x[o]), "r"(x[o + 1]), "r"(x[o + 2]), "r"(x[o + 3]), "r"(x[o + 4]), "r"(x[o + 5]), "r"(x[o + 6]), "r"(x[o + 7])
@@ -56,6 +61,10 @@ __device__ __forceinline__ void tc_ld32(uint32_t (&x)[32], uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
                  "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                  : TC_R8(x, 0), TC_R8(x, 8), TC_R8(x, 16), TC_R8(x, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t (&x)[16], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : TC_R8(x, 0), TC_R8(x, 8) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tc_ld64(uint32_t (&x)[64], uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
@@ -156,7 +165,7 @@ __device__ __forceinline__ uint32_t order_bits(const AttendArgs &a, int l, int t
 /* Layout                                                               */
 /* ------------------------------------------------------------------ */
 
-constexpr int TILE_Q = 128, TILE_ROWS = 2 * TILE_Q, TILE_K = 128;
+constexpr int TILE_Q = 128, TILE_ROWS = 2 * TILE_Q, TILE_K = 128, TILE_H = 64;      /* cache rows a step, a score tile */
 static_assert(TILE_K == TILE_STEP, "plan");
 constexpr int TILE_SOFT = 2 * TILE_Q;                    /* threads of the two weight groups */
 
@@ -180,6 +189,9 @@ struct TileLayout {
 /* Kernel                                                               */
 /* ------------------------------------------------------------------ */
 
+/* Lane 0's value for the whole warp, so that what depends on it is uniform. */
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 /* Where a block's walk stands: each role follows the same segments. */
 struct TileWalk {
     int64_t at, end, base;
@@ -202,9 +214,11 @@ __device__ __forceinline__ void tile_walk_start(TileWalk &w, const int32_t *step
 __device__ __forceinline__ bool tile_walk_segment(TileWalk &w, const int32_t *steps) {
     if (w.at >= w.end) return false;
     while (steps[w.it] <= w.at) w.it++;
-    w.base = w.it ? steps[w.it - 1] : 0;
-    w.i0 = (int)(w.at - w.base);
-    w.i1 = (int)(min(w.end, (int64_t)steps[w.it]) - w.base);
+    w.it = uniform(w.it);
+    const int base = uniform(w.it ? steps[w.it - 1] : 0), last = uniform(steps[w.it]);
+    w.base = base;
+    w.i0 = (int)(w.at - base);
+    w.i1 = (int)(min(w.end, (int64_t)last) - base);
     return true;
 }
 __device__ __forceinline__ void tile_walk_next(TileWalk &w) {
@@ -324,17 +338,17 @@ template <int KT, int HD, bool EXTRA>
 __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(const AttendArgs a) {
     using L = TileLayout<KT, HD>;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t b_q_full, b_q_free, b_o_full, b_s_full[2], b_p_ready[2];
+    __shared__ __align__(8) uint64_t b_q_full, b_q_free, b_o_full, b_pv[2], b_s_full[2][2], b_p_ready[2][2];
     __shared__ __align__(8) uint64_t b_k_full[L::STAGES], b_k_free[L::STAGES], b_v_full[L::STAGES], b_v_free[L::STAGES];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ int s_last;
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, w = uniform(tid >> 5);
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int32_t *s_pos = reinterpret_cast<const int32_t *>(smem_raw + (smem - smem_u32(smem_raw)) + L::POS);
     const int units = a.n_layer * a.n_head_kv, items = units * a.groups, R = a.T * a.G;
     const int32_t *steps = a.steps;
-    const int64_t total = steps[items - 1];
+    const int64_t total = uniform(steps[items - 1]);
     const int b = blockIdx.x, grid = (int)min((int64_t)gridDim.x, total);
     const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
 
@@ -343,8 +357,11 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
         mbar_init(&b_q_free, 1);
         mbar_init(&b_o_full, 1);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&b_s_full[i], 1);
-            mbar_init(&b_p_ready[i], TILE_Q / 32);
+            mbar_init(&b_pv[i], 1);
+            for (int d = 0; d < 2; d++) {
+                mbar_init(&b_s_full[i][d], 1);
+                mbar_init(&b_p_ready[i][d], TILE_Q / 32);
+            }
         }
         for (int i = 0; i < L::STAGES; i++) {
             mbar_init(&b_k_full[i], L::LOADERS / 32);
@@ -363,7 +380,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    /* columns: S (and P) of tile x at 128 x, O at 256 + 128 x */
+    /* columns: S (and P) of row tile x, buffer d at 128 x + 64 d, O at 256 + 128 x */
 
     TileWalk wk;
     if (b < grid) tile_walk_start(wk, steps, items, total, grid, b);
@@ -412,11 +429,20 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
             const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
             if (seg && !wait_free(&b_q_free, (seg - 1) & 1)) break;
-            for (int y = x; y < TILE_ROWS * (HD / 8); y += L::LOADERS) {
-                const int q = y / (HD / 8), c = y % (HD / 8), r = grp * TILE_ROWS + q;
-                const __half *s = a.q + l * a.q_cache;
-                if (r < R) s += (r / a.G) * a.q_tok + (h * a.G + r % a.G) * a.q_head + 8 * c;
-                cp_async16(smem + L::Q + (q / TILE_Q) * L::SIDE + tile_chunk(q % TILE_Q, c), s, r < R ? 16u : 0u);
+            {   /* a warp copies RPW query rows at a time; token and head step along */
+                constexpr int CH = HD / 8, RPW = 32 / CH, STEP = RPW * (L::LOADERS / 32);
+                const int c = lane % CH, first = (x >> 5) * RPW + lane / CH;
+                int r = grp * TILE_ROWS + first, t = r / a.G, g = r - t * a.G;
+                const int dt = STEP / a.G, dg = STEP - dt * a.G;
+                const __half *base = a.q + l * a.q_cache + (int64_t)h * a.G * a.q_head + 8 * c;
+                for (int q = first; q < TILE_ROWS; q += STEP, r += STEP) {
+                    const bool in = r < R;
+                    cp_async16(smem + L::Q + (q / TILE_Q) * L::SIDE + tile_chunk(q % TILE_Q, c),
+                               in ? base + t * a.q_tok + g * a.q_head : base, in ? 16u : 0u);
+                    t += dt;
+                    g += dg;
+                    if (g >= a.G) { g -= a.G; t++; }
+                }
             }
             issued(&b_q_full);
             for (int i = wk.i0; i < wk.i1; i++) {
@@ -440,66 +466,82 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
         if (pending) announce();
     } else if (w == TILE_SOFT / 32) {
         /* ---------------- products ---------------- */
-        /* the warp walks together, one lane issues */
-        constexpr uint32_t qk = tile_idesc(TILE_K, false), pv = tile_idesc(HD, true);
-        /* operand descriptors: the address is in the low bits, so a step is an addition */
-        const uint64_t d_q = tile_desc(smem + L::Q, 16), d_k = tile_desc(smem + L::K, 16), d_v = tile_desc(smem + L::V, L::PANEL);
-        uint32_t kc = 0, vc = 0, pc0 = 0, pc1 = 0;
-        bool ok = true;
-        auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a.status)); };
-        auto values = [&](int x, bool add) {                  /* O += P V */
-            if (lane == 0) {
-                const uint64_t vd = d_v + (uint64_t)((vc % L::STAGES) * (L::PARTS * L::SIDE >> 4));
-                const uint32_t o = tmem + 256 + 128 * x, p = tmem + 128 * x;
-                tc_mma_ts(o, p, vd, pv, add);
+        /* Every other role waits for this warp, so a product has to cost few instructions: the warp stays converged
+         * and one lane issues (operands then live in uniform registers), and the tensor-memory addresses are constants,
+         * for all of it is this block's. */
+        const uint32_t lead = lane == 0;
+        {
+            constexpr uint32_t qk = tile_idesc(TILE_H, false), pv = tile_idesc(HD, true);
+            constexpr uint32_t STEP = L::PARTS * L::SIDE >> 4, PART = L::SIDE >> 4;      /* stage to stage, part to part */
+            constexpr uint32_t HALF = TILE_H * 128 >> 4;                                 /* 64 rows of a panel */
+            const uint32_t d_q = tile_desc(smem + L::Q, 16), d_k = tile_desc(smem + L::K, 16), d_v = tile_desc(smem + L::V, L::PANEL);
+            uint32_t ks = 0, kp = 0, vs = 0, vp = 0, pp = 0;            /* stages and phases; pp: bit 2 x + d */
+            auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a.status)); };
+            auto values = [&](uint32_t x, uint32_t d, uint32_t vd, bool add) {           /* O += P V */
+                const uint32_t o = 256 + 128 * x, p = 128 * x + 64 * d;
+                tc_mma_ts(lead, o, p, vd, pv, add);
 #pragma unroll
-                for (int s = 1; s < L::PARTS * (TILE_K / 16); s++) {
-                    constexpr int PER = TILE_K / 16;
-                    tc_mma_ts(o, p + 8 * (s % PER), vd + ((s / PER) * (L::SIDE >> 4) + (s % PER) * (2048 >> 4)), pv, true);
+                for (int s = 1; s < L::PARTS * (TILE_H / 16); s++) {
+                    constexpr int PER = TILE_H / 16;
+                    tc_mma_ts(lead, o, p + 8 * (s % PER), vd + ((s / PER) * PART + (s % PER) * (2048 >> 4)), pv, true);
                 }
-            }
-        };
-        auto scores = [&](int x) {                            /* S = Q K^T */
-            if (lane == 0) {
-                const uint64_t qd = d_q + (uint64_t)(x * (L::SIDE >> 4)), kd = d_k + (uint64_t)((kc % L::STAGES) * (L::PARTS * L::SIDE >> 4));
+                tc_commit(lead, &b_pv[x]);
+            };
+            auto scores = [&](uint32_t x, uint32_t d, uint32_t kd) {                     /* S = Q K^T */
 #pragma unroll
                 for (int s = 0; s < L::PARTS * (HD / 16); s++) {
                     constexpr int PER = HD / 16;
                     const int off = ((s % PER) / 4) * (L::PANEL >> 4) + (s % 4) * (32 >> 4);
-                    tc_mma_ss(tmem + 128 * x, qd + off, kd + ((s / PER) * (L::SIDE >> 4) + off), qk, s > 0);
+                    tc_mma_ss(lead, 128 * x + 64 * d, d_q + x * PART + off, kd + ((s / PER) * PART + off), qk, s > 0);
                 }
-                tc_commit(&b_s_full[x]);
+                tc_commit(lead, &b_s_full[x][d]);
+            };
+            if (tmem != 0) {
+                s_abort = 1;
+                atomicOr(a.status, ST_TIMEOUT);
             }
-        };
-        for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
-            const int grp = wk.it % a.groups, N = wk.i1 - wk.i0;
-            const bool two = R - grp * TILE_ROWS > TILE_Q;
-            if (!wait(&b_q_full, seg & 1)) break;
-            for (int i = 0; i <= N; i++) {
-                if (i < N && !(ok = wait(&b_k_full[kc % L::STAGES], (kc / L::STAGES) & 1))) break;
-                if (i > 0) {
-                    if (!(ok = wait(&b_v_full[vc % L::STAGES], (vc / L::STAGES) & 1) && wait(&b_p_ready[0], pc0++ & 1))) break;
-                    tc_fence_after();
-                    values(0, i > 1);
+            bool ok = tmem == 0;
+            for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+                const bool two = R - (wk.it % a.groups) * TILE_ROWS > TILE_Q;
+                const int N = wk.i1 - wk.i0;
+                if (!(ok = wait(&b_q_full, seg & 1) && wait(&b_k_full[ks], kp))) break;
+                for (uint32_t d = 0; d < 2; d++) {
+                    scores(0, d, d_k + ks * STEP + d * HALF);
+                    if (two) scores(1, d, d_k + ks * STEP + d * HALF);
                 }
-                if (i < N) scores(0);
-                if (two) {
-                    if (i > 0) {
-                        if (!(ok = wait(&b_p_ready[1], pc1++ & 1))) break;
+                tc_commit(lead, &b_k_free[ks]);
+                if (++ks == L::STAGES) { ks = 0; kp ^= 1; }
+                if (N == 1) tc_commit(lead, &b_q_free);
+                for (int i = 0; ok && i < N; i++) {
+                    const uint32_t kd = d_k + ks * STEP, vd = d_v + vs * STEP;
+                    const bool more = i + 1 < N;
+                    if (!(ok = wait(&b_v_full[vs], vp))) break;
+                    for (uint32_t d = 0; d < 2; d++) {
+                        if (!(ok = wait(&b_p_ready[0][d], pp >> d & 1))) break;
+                        pp ^= 1u << d;
                         tc_fence_after();
-                        values(1, i > 1);
+                        values(0, d, vd + d * HALF, i > 0 || d > 0);
+                        if (more && d == 0 && !(ok = wait(&b_k_full[ks], kp))) break;
+                        if (more) scores(0, d, kd + d * HALF);
+                        if (two) {
+                            if (!(ok = wait(&b_p_ready[1][d], pp >> (2 + d) & 1))) break;
+                            pp ^= 4u << d;
+                            tc_fence_after();
+                            values(1, d, vd + d * HALF, i > 0 || d > 0);
+                            if (more) scores(1, d, kd + d * HALF);
+                        }
                     }
-                    if (i < N) scores(1);
+                    if (!ok) break;
+                    tc_commit(lead, &b_v_free[vs]);
+                    if (++vs == L::STAGES) { vs = 0; vp ^= 1; }
+                    if (more) {
+                        tc_commit(lead, &b_k_free[ks]);
+                        if (++ks == L::STAGES) { ks = 0; kp ^= 1; }
+                        if (i + 2 == N) tc_commit(lead, &b_q_free);
+                    }
                 }
-                if (i > 0 && lane == 0) tc_commit(&b_v_free[vc % L::STAGES]);
-                if (i > 0) vc++;
-                if (i < N && lane == 0) tc_commit(&b_k_free[kc % L::STAGES]);
-                if (i < N) kc++;
-            }
-            if (!ok) break;
-            if (lane == 0) {
-                tc_commit(&b_o_full);
-                tc_commit(&b_q_free);
+                if (!ok) break;
+                tc_commit(lead, &b_o_full);
             }
         }
         __syncwarp();
@@ -509,7 +551,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
         const uint32_t mine = tmem + ((uint32_t)(w & 3) << 21);      /* lanes 32 (w mod 4) on */
         const uint32_t S = mine + 128 * x, O = mine + 256 + 128 * x;
         const ScoreMap map(a);
-        uint32_t sc = 0, tiles = 0;                           /* scores seen, tiles of the segments before */
+        uint32_t sc = 0, tiles = 0;                           /* score tiles seen, steps of the segments before */
         bool ok = true;
 
         /* items without a row to see */
@@ -544,120 +586,102 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const int64_t lo = (int64_t)tp - a.window;
             float m = -INFINITY;
             uint64_t sum = 0ull;                              /* two partial sums */
-            for (int i = wk.i0; active && i < wk.i1; i++) {
-                const int j0 = i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K;
-                const uint32_t tc = tiles + (i - wk.i0);
-                if (!tile_wait(&b_s_full[x], sc & 1, &s_abort, a.status)) ok = false;
+            for (int y = 0; active && y < 2 * (wk.i1 - wk.i0); y++) {
+                const int i = wk.i0 + (y >> 1);
+                const uint32_t d = y & 1, tc = tiles + (y >> 1), T = S + 64 * d;
+                const int j0 = (i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K) + TILE_H * d;
+                if (!tile_wait(&b_s_full[x][d], sc >> 1 & 1, &s_abort, a.status)) ok = false;
                 if (want_pos && ok && !tile_wait(&b_v_full[tc % L::STAGES], (tc / L::STAGES) & 1, &s_abort, a.status)) ok = false;
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                sc++;
                 tc_fence_after();
-                const bool all = j0 + TILE_K <= n - a.T && (!EXTRA || a.window <= 0);
-                /* rescales what is there when the maximum has outrun it; the sums so far are complete when S is */
-                auto raise = [&](float top) {
-                    if (!__any_sync(0xffffffffu, top > m + FEW_SLACK)) return;
+                const bool all = j0 + TILE_H <= n - a.T && (!EXTRA || a.window <= 0);    /* every token sees every row */
+                uint32_t v[64], p[32];
+                tc_ld64(v, T);
+                tc_wait_ld();
+                uint64_t mul = pair(map.scale, map.scale);
+                if (EXTRA) {                                  /* the scores made final in place */
+                    float far = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const float2 z = unpair(mul2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), mul));
+                        v[2 * e] = __float_as_uint(z.x);
+                        v[2 * e + 1] = __float_as_uint(z.y);
+                        far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
+                    }
+                    if (map.cap > 0.0f) {
+                        const uint64_t cap = pair(map.cap, map.cap);
+                        if (__any_sync(0xffffffffu, !(far < 0.4f))) {
+#pragma unroll
+                            for (int e = 0; e < 64; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) {
+                                const float2 z = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
+                                v[2 * e] = __float_as_uint(z.x);
+                                v[2 * e + 1] = __float_as_uint(z.y);
+                            }
+                        }
+                    }
+                    mul = pair(1.0f, 1.0f);
+                }
+                if (want_pos || !all || (!EXTRA && map.scale <= 0.0f)) {
+                    uint32_t b0 = order_bits(a, l, t, j0, n), b1 = order_bits(a, l, t, j0 + 32, n);
+                    if (want_pos) {
+                        const int4 *ps = reinterpret_cast<const int4 *>(s_pos + (tc % L::STAGES) * TILE_K + TILE_H * d);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int4 q = ps[e];
+                            const int pj[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int f = 0; f < 4; f++) {
+                                v[4 * e + f] = __float_as_uint(fmaf(-slope2, (float)(tp - pj[f]), __uint_as_float(v[4 * e + f])));
+                                if (a.window > 0 && !(pj[f] >= lo || pj[f] < a.sink)) {
+                                    if (e < 8) b0 &= ~(1u << (4 * e + f));
+                                    else b1 &= ~(1u << (4 * e + f - 32));
+                                }
+                            }
+                        }
+                    }
+                    if (!EXTRA && map.scale <= 0.0f) {        /* a masked score below stays below only if final */
+#pragma unroll
+                        for (int e = 0; e < 64; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
+                        mul = pair(1.0f, 1.0f);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        if (!(b0 >> e & 1u)) v[e] = 0xff800000u;
+                        if (!(b1 >> e & 1u)) v[e + 32] = 0xff800000u;
+                    }
+                }
+                const float top = tile_max<64>(v) * unpair(mul).x;
+                if (__any_sync(0xffffffffu, top > m + FEW_SLACK)) {
+                    /* the maximum has outrun the sums: rescale them, once the products under way have landed */
                     const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
                     m = to;
                     sum = mul2(sum, pair(f, f));
-                    if (i == wk.i0) return;
+                    if (y > 0) {
+                        if (!tile_wait(&b_pv[x], (sc - 1) & 1, &s_abort, a.status)) ok = false;
+                        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                        tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < HD / 32; c++) {
-                        uint32_t v[32];
-                        tc_ld32(v, O + 32 * c);
-                        tc_wait_ld();
+                        for (int c = 0; c < HD / 16; c++) {
+                            uint32_t o[16];
+                            tc_ld16(o, O + 16 * c);
+                            tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                        tc_st32(O + 32 * c, v);
-                    }
-                };
-                if (!EXTRA && all && map.scale >= 0.0f) {
-                    /* straight: the second half's scores stay in registers between the two passes */
-                    uint32_t v[64], p[32];
-                    tc_ld64(v, S);
-                    tc_wait_ld();
-                    float top = tile_max<64>(v);
-                    tc_ld64(v, S + 64);
-                    tc_wait_ld();
-                    top = fmaxf(top, tile_max<64>(v));
-                    raise(top * map.scale);
-                    const float from = m == -INFINITY ? 0.0f : FEW_LIFT - m;
-                    const uint64_t mul = pair(map.scale, map.scale), off = pair(from, from);
-                    tile_weights<64>(v, mul, off, p, sum);
-                    tc_ld64(v, S);
-                    tc_wait_ld();
-                    tc_st32(S + 32, p);                       /* over scores already read */
-                    tile_weights<64>(v, mul, off, p, sum);
-                    tc_st32(S, p);
-                } else {
-                    /* the scores are made final in tensor memory first */
-                    float top = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < TILE_K / 32; c++) {
-                        uint32_t v[32];
-                        tc_ld32(v, S + 32 * c);
-                        tc_wait_ld();
-                        const uint64_t ms = pair(map.scale, map.scale);
-                        float far = 0.0f;
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const float2 y = unpair(mul2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), ms));
-                            v[2 * e] = __float_as_uint(y.x);
-                            v[2 * e + 1] = __float_as_uint(y.y);
-                            if (EXTRA) far = fmaxf(far, fmaxf(fabsf(y.x), fabsf(y.y)));
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tc_st16(O + 16 * c, o);
                         }
-                        if (EXTRA && map.cap > 0.0f) {
-                            const uint64_t cap = pair(map.cap, map.cap);
-                            if (__any_sync(0xffffffffu, !(far < 0.4f))) {
-#pragma unroll
-                                for (int e = 0; e < 32; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 16; e++) {
-                                    const float2 y = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
-                                    v[2 * e] = __float_as_uint(y.x);
-                                    v[2 * e + 1] = __float_as_uint(y.y);
-                                }
-                            }
-                        }
-                        uint32_t bits = all ? 0xffffffffu : order_bits(a, l, t, j0 + 32 * c, n);
-                        if (want_pos) {
-                            const int4 *ps = reinterpret_cast<const int4 *>(s_pos + (tc % L::STAGES) * TILE_K + 32 * c);
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                const int4 q = ps[e];
-                                const int pj[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                                for (int f = 0; f < 4; f++) {
-                                    v[4 * e + f] = __float_as_uint(fmaf(-slope2, (float)(tp - pj[f]), __uint_as_float(v[4 * e + f])));
-                                    if (a.window > 0 && !(pj[f] >= lo || pj[f] < a.sink)) bits &= ~(1u << (4 * e + f));
-                                }
-                            }
-                        }
-                        if (__any_sync(0xffffffffu, bits != 0xffffffffu)) {
-#pragma unroll
-                            for (int e = 0; e < 32; e++)
-                                if (!(bits >> e & 1u)) v[e] = 0xff800000u;
-                        }
-                        top = fmaxf(top, tile_max<32>(v));
-                        tc_st32(S + 32 * c, v);
-                    }
-                    tc_wait_st();
-                    raise(top);
-                    const float from = m == -INFINITY ? 0.0f : FEW_LIFT - m;
-                    const uint64_t one = pair(1.0f, 1.0f), off = pair(from, from);
-#pragma unroll 1
-                    for (int c = 0; c < TILE_K / 32; c++) {
-                        uint32_t v[32], p[16];
-                        tc_ld32(v, S + 32 * c);
-                        tc_wait_ld();
-                        tile_weights<32>(v, one, off, p, sum);
-                        tc_st16(S + 16 * c, p);
                     }
                 }
+                const float from = m == -INFINITY ? 0.0f : FEW_LIFT - m;
+                tile_weights<64>(v, mul, pair(from, from), p, sum);
+                tc_st32(T, p);                                /* over the scores */
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&b_p_ready[x]);
+                if (lane == 0) mbar_arrive(&b_p_ready[x][d]);
+                sc++;
             }
             if (!ok) break;
             if (!tile_wait(&b_o_full, seg & 1, &s_abort, a.status)) ok = false;
@@ -796,7 +820,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             if (lane == 0) {
                 mbar_init(&b_q_full, 1);
                 asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-                tc_commit(&b_q_full);
+                tc_commit(1, &b_q_full);
                 mbar_wait(&b_q_full, 0);
             }
             __syncwarp();
