@@ -165,7 +165,7 @@ __device__ __forceinline__ uint32_t order_bits(const AttendArgs &a, int l, int t
 /* Layout                                                               */
 /* ------------------------------------------------------------------ */
 
-constexpr int TILE_Q = 128, TILE_ROWS = 2 * TILE_Q, TILE_K = 128, TILE_H = 64;      /* cache rows a step, a score tile */
+constexpr int TILE_Q = 128, TILE_ROWS = 2 * TILE_Q, TILE_K = 128;      /* cache rows a step */
 static_assert(TILE_K == TILE_STEP, "plan");
 constexpr int TILE_SOFT = 2 * TILE_Q;                    /* threads of the two weight groups */
 
@@ -337,6 +337,7 @@ __device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p,
 template <int KT, int HD, bool EXTRA>
 __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(const AttendArgs a) {
     using L = TileLayout<KT, HD>;
+    constexpr int NB = EXTRA || KT == KT_Q8_0 ? 2 : 1, TILE_H = TILE_K / NB;      /* score buffers of a row tile, cache rows of each */
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t b_q_full, b_q_free, b_o_full, b_pv[2], b_s_full[2][2], b_p_ready[2][2];
     __shared__ __align__(8) uint64_t b_k_full[L::STAGES], b_k_free[L::STAGES], b_v_full[L::STAGES], b_v_free[L::STAGES];
@@ -473,19 +474,20 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
         {
             constexpr uint32_t qk = tile_idesc(TILE_H, false), pv = tile_idesc(HD, true);
             constexpr uint32_t STEP = L::PARTS * L::SIDE >> 4, PART = L::SIDE >> 4;      /* stage to stage, part to part */
-            constexpr uint32_t HALF = TILE_H * 128 >> 4;                                 /* 64 rows of a panel */
+            constexpr uint32_t HALF = 64 * 128 >> 4;                                     /* 64 rows of a panel */
             const uint32_t d_q = tile_desc(smem + L::Q, 16), d_k = tile_desc(smem + L::K, 16), d_v = tile_desc(smem + L::V, L::PANEL);
             uint32_t ks = 0, kp = 0, vs = 0, vp = 0, pp = 0;            /* stages and phases; pp: bit 2 x + d */
             auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a.status)); };
-            auto values = [&](uint32_t x, uint32_t d, uint32_t vd, bool add) {           /* O += P V */
-                const uint32_t o = 256 + 128 * x, p = 128 * x + 64 * d;
+            /* O += P V over cache rows 64 e .. 64 e + 63 of the step */
+            auto values = [&](uint32_t x, uint32_t e, uint32_t vd, bool add) {
+                const uint32_t o = 256 + 128 * x, p = 128 * x + (NB == 2 ? 64 : 32) * e;
                 tc_mma_ts(lead, o, p, vd, pv, add);
 #pragma unroll
-                for (int s = 1; s < L::PARTS * (TILE_H / 16); s++) {
-                    constexpr int PER = TILE_H / 16;
+                for (int s = 1; s < L::PARTS * (64 / 16); s++) {
+                    constexpr int PER = 64 / 16;
                     tc_mma_ts(lead, o, p + 8 * (s % PER), vd + ((s / PER) * PART + (s % PER) * (2048 >> 4)), pv, true);
                 }
-                tc_commit(lead, &b_pv[x]);
+                if (NB == 2) tc_commit(lead, &b_pv[x]);
             };
             auto scores = [&](uint32_t x, uint32_t d, uint32_t kd) {                     /* S = Q K^T */
 #pragma unroll
@@ -505,7 +507,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                 const bool two = R - (wk.it % a.groups) * TILE_ROWS > TILE_Q;
                 const int N = wk.i1 - wk.i0;
                 if (!(ok = wait(&b_q_full, seg & 1) && wait(&b_k_full[ks], kp))) break;
-                for (uint32_t d = 0; d < 2; d++) {
+                for (uint32_t d = 0; d < NB; d++) {
                     scores(0, d, d_k + ks * STEP + d * HALF);
                     if (two) scores(1, d, d_k + ks * STEP + d * HALF);
                 }
@@ -516,19 +518,25 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                     const uint32_t kd = d_k + ks * STEP, vd = d_v + vs * STEP;
                     const bool more = i + 1 < N;
                     if (!(ok = wait(&b_v_full[vs], vp))) break;
-                    for (uint32_t d = 0; d < 2; d++) {
-                        if (!(ok = wait(&b_p_ready[0][d], pp >> d & 1))) break;
-                        pp ^= 1u << d;
+                    /* one row tile's weights of 64 cache rows, and the scores that take their place */
+                    auto turn = [&](uint32_t x, uint32_t e) {
+                        if (!(ok = wait(&b_p_ready[x][e], pp >> (2 * x + e) & 1))) return;
+                        pp ^= 1u << (2 * x + e);
                         tc_fence_after();
-                        values(0, d, vd + d * HALF, i > 0 || d > 0);
-                        if (more && d == 0 && !(ok = wait(&b_k_full[ks], kp))) break;
-                        if (more) scores(0, d, kd + d * HALF);
-                        if (two) {
-                            if (!(ok = wait(&b_p_ready[1][d], pp >> (2 + d) & 1))) break;
-                            pp ^= 4u << d;
-                            tc_fence_after();
-                            values(1, d, vd + d * HALF, i > 0 || d > 0);
-                            if (more) scores(1, d, kd + d * HALF);
+                        values(x, e, vd + e * HALF, i > 0 || e > 0);
+                        if (!more || (NB == 1 && e == 0)) return;
+                        if (x == 0 && (NB == 1 || e == 0) && !(ok = wait(&b_k_full[ks], kp))) return;
+                        scores(x, NB == 2 ? e : 0, kd + (NB == 2 ? e * HALF : 0));
+                    };
+                    if (NB == 2) {
+                        for (uint32_t e = 0; ok && e < 2; e++) {
+                            turn(0, e);
+                            if (ok && two) turn(1, e);
+                        }
+                    } else {
+                        for (uint32_t x = 0; ok && x < (two ? 2 : 1); x++) {
+                            turn(x, 0);
+                            if (ok) turn(x, 1);
                         }
                     }
                     if (!ok) break;
@@ -586,23 +594,24 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const int64_t lo = (int64_t)tp - a.window;
             float m = -INFINITY;
             uint64_t sum = 0ull;                              /* two partial sums */
-            for (int y = 0; active && y < 2 * (wk.i1 - wk.i0); y++) {
-                const int i = wk.i0 + (y >> 1);
-                const uint32_t d = y & 1, tc = tiles + (y >> 1), T = S + 64 * d;
+            for (int y = 0; active && y < NB * (wk.i1 - wk.i0); y++) {
+                const int i = wk.i0 + y / NB;
+                const uint32_t d = y % NB, tc = tiles + y / NB, T = S + 64 * d;
                 const int j0 = (i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K) + TILE_H * d;
-                if (!tile_wait(&b_s_full[x][d], sc >> 1 & 1, &s_abort, a.status)) ok = false;
+                if (!tile_wait(&b_s_full[x][d], sc / NB & 1, &s_abort, a.status)) ok = false;
                 if (want_pos && ok && !tile_wait(&b_v_full[tc % L::STAGES], (tc / L::STAGES) & 1, &s_abort, a.status)) ok = false;
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tc_fence_after();
                 const bool all = j0 + TILE_H <= n - a.T && (!EXTRA || a.window <= 0);    /* every token sees every row */
-                uint32_t v[64], p[32];
-                tc_ld64(v, T);
+                uint32_t v[TILE_H];
+                tc_ld64(*reinterpret_cast<uint32_t (*)[64]>(v), T);
+                if (TILE_H > 64) tc_ld64(*reinterpret_cast<uint32_t (*)[64]>(v + TILE_H - 64), T + TILE_H - 64);
                 tc_wait_ld();
                 uint64_t mul = pair(map.scale, map.scale);
                 if (EXTRA) {                                  /* the scores made final in place */
                     float far = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
+                    for (int e = 0; e < TILE_H / 2; e++) {
                         const float2 z = unpair(mul2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), mul));
                         v[2 * e] = __float_as_uint(z.x);
                         v[2 * e + 1] = __float_as_uint(z.y);
@@ -612,10 +621,10 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                         const uint64_t cap = pair(map.cap, map.cap);
                         if (__any_sync(0xffffffffu, !(far < 0.4f))) {
 #pragma unroll
-                            for (int e = 0; e < 64; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
+                            for (int e = 0; e < TILE_H; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 32; e++) {
+                            for (int e = 0; e < TILE_H / 2; e++) {
                                 const float2 z = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
                                 v[2 * e] = __float_as_uint(z.x);
                                 v[2 * e + 1] = __float_as_uint(z.y);
@@ -625,42 +634,39 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                     mul = pair(1.0f, 1.0f);
                 }
                 if (want_pos || !all || (!EXTRA && map.scale <= 0.0f)) {
-                    uint32_t b0 = order_bits(a, l, t, j0, n), b1 = order_bits(a, l, t, j0 + 32, n);
+                    uint32_t bits[TILE_H / 32];
+#pragma unroll
+                    for (int e = 0; e < TILE_H / 32; e++) bits[e] = order_bits(a, l, t, j0 + 32 * e, n);
                     if (want_pos) {
                         const int4 *ps = reinterpret_cast<const int4 *>(s_pos + (tc % L::STAGES) * TILE_K + TILE_H * d);
 #pragma unroll
-                        for (int e = 0; e < 16; e++) {
+                        for (int e = 0; e < TILE_H / 4; e++) {
                             const int4 q = ps[e];
                             const int pj[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                             for (int f = 0; f < 4; f++) {
                                 v[4 * e + f] = __float_as_uint(fmaf(-slope2, (float)(tp - pj[f]), __uint_as_float(v[4 * e + f])));
-                                if (a.window > 0 && !(pj[f] >= lo || pj[f] < a.sink)) {
-                                    if (e < 8) b0 &= ~(1u << (4 * e + f));
-                                    else b1 &= ~(1u << (4 * e + f - 32));
-                                }
+                                if (a.window > 0 && !(pj[f] >= lo || pj[f] < a.sink)) bits[e / 8] &= ~(1u << (4 * (e % 8) + f));
                             }
                         }
                     }
                     if (!EXTRA && map.scale <= 0.0f) {        /* a masked score below stays below only if final */
 #pragma unroll
-                        for (int e = 0; e < 64; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
+                        for (int e = 0; e < TILE_H; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
                         mul = pair(1.0f, 1.0f);
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        if (!(b0 >> e & 1u)) v[e] = 0xff800000u;
-                        if (!(b1 >> e & 1u)) v[e + 32] = 0xff800000u;
-                    }
+                    for (int e = 0; e < TILE_H; e++)
+                        if (!(bits[e / 32] >> (e & 31) & 1u)) v[e] = 0xff800000u;
                 }
-                const float top = tile_max<64>(v) * unpair(mul).x;
+                const float top = tile_max<TILE_H>(v) * unpair(mul).x;
                 if (__any_sync(0xffffffffu, top > m + FEW_SLACK)) {
                     /* the maximum has outrun the sums: rescale them, once the products under way have landed */
                     const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
                     m = to;
                     sum = mul2(sum, pair(f, f));
-                    if (y > 0) {
-                        if (!tile_wait(&b_pv[x], (sc - 1) & 1, &s_abort, a.status)) ok = false;
+                    if (y > 0) {                              /* (with one buffer they have, or S would not be full) */
+                        if (NB == 2 && !tile_wait(&b_pv[x], (sc - 1) & 1, &s_abort, a.status)) ok = false;
                         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                         tc_fence_after();
 #pragma unroll 1
@@ -675,12 +681,19 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                     }
                 }
                 const float from = m == -INFINITY ? 0.0f : FEW_LIFT - m;
-                tile_weights<64>(v, mul, pair(from, from), p, sum);
-                tc_st32(T, p);                                /* over the scores */
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&b_p_ready[x][d]);
+                const uint64_t off = pair(from, from);
+#pragma unroll
+                for (int e = 0; e < TILE_H / 32; e++) {       /* over the scores */
+                    uint32_t p[16];
+                    tile_weights<32>(*reinterpret_cast<const uint32_t (*)[32]>(v + 32 * e), mul, off, p, sum);
+                    tc_st16(T + 16 * e, p);
+                    if (e & 1) {                              /* 64 cache rows: the value product may start */
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&b_p_ready[x][NB == 2 ? d : e / 2]);
+                    }
+                }
                 sc++;
             }
             if (!ok) break;
