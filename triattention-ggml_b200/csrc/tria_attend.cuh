@@ -51,6 +51,9 @@ struct AttendArgs {
     int64_t score_stride;
 };
 
+/* Lane 0's value for the whole warp, so that what depends on it is uniform. */
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 /* Rows of unit u: a count outside the cache is clamped and reported. */
 __device__ __forceinline__ int attend_rows(const AttendArgs &a, int u) {
     const int n = a.n_rows[u];
@@ -659,7 +662,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
     __shared__ RowShared<HD> s_row;
     __shared__ int s_redo[ROWS];
     __shared__ float s_inv[ROWS];
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, r8 = lane >> 2, c = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, w = uniform(tid >> 5), r8 = lane >> 2, c = lane & 3;
     const int units = a.n_layer * a.n_head_kv, items = units * a.groups, R = a.T * a.G;
     const int *steps = a.steps;
     if (!steps) {                                             /* few items, no window */
@@ -675,7 +678,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
         __syncthreads();
         steps = s_steps;
     }
-    const int64_t total = steps[items - 1];
+    const int64_t total = uniform(steps[items - 1]);
     const int b = blockIdx.x, grid = (int)min((int64_t)gridDim.x, total);     /* no block between an item's first and last is idle */
     const ScoreMap map(a);
     const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
@@ -711,11 +714,13 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
     }
     for (bool first = true; at < end; first = false) {
         while (steps[it] <= at) it++;
-        const int64_t base = it ? steps[it - 1] : 0;
-        const int i0 = (int)(at - base), i1 = (int)(min(end, (int64_t)steps[it]) - base);
+        it = uniform(it);
+        const int64_t base = uniform(it ? steps[it - 1] : 0), upto = uniform(steps[it]);
+        const int i0 = (int)(at - base), i1 = (int)(min(end, upto) - base);
         const int u = it / a.groups, grp = it - u * a.groups, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
-        const int n = attend_rows(a, u);
-        const int2 span = a.span ? a.span[it] : make_int2(0, 0);
+        const int n = uniform(attend_rows(a, u));
+        int2 span = a.span ? a.span[it] : make_int2(0, 0);
+        span = make_int2(uniform(span.x), uniform(span.y));
         const int head_steps = (min(span.x, n) + ATT_STEP - 1) / ATT_STEP;
         auto slice_row = [&](int i) { return (i < head_steps ? i * ATT_STEP : span.y + (i - head_steps) * ATT_STEP) + FEW_SLICE * w; };
         const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
@@ -914,7 +919,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
         __syncthreads();
 
         /* blocks that share the item: owner(s) = the block whose range holds step s */
-        const int c0 = (int)(((base + 1) * grid - 1) / total), c1 = (int)(((int64_t)steps[it] * grid - 1) / total);
+        const int c0 = (int)(((base + 1) * grid - 1) / total), c1 = (int)((upto * grid - 1) / total);
         const int rows = min(ROWS, R - grp * ROWS);
         constexpr int DPT = FEW_THREADS / HD;                 /* rows a pass covers */
         const int d = tid % HD, dr = tid / HD;

@@ -189,9 +189,6 @@ struct TileLayout {
 /* Kernel                                                               */
 /* ------------------------------------------------------------------ */
 
-/* Lane 0's value for the whole warp, so that what depends on it is uniform. */
-__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
-
 /* Where a block's walk stands: each role follows the same segments. */
 struct TileWalk {
     int64_t at, end, base;
