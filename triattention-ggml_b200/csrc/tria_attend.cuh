@@ -346,26 +346,20 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 }
 /* d += a b, 16 x 8 x 16, f16 operands, fp32 sums. */
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
+/* d = a b. */
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float lds_half(uint32_t addr) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-    return __half2float(__ushort_as_half(v));
-}
+__device__ __forceinline__ uint32_t word_at(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
+__device__ __forceinline__ uint2 two_words_at(const uint8_t *p) { return *reinterpret_cast<const uint2 *>(p); }
+__device__ __forceinline__ float half_at(const uint8_t *p) { return __half2float(*reinterpret_cast<const __half *>(p)); }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -490,7 +484,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 /* The products of 16 cache rows with 8 NT query rows, rows of the cache as the
  * matrix rows: s[t][e] is cache row r8 + 8 (e >> 1) with query row 8 t + 2 c + (e & 1). */
 template <int KT, int HD, int NT>
-__device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], uint32_t st, int lead, int lane, float (&s)[NT][4]) {
+__device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], const uint8_t *st, int lead, int lane, float (&s)[NT][4]) {
     constexpr int KS = FewStage<KT, HD>::KS;
 #pragma unroll
     for (int t = 0; t < NT; t++)
@@ -498,10 +492,11 @@ __device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], uin
         for (int i = 0; i < 4; i++) s[t][i] = 0.0f;
     if constexpr (KT == KT_F16) {
         const int row = lane & 15, hi = lane >> 4;
+        const uint32_t at = smem_u32(st) + row * KS;
 #pragma unroll
         for (int x = 0; x < HD / 16; x++) {
             uint32_t k[4];
-            ldsm4(k, st + row * KS + 16 * ((2 * x + hi) ^ (row & 7)));
+            ldsm4(k, at + 16 * ((2 * x + hi) ^ (row & 7)));
 #pragma unroll
             for (int t = 0; t < NT; t++) mma16816(s[t], k, qf[t][x][0], qf[t][x][1]);
         }
@@ -515,27 +510,27 @@ __device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], uin
             float d[2];
 #pragma unroll
             for (int hi = 0; hi < 2; hi++) {
-                const uint32_t at = st + 8 * hi * KS + 34 * blk + 2 + 8 * c - sh;
-                const uint2 x = lds64(at);
+                const uint8_t *at = st + 8 * c + (8 * hi * KS + 34 * blk + 2 - sh);
+                const uint2 x = two_words_at(at);
                 uint32_t w0, w1;
                 if (sh == 0) {
                     w0 = x.x;
                     w1 = x.y;
                 } else {
-                    const uint2 y = lds64(at + 8);
+                    const uint2 y = two_words_at(at + 8);
                     w0 = sh == 2 ? __funnelshift_r(x.x, x.y, 16) : sh == 4 ? x.y : __funnelshift_r(x.y, y.x, 16);
                     w1 = sh == 2 ? __funnelshift_r(x.y, y.x, 16) : sh == 4 ? y.x : __funnelshift_r(y.x, y.y, 16);
                 }
                 int8x4_half(w0, k[0][hi], k[0][hi + 2]);
                 int8x4_half(w1, k[1][hi], k[1][hi + 2]);
-                d[hi] = lds_half(st + 8 * hi * KS + 34 * blk);
+                d[hi] = half_at(st + 8 * hi * KS + 34 * blk);
             }
             /* the block's scale belongs to the cache row, so it multiplies the block's sum: the f16 operands stay the
              * stored integers and the scores keep fp32 */
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma16816(p, k[0], qf[t][2 * blk][0], qf[t][2 * blk][1]);
+                float p[4];
+                mma16816_first(p, k[0], qf[t][2 * blk][0], qf[t][2 * blk][1]);
                 mma16816(p, k[1], qf[t][2 * blk + 1][0], qf[t][2 * blk + 1][1]);
                 s[t][0] = fmaf(p[0], d[0], s[t][0]);
                 s[t][1] = fmaf(p[1], d[0], s[t][1]);
@@ -551,7 +546,7 @@ __device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], uin
  * whose row some query row sees, and a q8_0 scale only enters where p is not 0
  * (a row that is not seen may hold NaN). */
 template <int KT, int HD, int NT, bool FULL>
-__device__ __forceinline__ void few_pv(const float (&p)[NT][4], uint32_t st, int lead, int lane, uint32_t keep0, uint32_t keep1,
+__device__ __forceinline__ void few_pv(const float (&p)[NT][4], const uint8_t *st, int lead, int lane, uint32_t keep0, uint32_t keep1,
                                        float (&o)[NT][HD / 16][4]) {
     constexpr int VS = FewStage<KT, HD>::VS;
     if constexpr (KT == KT_F16) {
@@ -562,10 +557,11 @@ __device__ __forceinline__ void few_pv(const float (&p)[NT][4], uint32_t st, int
             pf[t][1] = transpose8(pack_half2(p[t][2], p[t][3]));
         }
         const int row = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
+        const uint32_t at = smem_u32(st) + row * VS;
 #pragma unroll
         for (int j = 0; j < HD / 16; j++) {
             uint32_t v[4];
-            ldsm4t(v, st + row * VS + 16 * ((2 * j + hi) ^ (row & 7)));
+            ldsm4t(v, at + 16 * ((2 * j + hi) ^ (row & 7)));
             if (!FULL) {
                 v[0] &= keep0;
                 v[1] &= keep0;
@@ -578,18 +574,18 @@ __device__ __forceinline__ void few_pv(const float (&p)[NT][4], uint32_t st, int
     } else {
         const int r8 = lane >> 2, c = lane & 3;
         st += lead;
-        const uint32_t v0 = st + 2 * c * VS + 4 * r8, d0 = st + r8 * VS;      /* rows 2c, 2c+1, 2c+8, 2c+9; scales of r8, r8+8 */
+        const uint8_t *v0 = st + 2 * c * VS + 4 * r8, *d0 = st + r8 * VS;      /* rows 2c, 2c+1, 2c+8, 2c+9; scales of r8, r8+8 */
 #pragma unroll
         for (int blk = 0; blk < HD / 32; blk++) {
             const int sh = (2 * blk + 2) & 3;
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t at = v0 + ((i & 1) + (i >> 1) * 8) * VS + 34 * blk;
-                if (sh == 0) w[i] = lds32(at + 2);
-                else w[i] = __funnelshift_r(lds32(at), lds32(at + 4), 16);
+                const uint8_t *at = v0 + ((i & 1) + (i >> 1) * 8) * VS + 34 * blk;
+                if (sh == 0) w[i] = word_at(at + 2);
+                else w[i] = __funnelshift_r(word_at(at), word_at(at + 4), 16);
             }
-            const float da = lds_half(d0 + 34 * blk), db = lds_half(d0 + 8 * VS + 34 * blk);
+            const float da = half_at(d0 + 34 * blk), db = half_at(d0 + 8 * VS + 34 * blk);
             /* the scales go into the weights before their one rounding to f16; the V operands are the stored integers */
             uint32_t pf[NT][2];
 #pragma unroll
@@ -682,7 +678,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
     const int b = blockIdx.x, grid = (int)min((int64_t)gridDim.x, total);     /* no block between an item's first and last is idle */
     const ScoreMap map(a);
     const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
-    const uint32_t ring = smem_u32(smem) + w * ST * S::BYTES;
+    uint8_t *const ring = smem + w * ST * S::BYTES;
 
     /* items without a row to see */
     for (int it = b; it < items; it += gridDim.x) {
@@ -731,14 +727,14 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
         auto load_k = [&](int i) {
             if (i < i1) {
                 const int row = slice_row(i);
-                const uint32_t st = ring + ((i - i0) % ST) * S::BYTES;
+                const uint32_t st = smem_u32(ring + (i - i0) % ST * S::BYTES);
                 few_load<KT, HD, S::KS>(a, k, lead, row, n, st + S::K, lane);
                 if (want_pos) few_load_pos(pos, row, n, st + S::P, lane);
             }
             cp_async_commit();
         };
         auto load_v = [&](int i) {
-            if (i < i1) few_load<KT, HD, S::VS>(a, v, lead, slice_row(i), n, ring + ((i - i0) % ST) * S::BYTES + S::V, lane);
+            if (i < i1) few_load<KT, HD, S::VS>(a, v, lead, slice_row(i), n, smem_u32(ring + (i - i0) % ST * S::BYTES + S::V), lane);
             cp_async_commit();
         };
         /* prologue: copies first, then the queries while they fly */
@@ -783,7 +779,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
         }
 
         for (int i = i0; i < i1; i++) {
-            const uint32_t st = ring + ((i - i0) % ST) * S::BYTES;
+            const uint8_t *const st = ring + (i - i0) % ST * S::BYTES;
             const int row0 = slice_row(i);
             const bool live = row0 < n;
             float s[NT][4];
@@ -806,8 +802,8 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
                 }
                 int pk[2] = {0, 0};
                 if (want_pos) {
-                    pk[0] = (int)lds32(st + S::P + 4 * r8);
-                    pk[1] = (int)lds32(st + S::P + 4 * (r8 + 8));
+                    pk[0] = (int)word_at(st + S::P + 4 * r8);
+                    pk[1] = (int)word_at(st + S::P + 4 * (r8 + 8));
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -1085,19 +1081,19 @@ __global__ void __launch_bounds__(MASS_THREADS) k_mass_tiles(const AttendArgs a)
     const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
     const bool want_pos = a.window > 0 || a.slopes != nullptr;
     const ScoreMap map(a);
-    const uint32_t st = smem_u32(s_keys[w]);
+    const uint8_t *const st = s_keys[w];
     const int lead = KT == KT_Q8_0 && HD == 128 ? (int)((h * a.head_stride) & 8) : 0;
     for (int row0 = (blockIdx.x * (MASS_THREADS / 32) + w) * 16; row0 < n; row0 += gridDim.x * MASS_KEYS) {
         __syncwarp();
-        few_load<KT, HD, S::KS>(a, k, lead, row0, n, st, lane);
-        if (want_pos) few_load_pos(pos, row0, n, st + 16 * S::KS, lane);
+        few_load<KT, HD, S::KS>(a, k, lead, row0, n, smem_u32(st), lane);
+        if (want_pos) few_load_pos(pos, row0, n, smem_u32(st) + 16 * S::KS, lane);
         cp_async_commit();
         cp_async_wait<0>();
         __syncwarp();
         int pk[2] = {0, 0};
         if (want_pos) {
-            pk[0] = (int)lds32(st + 16 * S::KS + 4 * r8);
-            pk[1] = (int)lds32(st + 16 * S::KS + 4 * (r8 + 8));
+            pk[0] = (int)word_at(st + 16 * S::KS + 4 * r8);
+            pk[1] = (int)word_at(st + 16 * S::KS + 4 * (r8 + 8));
         }
         float mass[2] = {0.0f, 0.0f};                           /* cache rows r8, r8 + 8 */
         /* by order, token t sees row j only if j <= n - T + t: query rows before that see none of these 16 */
