@@ -138,6 +138,8 @@ class AttendParams(C.Structure):
                 ("tok_pos_stride", C.c_int64), ("tree_stride", C.c_int64),
                 ("q_cache_stride", C.c_int64), ("q_tok_stride", C.c_int64), ("q_head_stride", C.c_int64),
                 ("o_cache_stride", C.c_int64), ("o_tok_stride", C.c_int64), ("o_head_stride", C.c_int64)]
+    _keep = (None, None, None)      # slopes, tok_pos, tree
+    _sig = None                     # the shapes that the strides were last taken from
 
 
 class AppendParams(C.Structure):
@@ -545,41 +547,59 @@ class Context:
         """tria_append: device tensors k, v [caches][n_tok][kv heads][head_dim]
         (f16 or fp32, contiguous last dimension) behind each unit's n_rows (device
         int32); n_rows_out defaults to n_rows, updated in place."""
+        L, KV, T = view.n_layer, view.n_head_kv, _torch()
         shape, stride, dtype = k.shape, k.stride(), k.dtype
         if len(shape) != 4 or stride[3] != 1 or v.shape != shape or v.stride() != stride or v.dtype != dtype:
             raise ValueError("k and v must have the same shape [caches][n_tok][kv heads][head_dim], type and strides, the last "
                              "dimension contiguous")
-        f32 = dtype == _torch().float32
-        if not f32 and dtype != _torch().float16:
+        f32 = dtype is T.float32
+        if not f32 and dtype is not T.float16:
             raise ValueError(f"k and v must be float16 or float32, not {dtype}")
-        if shape[0] != view.n_layer or shape[2] != view.n_head_kv or shape[3] != self.head_dim:
-            raise ValueError(f"k of shape {tuple(shape)} for {view.n_layer} caches of {view.n_head_kv} heads of {self.head_dim}")
-        self._shared_or_own(tok_pos, "tok_pos", (shape[1],), view.n_layer)
-        _ints_or_floats(tok_pos, "tok_pos", 2, _torch().int32)
-        self._mass(mass, view)
-        self._here(k, v, tok_pos, mass)
+        if shape[0] != L or shape[2] != KV or shape[3] != self.head_dim:
+            raise ValueError(f"k of shape {tuple(shape)} for {L} caches of {KV} heads of {self.head_dim}")
+        own = tok_pos.dim() == 2
+        if tok_pos.dtype is not T.int32 or tok_pos.shape != ((L, shape[1]) if own else (shape[1],)) or \
+                (shape[1] > 1 and tok_pos.stride(-1) != 1):
+            raise ValueError(f"tok_pos must be int32 [{shape[1]}] or [{L}][{shape[1]}] with a contiguous last dimension")
+        if mass is not None:
+            self._mass(mass, view)
         rows_out = n_rows if n_rows_out is None else n_rows_out
-        self._counts(view, n_rows, rows_out)
+        self._counts(L * KV, n_rows, rows_out)
+        dev = self.device
+        if k.get_device() != dev or v.get_device() != dev or tok_pos.get_device() != dev:
+            self._elsewhere(k, v, tok_pos)
         p = AppendParams(shape[1], SRC_F32 if f32 else SRC_F16, stride[0], stride[1], stride[2], tok_pos.data_ptr(),
-                         tok_pos.stride(0) if tok_pos.dim() == 2 else 0)
-        check(lib().tria_append(self.h, C.byref(view), n_rows.data_ptr(), C.byref(p), k.data_ptr(), v.data_ptr(), _ptr(mass),
-                                rows_out.data_ptr(), _stream(stream)))
+                         tok_pos.stride(0) if own else 0)
+        r = _lib.tria_append(self.h, C.byref(view), n_rows.data_ptr(), C.byref(p), k.data_ptr(), v.data_ptr(),
+                             0 if mass is None else mass.data_ptr(), rows_out.data_ptr(), _stream(stream))
+        if r:
+            check(r)
 
     def attend(self, view, n_rows, q, out, params, lse=None, mass_in=None, mass_out=None, stream=None):
         """tria_attend: device f16 tensors q, out [caches][n_tok][heads][head_dim]
         (any strides that are multiples of 8, the last dimension contiguous)."""
-        sig = (view.n_layer, view.n_head_kv, self.gqa, self.head_dim, q.shape, q.stride(), out.shape, out.stride(), q.dtype, out.dtype)
-        if getattr(params, "_sig", None) != sig:
+        L, KV = view.n_layer, view.n_head_kv
+        sig = (self.device, self.gqa, self.head_dim, L, KV, q.shape, q.stride(), out.shape, out.stride(), q.dtype, out.dtype)
+        if params._sig != sig:
             self._attend_shapes(view, q, out, params)
             params._sig = sig
-        if lse is not None and (lse.dtype != _torch().float32 or tuple(lse.shape) != tuple(q.shape[:3]) or not lse.is_contiguous()):
-            raise ValueError("lse must be a contiguous fp32 [caches][n_tok][heads]")
-        self._mass(mass_in, view)
-        self._mass(mass_out, view)
-        self._here(q, out, lse, mass_in, mass_out, *params._keep)
-        self._counts(view, n_rows)
-        check(lib().tria_attend(self.h, C.byref(view), n_rows.data_ptr(), C.byref(params), q.data_ptr(), out.data_ptr(),
-                                _ptr(lse), _ptr(mass_in), _ptr(mass_out), _stream(stream)))
+        if lse is not None:
+            if lse.dtype is not _torch().float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
+                raise ValueError("lse must be a contiguous fp32 [caches][n_tok][heads]")
+            self._here(lse)
+        if mass_out is not None:
+            self._mass(mass_out, view)
+        if mass_in is not None:
+            self._mass(mass_in, view)
+        self._counts(L * KV, n_rows)
+        dev = self.device
+        if q.get_device() != dev or out.get_device() != dev:
+            self._elsewhere(q, out)
+        r = _lib.tria_attend(self.h, C.byref(view), n_rows.data_ptr(), C.byref(params), q.data_ptr(), out.data_ptr(),
+                             0 if lse is None else lse.data_ptr(), 0 if mass_in is None else mass_in.data_ptr(),
+                             0 if mass_out is None else mass_out.data_ptr(), _stream(stream))
+        if r:
+            check(r)
 
     def _attend_shapes(self, view, q, out, params):
         """Checks q and out against the view and the params, and puts their strides into the params."""
@@ -591,6 +611,7 @@ class Context:
             raise ValueError(f"q of shape {tuple(q.shape)} for {view.n_layer} caches of {view.n_head_kv} x {self.gqa} heads "
                              f"of {self.head_dim}")
         slopes, tok_pos, tree = params._keep
+        self._here(*params._keep)
         if slopes is not None and slopes.shape[0] != q.shape[2]:
             raise ValueError(f"{slopes.shape[0]} slopes for {q.shape[2]} heads")
         self._shared_or_own(tok_pos, "tok_pos", (q.shape[1],), view.n_layer)
@@ -601,33 +622,36 @@ class Context:
 
     def accept(self, view, n_rows, n_tok, path, n_path, n_rows_out=None, mass=None, stream=None):
         """tria_accept: device int32 path [caches or 1][entries] and n_path [caches or 1]."""
-        i32 = _torch().int32
-        if path.dtype != i32 or path.dim() != 2 or n_path.dtype != i32 or not n_path.is_contiguous():
+        L, KV, i32 = view.n_layer, view.n_head_kv, _torch().int32
+        if path.dtype is not i32 or path.dim() != 2 or n_path.dtype is not i32 or not n_path.is_contiguous():
             raise ValueError("path must be an int32 [caches or 1][entries], n_path a contiguous int32 [caches or 1]")
         lists, entries = path.shape
-        if lists not in (1, view.n_layer) or n_path.numel() != lists or (path.stride(1) != 1 and entries > 1):
+        if (lists != 1 and lists != L) or n_path.numel() != lists or (path.stride(1) != 1 and entries > 1):
             raise ValueError("path must be [caches or 1][entries], its rows contiguous, n_path [caches or 1]")
         if entries < n_tok:
             raise ValueError(f"path holds {entries} entries a cache: room for n_tok = {n_tok} is wanted")
-        self._mass(mass, view)
-        self._here(path, n_path, mass)
+        if mass is not None:
+            self._mass(mass, view)
         rows_out = n_rows if n_rows_out is None else n_rows_out
-        self._counts(view, n_rows, rows_out)
-        check(lib().tria_accept(self.h, C.byref(view), n_rows.data_ptr(), n_tok, path.data_ptr(),
-                                path.stride(0) if lists > 1 else 0, n_path.data_ptr(), _ptr(mass), rows_out.data_ptr(),
-                                _stream(stream)))
+        self._counts(L * KV, n_rows, rows_out)
+        if path.get_device() != self.device or n_path.get_device() != self.device:
+            self._elsewhere(path, n_path)
+        r = _lib.tria_accept(self.h, C.byref(view), n_rows.data_ptr(), n_tok, path.data_ptr(), path.stride(0) if lists > 1 else 0,
+                             n_path.data_ptr(), 0 if mass is None else mass.data_ptr(), rows_out.data_ptr(), _stream(stream))
+        if r:
+            check(r)
 
     def evict_mass(self, src, dst, n_rows, mass, mass_dst, params, n_kept_out=None, stream=None):
         """tria_evict_mass: one eviction step ranked by device `mass`
         [layers][kv heads][n_cells]; n_rows is a host array."""
         a, p = self._rows(n_rows)
         self._mass(mass, src)
-        self._mass(mass_dst, dst)
-        self._here(mass, mass_dst)
+        if mass_dst is not None:
+            self._mass(mass_dst, dst)
         if a.shape[0] != src.n_layer * src.n_head_kv:
             raise ValueError(f"{a.shape[0]} row counts for {src.n_layer} x {src.n_head_kv} units")
         if n_kept_out is not None:
-            self._counts(src, n_kept_out)
+            self._counts(src.n_layer * src.n_head_kv, n_kept_out)
         check(lib().tria_evict_mass(self.h, C.byref(src), C.byref(dst), p, _ptr(mass), _ptr(mass_dst), C.byref(params),
                                     _ptr(n_kept_out), _stream(stream)))
 
@@ -635,22 +659,23 @@ class Context:
         """Tensors that kernels read or write must live on the context's device."""
         for x in tensors:
             if x is not None and x.get_device() != self.device:
-                raise ValueError(f"a tensor on {x.device} was given to a context of cuda:{self.device}")
+                self._elsewhere(x)
 
-    def _counts(self, view, *counts):
-        i32, units = _torch().int32, view.n_layer * view.n_head_kv
+    def _elsewhere(self, *tensors):
+        raise ValueError(f"a tensor on {', '.join(str(x.device) for x in tensors)} was given to a context of cuda:{self.device}")
+
+    def _counts(self, units, *counts):
         for x in counts:
-            if x.dtype != i32 or x.numel() != units or not x.is_contiguous() or x.get_device() != self.device:
-                raise ValueError(f"row counts must be a contiguous int32 tensor of {view.n_layer} x {view.n_head_kv} on "
-                                 f"cuda:{self.device}")
+            if x.dtype is not _torch().int32 or x.numel() != units or x.get_device() != self.device or not x.is_contiguous():
+                raise ValueError(f"row counts must be a contiguous int32 tensor of {units} units on cuda:{self.device}")
 
     @staticmethod
     def _shared_or_own(x, name, shape, caches):
         if x is not None and tuple(x.shape) not in (shape, (caches,) + shape):
             raise ValueError(f"{name} of shape {tuple(x.shape)}: {shape} or {(caches,) + shape} is wanted")
 
-    @staticmethod
-    def _mass(x, view):
-        if x is not None and (x.dtype != _torch().float32 or x.shape != (view.n_layer, view.n_head_kv, view.n_cells)
-                              or not x.is_contiguous()):
-            raise ValueError(f"mass must be a contiguous fp32 [{view.n_layer}][{view.n_head_kv}][{view.n_cells}] tensor")
+    def _mass(self, x, view):
+        if x.dtype is not _torch().float32 or x.shape != (view.n_layer, view.n_head_kv, view.n_cells) \
+                or x.get_device() != self.device or not x.is_contiguous():
+            raise ValueError(f"mass must be a contiguous fp32 [{view.n_layer}][{view.n_head_kv}][{view.n_cells}] tensor on "
+                             f"cuda:{self.device}")
