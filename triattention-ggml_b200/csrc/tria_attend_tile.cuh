@@ -280,11 +280,11 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) { return (c >> 3) *
 
 /* Starts (f16) or does (q8_0) the copy of rows [r0, r0 + 128) of one side;
  * rows at and behind n become zeros. */
-template <int KT, int HD>
+template <int KT, int HD, int LOADERS>
 __device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p, int r0, int n, uint32_t st, int x) {
     using L = TileLayout<KT, HD>;
     if constexpr (KT == KT_F16) {
-        constexpr int CH = HD / 8, RPW = 32 / CH, NW = L::LOADERS / 32;      /* rows a warp copies at a time */
+        constexpr int CH = HD / 8, RPW = 32 / CH, NW = LOADERS / 32;      /* rows a warp copies at a time */
         if (a.copy16) {
             const int w = x >> 5, r = (x & 31) / CH, c = x % CH;
             const uint8_t *s = p + (int64_t)(r0 + r + RPW * w) * a.cell_stride + 16 * c;
@@ -303,7 +303,7 @@ __device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p,
                 }
             }
         } else {
-            for (int y = x; y < TILE_K * CH * 4; y += L::LOADERS) {
+            for (int y = x; y < TILE_K * CH * 4; y += LOADERS) {
                 const int r = y / (CH * 4), c = y / 4 % CH, q = y & 3;
                 const bool in = r0 + r < n;
                 cp_async4(st + tile_chunk(r, c) + 4 * q, p + (in ? (int64_t)(r0 + r) * a.cell_stride + 16 * c + 4 * q : 0), in ? 4u : 0u);
@@ -312,7 +312,7 @@ __device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p,
     } else {
         constexpr int NB = HD / 32;
 #pragma unroll 1
-        for (int y = x; y < TILE_K * NB; y += L::LOADERS) {
+        for (int y = x; y < TILE_K * NB; y += LOADERS) {
             const int r = y / NB, b = y % NB;
             uint32_t hi[16], lo[16];
             if (r0 + r < n) {
@@ -328,6 +328,25 @@ __device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p,
                 sts128(d + L::SIDE, lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
             }
         }
+    }
+}
+
+/* Starts the copy of query rows [r0, r0 + ROWS) of kv head h of cache l as
+ * operands of 128 rows; rows at and behind R become zeros.  A warp copies 32 /
+ * (HD / 8) rows at a time, token and head stepping along. */
+template <int HD, int ROWS, int LOADERS>
+__device__ __forceinline__ void tile_load_q(const AttendArgs &a, int l, int h, int r0, uint32_t st, int x) {
+    constexpr int CH = HD / 8, RPW = 32 / CH, STEP = RPW * (LOADERS / 32), SIDE = HD / 64 * TILE_K * 128;
+    const int c = x % CH, first = (x >> 5) * RPW + (x & 31) / CH, R = a.T * a.G;
+    int r = r0 + first, t = r / a.G, g = r - t * a.G;
+    const int dt = STEP / a.G, dg = STEP - dt * a.G;
+    const __half *base = a.q + l * a.q_cache + (int64_t)h * a.G * a.q_head + 8 * c;
+    for (int q = first; q < ROWS; q += STEP, r += STEP) {
+        const bool in = r < R;
+        cp_async16(st + (q / TILE_Q) * SIDE + tile_chunk(q % TILE_Q, c), in ? base + t * a.q_tok + g * a.q_head : base, in ? 16u : 0u);
+        t += dt;
+        g += dg;
+        if (g >= a.G) { g -= a.G; t++; }
     }
 }
 
@@ -427,31 +446,17 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
             const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
             if (seg && !wait_free(&b_q_free, (seg - 1) & 1)) break;
-            {   /* a warp copies RPW query rows at a time; token and head step along */
-                constexpr int CH = HD / 8, RPW = 32 / CH, STEP = RPW * (L::LOADERS / 32);
-                const int c = lane % CH, first = (x >> 5) * RPW + lane / CH;
-                int r = grp * TILE_ROWS + first, t = r / a.G, g = r - t * a.G;
-                const int dt = STEP / a.G, dg = STEP - dt * a.G;
-                const __half *base = a.q + l * a.q_cache + (int64_t)h * a.G * a.q_head + 8 * c;
-                for (int q = first; q < TILE_ROWS; q += STEP, r += STEP) {
-                    const bool in = r < R;
-                    cp_async16(smem + L::Q + (q / TILE_Q) * L::SIDE + tile_chunk(q % TILE_Q, c),
-                               in ? base + t * a.q_tok + g * a.q_head : base, in ? 16u : 0u);
-                    t += dt;
-                    g += dg;
-                    if (g >= a.G) { g -= a.G; t++; }
-                }
-            }
+            tile_load_q<HD, TILE_ROWS, L::LOADERS>(a, l, h, grp * TILE_ROWS, smem + L::Q, x);
             issued(&b_q_full);
             for (int i = wk.i0; i < wk.i1; i++) {
                 const int row0 = i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K;
                 const int ks = kc % L::STAGES, vs = vc % L::STAGES;
                 if (kc >= L::STAGES && !wait_free(&b_k_free[ks], (kc / L::STAGES - 1) & 1)) { ok = false; break; }
-                tile_load<KT, HD>(a, k, row0, n, smem + L::K + ks * L::PARTS * L::SIDE, x);
+                tile_load<KT, HD, L::LOADERS>(a, k, row0, n, smem + L::K + ks * L::PARTS * L::SIDE, x);
                 issued(&b_k_full[ks]);
                 kc++;
                 if (vc >= L::STAGES && !wait_free(&b_v_free[vs], (vc / L::STAGES - 1) & 1)) { ok = false; break; }
-                tile_load<KT, HD>(a, v, row0, n, smem + L::V + vs * L::PARTS * L::SIDE, x);
+                tile_load<KT, HD, L::LOADERS>(a, v, row0, n, smem + L::V + vs * L::PARTS * L::SIDE, x);
                 for (int y = x; want_pos && y < TILE_K; y += L::LOADERS) {      /* with V: free once the weights are made */
                     const bool in = row0 + y < n;
                     cp_async4(smem + L::POS + (vs * TILE_K + y) * 4, pos + (in ? row0 + y : 0), in ? 4u : 0u);
@@ -836,6 +841,238 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             __syncwarp();
         }
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+/* ------------------------------------------------------------------ */
+/* Masses                                                               */
+/* ------------------------------------------------------------------ */
+
+constexpr int MASS_TILE_THREADS = 256;
+template <int KT, int HD>
+struct MassTileLayout {
+    using T = TileLayout<KT, HD>;
+    static constexpr int K = 0, Q = T::PARTS * T::SIDE;           /* two query tiles */
+    static constexpr int COLS = Q + 2 * T::SIDE;                  /* per query row: -log2 of its denominator, slope, position */
+    static constexpr int SUM = COLS + 3 * 3 * TILE_Q * 4;         /* three tiles': the next is written while one is slow to read the last */
+    static constexpr int BYTES = SUM + TILE_K * 4 + 1024;
+};
+
+/* The scores again, now with the denominators known: S^T = K Q^T with the 128
+ * cache rows as the matrix rows, so a thread owns a cache row and adds up its
+ * weights over the query rows as they come by, 128 a tile, in one order; no
+ * weight leaves the thread.  Two threads share a cache row (64 columns each).
+ * While a tile's weights are made, the next one's product runs. */
+template <int KT, int HD, bool EXTRA>
+__global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArgs a) {
+    using L = TileLayout<KT, HD>;
+    using M = MassTileLayout<KT, HD>;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t b_done[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_abort;
+    __shared__ int s_first[MASS_TILE_THREADS / 32];
+    const int tid = threadIdx.x, lane = tid & 31, w = uniform(tid >> 5), row = tid & (TILE_K - 1), half = tid >> 7;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *const base = smem_raw + (smem - smem_u32(smem_raw));
+    float *const s_cols = reinterpret_cast<float *>(base + M::COLS);        /* [3][3][128] */
+    float *const s_sum = reinterpret_cast<float *>(base + M::SUM);
+    const int u = blockIdx.y, l = u / a.n_head_kv, h = u - l * a.n_head_kv, R = a.T * a.G;
+    const int n = uniform(attend_rows(a, u));
+    const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
+    const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride;
+    const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
+    const ScoreMap map(a);
+    if (blockIdx.x * TILE_K >= n) return;
+    if (tid == 0) {
+        mbar_init(&b_done[0], 1);
+        mbar_init(&b_done[1], 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (w == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    /* the earliest position that some token's window reaches */
+    int first = INT_MAX;
+    if (EXTRA && a.window > 0) {
+        for (int t = tid; t < a.T; t += MASS_TILE_THREADS) first = min(first, a.tok_pos[l * a.tok_pos_stride + t]);
+        first = __reduce_min_sync(0xffffffffu, first);
+        if (lane == 0) s_first[w] = first;
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (EXTRA && a.window > 0)
+        for (int i = 0; i < MASS_TILE_THREADS / 32; i++) first = min(first, s_first[i]);
+    const uint32_t tmem = uniform(s_tmem);
+    uint32_t done = 0;                                        /* products issued so far, of the whole block */
+    bool ok = true;
+    for (int j0 = blockIdx.x * TILE_K; ok && j0 < n; j0 += gridDim.x * TILE_K) {
+        const int j = j0 + row, pj = want_pos && j < n ? pos[j] : 0;
+        const bool near = j < n && (!EXTRA || a.window <= 0 || pj >= (int64_t)first - a.window || pj < a.sink);
+        uint64_t sum = 0ull;
+        /* by order, token t sees row j only if j <= n - T + t: query rows before that see none of the tile */
+        const int q_from = a.tree ? 0 : max(0, j0 - (n - a.T)) * a.G / TILE_Q * TILE_Q;
+        const int tiles = R > q_from ? (R - q_from + TILE_Q - 1) / TILE_Q : 0;
+        if (__syncthreads_or(near) && tiles > 0) {
+            auto load = [&](int i) {                          /* query tile i and its columns' constants */
+                const int r0 = q_from + i * TILE_Q;
+                tile_load_q<HD, TILE_Q, MASS_TILE_THREADS>(a, l, h, r0, smem + M::Q + (i & 1) * L::SIDE, tid);
+                if (tid < TILE_Q) {
+                    const int r = r0 + tid;
+                    const bool in = r < R;
+                    const float2 nm = in ? a.norm[(int64_t)u * R + r] : make_float2(0.0f, 0.0f);
+                    float *c = s_cols + (i % 3) * 3 * TILE_Q + tid;
+                    c[0] = log2f(nm.y) - nm.x;
+                    if (EXTRA) {
+                        c[TILE_Q] = in && a.slopes ? -LOG2E * a.slopes[h * a.G + r % a.G] : 0.0f;
+                        c[2 * TILE_Q] = __int_as_float(in && want_pos ? a.tok_pos[l * a.tok_pos_stride + r / a.G] : 0);
+                    }
+                }
+            };
+            const uint32_t lead = tid == 0;
+            auto product = [&](int i) {
+                if (w != 0) return;
+                const uint32_t dk = tile_desc(smem + M::K, 16), dq = tile_desc(smem + M::Q + (i & 1) * L::SIDE, 16);
+                tc_fence_after();
+#pragma unroll
+                for (int s = 0; s < L::PARTS * (HD / 16); s++) {
+                    constexpr int PER = HD / 16;
+                    const int off = ((s % PER) / 4) * (L::PANEL >> 4) + (s % 4) * (32 >> 4);
+                    tc_mma_ss(lead, tmem + TILE_Q * (i & 1), dk + (s / PER) * (L::SIDE >> 4) + off, dq + off,
+                              tile_idesc(TILE_Q, false), s > 0);
+                }
+                tc_commit(lead, &b_done[(done + i) & 1]);
+            };
+            auto ready = [&]() {                              /* what was copied is there for all, and for the product */
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_async_smem();
+                tc_fence_before();
+                __syncthreads();
+            };
+            tile_load<KT, HD, MASS_TILE_THREADS>(a, k, j0, n, smem + M::K, tid);
+            load(0);
+            ready();
+            product(0);
+            for (int i = 0; i < tiles; i++) {
+                if (i + 1 < tiles) load(i + 1);
+                if (!tile_wait(&b_done[(done + i) & 1], ((done + i) >> 1) & 1, &s_abort, a.status)) ok = false;
+                if (i + 1 < tiles) {
+                    ready();                                  /* everyone is done with the product before this one, too */
+                    product(i + 1);
+                }
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; continue; }
+                tc_fence_after();
+                const int r0 = q_from + i * TILE_Q + 64 * half;
+                uint32_t v[64];
+                tc_ld64(v, tmem + ((uint32_t)(w & 3) << 21) + TILE_Q * (i & 1) + 64 * half);
+                tc_wait_ld();
+                const float *c = s_cols + (i % 3) * 3 * TILE_Q + 64 * half;
+                uint64_t mul = pair(map.scale, map.scale);
+                if (EXTRA) {
+                    float far = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const float2 z = unpair(mul2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), mul));
+                        v[2 * e] = __float_as_uint(z.x);
+                        v[2 * e + 1] = __float_as_uint(z.y);
+                        far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
+                    }
+                    mul = pair(1.0f, 1.0f);
+                    if (map.cap > 0.0f) {
+                        if (__any_sync(0xffffffffu, !(far < 0.4f))) {
+#pragma unroll
+                            for (int e = 0; e < 64; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
+                        } else {
+                            const uint64_t cap = pair(map.cap, map.cap);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) {
+                                const float2 z = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
+                                v[2 * e] = __float_as_uint(z.x);
+                                v[2 * e + 1] = __float_as_uint(z.y);
+                            }
+                        }
+                    }
+                    if (want_pos) {
+#pragma unroll
+                        for (int e = 0; e < 64; e++) {
+                            const int tp = __float_as_int(c[2 * TILE_Q + e]);
+                            float y = fmaf(c[TILE_Q + e], (float)(tp - pj), __uint_as_float(v[e]));
+                            if (a.window > 0 && !(pj >= (int64_t)tp - a.window || pj < a.sink)) y = -INFINITY;
+                            v[e] = __float_as_uint(y);
+                        }
+                    }
+                }
+                if (j0 + TILE_K > n - a.T || r0 + 64 > R) {   /* some query rows of these see the cache row, not all */
+                    const int own = j - (n - a.T);
+                    uint64_t bits = R - r0 >= 64 ? ~0ull : R > r0 ? (1ull << (R - r0)) - 1ull : 0ull;
+                    if (j >= n) bits = 0ull;
+                    if (own > 0 && !a.tree) {
+                        const int skip = own * a.G - r0;      /* tokens before `own` do not see it */
+                        bits &= skip >= 64 ? 0ull : skip > 0 ? ~0ull << skip : ~0ull;
+                    }
+                    if (own >= 0 && a.tree && j < n) {
+                        int t = r0 / a.G, g = r0 - t * a.G;
+                        bool see = false;
+#pragma unroll 1
+                        for (int e = 0; e < 64 && r0 + e < R; e++) {
+                            if (e == 0 || g == 0)
+                                see = a.tree[l * a.tree_stride + (int64_t)t * a.tree_words + (own >> 5)] >> (own & 31) & 1u;
+                            if (!see) bits &= ~(1ull << e);
+                            if (++g == a.G) { g = 0; t++; }
+                        }
+                    }
+                    if (!EXTRA) {                             /* a masked score stays masked only once it is final */
+#pragma unroll
+                        for (int e = 0; e < 64; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
+                        mul = pair(1.0f, 1.0f);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 64; e++)
+                        if (!(bits >> e & 1ull)) v[e] = 0xff800000u;
+                }
+                uint64_t part[2] = {0ull, 0ull};
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float4 nc = reinterpret_cast<const float4 *>(c)[e];
+                    const float2 x = unpair(fma2(pair(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1])), mul, pair(nc.x, nc.y)));
+                    const float2 y = unpair(fma2(pair(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])), mul, pair(nc.z, nc.w)));
+                    part[0] = add2(part[0], pair(ex2(x.x), ex2(x.y)));
+                    part[1] = add2(part[1], pair(ex2(y.x), ex2(y.y)));
+                }
+                sum = add2(sum, add2(part[0], part[1]));
+            }
+            done += tiles;
+        }
+        const float2 s2 = unpair(sum);
+        if (half) s_sum[row] = s2.x + s2.y;
+        tc_fence_before();
+        __syncthreads();
+        if (!half && j < n) {
+            const float mass = s2.x + s2.y + s_sum[row];
+            const int64_t x = (int64_t)u * a.n_cells + j;
+            a.mass_out[x] = a.mass_in ? fmaf(a.mass_decay, a.mass_in[x], mass) : mass;
+        }
+        ok = !__syncthreads_or(!ok);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (w == 0) {
+        tc_fence_after();
+        if (s_abort) {                                        /* a product may still run: wait for it, within a bound */
+            if (lane == 0) {
+                mbar_init(&b_done[0], 1);
+                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            }
+            __syncwarp();
+            tc_commit(lane == 0, &b_done[0]);
+            mbar_wait(&b_done[0], 0);
+            __syncwarp();
+        }
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
     }
 }
 

@@ -386,6 +386,17 @@ static int launch_tile(tria_ctx *c, const AttendArgs &a, const AttendPlan &pl, c
 }
 
 template <int KT, int HD>
+static int launch_mass_tile(const AttendArgs &a, int units, cudaStream_t st) {
+    constexpr int smem = MassTileLayout<KT, HD>::BYTES;
+    const bool extra = a.softcap > 0.0f || a.window > 0 || a.slopes;
+    auto fn = extra ? k_mass_tile<KT, HD, true> : k_mass_tile<KT, HD, false>;
+    CUDA_TRY(raise_smem_limit((const void *)fn, smem));
+    const int gx = std::max(1, std::min((a.n_cells + TILE_K - 1) / TILE_K, 65535));
+    fn<<<dim3((unsigned)gx, (unsigned)units), MASS_TILE_THREADS, smem, st>>>(a);
+    return TRIA_OK;
+}
+
+template <int KT, int HD>
 static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStream_t st) {
     const int units = a.n_layer * a.n_head_kv;
     uint8_t *ws = c->d_attend;
@@ -417,6 +428,9 @@ static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStre
         if (pl.keep_scores && a.T > 0) {
             const int gx = std::max(1, std::min((a.n_cells + 255) / 256, 8 * c->sm_count / std::min(units, 8 * c->sm_count)));
             k_mass_scores<<<dim3((unsigned)gx, (unsigned)units), 256, 0, st>>>(a);
+        } else if (pl.tile) {
+            const int rc = launch_mass_tile<KT, HD>(a, units, st);
+            if (rc) return rc;
         } else {
             const int gx = std::max(1, std::min((a.n_cells + MASS_KEYS - 1) / MASS_KEYS, 65535));
             k_mass_tiles<KT, HD><<<dim3((unsigned)gx, (unsigned)units), MASS_THREADS, 0, st>>>(a);
