@@ -275,8 +275,9 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, ui
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-/* Byte offset of 16-byte chunk c (of a row's HD / 8) of row r in an operand. */
-__device__ __forceinline__ uint32_t tile_chunk(int r, int c) { return (c >> 3) * (TILE_K * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+/* Byte offset of 16-byte chunk c (of a row's HD / 8) of row r in an operand of PR rows. */
+template <int PR = TILE_K>
+__device__ __forceinline__ uint32_t tile_chunk(int r, int c) { return (c >> 3) * (PR * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
 
 /* Starts (f16) or does (q8_0) the copy of rows [r0, r0 + 128) of one side;
  * rows at and behind n become zeros. */
@@ -332,18 +333,18 @@ __device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p,
 }
 
 /* Starts the copy of query rows [r0, r0 + ROWS) of kv head h of cache l as
- * operands of 128 rows; rows at and behind R become zeros.  A warp copies 32 /
+ * operands of PR rows; rows at and behind R become zeros.  A warp copies 32 /
  * (HD / 8) rows at a time, token and head stepping along. */
-template <int HD, int ROWS, int LOADERS>
+template <int HD, int ROWS, int PR, int LOADERS>
 __device__ __forceinline__ void tile_load_q(const AttendArgs &a, int l, int h, int r0, uint32_t st, int x) {
-    constexpr int CH = HD / 8, RPW = 32 / CH, STEP = RPW * (LOADERS / 32), SIDE = HD / 64 * TILE_K * 128;
+    constexpr int CH = HD / 8, RPW = 32 / CH, STEP = RPW * (LOADERS / 32), SIDE = HD / 64 * PR * 128;
     const int c = x % CH, first = (x >> 5) * RPW + (x & 31) / CH, R = a.T * a.G;
     int r = r0 + first, t = r / a.G, g = r - t * a.G;
     const int dt = STEP / a.G, dg = STEP - dt * a.G;
     const __half *base = a.q + l * a.q_cache + (int64_t)h * a.G * a.q_head + 8 * c;
     for (int q = first; q < ROWS; q += STEP, r += STEP) {
         const bool in = r < R;
-        cp_async16(st + (q / TILE_Q) * SIDE + tile_chunk(q % TILE_Q, c), in ? base + t * a.q_tok + g * a.q_head : base, in ? 16u : 0u);
+        cp_async16(st + (q / PR) * SIDE + tile_chunk<PR>(q % PR, c), in ? base + t * a.q_tok + g * a.q_head : base, in ? 16u : 0u);
         t += dt;
         g += dg;
         if (g >= a.G) { g -= a.G; t++; }
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
             const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
             if (seg && !wait_free(&b_q_free, (seg - 1) & 1)) break;
-            tile_load_q<HD, TILE_ROWS, L::LOADERS>(a, l, h, grp * TILE_ROWS, smem + L::Q, x);
+            tile_load_q<HD, TILE_ROWS, TILE_Q, L::LOADERS>(a, l, h, grp * TILE_ROWS, smem + L::Q, x);
             issued(&b_q_full);
             for (int i = wk.i0; i < wk.i1; i++) {
                 const int row0 = i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K;
@@ -848,23 +849,26 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
 /* Masses                                                               */
 /* ------------------------------------------------------------------ */
 
-constexpr int MASS_TILE_THREADS = 256;
+constexpr int MASS_TILE_THREADS = 256, MASS_Q = 64, MASS_C = MASS_Q / 2;      /* query rows a tile, a thread */
 template <int KT, int HD>
 struct MassTileLayout {
     using T = TileLayout<KT, HD>;
+    static constexpr int QSIDE = HD / 64 * MASS_Q * 128;
     static constexpr int K = 0, Q = T::PARTS * T::SIDE;           /* two query tiles */
-    static constexpr int COLS = Q + 2 * T::SIDE;                  /* per query row: -log2 of its denominator, slope, position */
-    static constexpr int SUM = COLS + 3 * 3 * TILE_Q * 4;         /* three tiles': the next is written while one is slow to read the last */
+    static constexpr int COLS = Q + 2 * QSIDE;                   /* per query row: -log2 of its denominator, slope, position */
+    static constexpr int SUM = COLS + 3 * 3 * MASS_Q * 4;         /* three tiles': the next is written while one is slow to read the last */
     static constexpr int BYTES = SUM + TILE_K * 4 + 1024;
 };
 
 /* The scores again, now with the denominators known: S^T = K Q^T with the 128
  * cache rows as the matrix rows, so a thread owns a cache row and adds up its
- * weights over the query rows as they come by, 128 a tile, in one order; no
- * weight leaves the thread.  Two threads share a cache row (64 columns each).
- * While a tile's weights are made, the next one's product runs. */
+ * weights over the query rows as they come by, 64 a tile, in one order; no
+ * weight leaves the thread.  Two threads share a cache row (32 columns each).
+ * While a tile's weights are made, the next one's product runs; a block is
+ * short (one tile of cache rows against a few of query rows), so two of them
+ * share an SM and cover each other's start. */
 template <int KT, int HD, bool EXTRA>
-__global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArgs a) {
+__global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const AttendArgs a) {
     using L = TileLayout<KT, HD>;
     using M = MassTileLayout<KT, HD>;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -875,7 +879,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArg
     const int tid = threadIdx.x, lane = tid & 31, w = uniform(tid >> 5), row = tid & (TILE_K - 1), half = tid >> 7;
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *const base = smem_raw + (smem - smem_u32(smem_raw));
-    float *const s_cols = reinterpret_cast<float *>(base + M::COLS);        /* [3][3][128] */
+    float *const s_cols = reinterpret_cast<float *>(base + M::COLS);        /* [3][3][64] */
     float *const s_sum = reinterpret_cast<float *>(base + M::SUM);
     const int u = blockIdx.y, l = u / a.n_head_kv, h = u - l * a.n_head_kv, R = a.T * a.G;
     const int n = uniform(attend_rows(a, u));
@@ -891,7 +895,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArg
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (w == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 128;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_fence_before();
     }
@@ -914,35 +918,35 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArg
         const bool near = j < n && (!EXTRA || a.window <= 0 || pj >= (int64_t)first - a.window || pj < a.sink);
         uint64_t sum = 0ull;
         /* by order, token t sees row j only if j <= n - T + t: query rows before that see none of the tile */
-        const int q_from = a.tree ? 0 : max(0, j0 - (n - a.T)) * a.G / TILE_Q * TILE_Q;
-        const int tiles = R > q_from ? (R - q_from + TILE_Q - 1) / TILE_Q : 0;
+        const int q_from = a.tree ? 0 : max(0, j0 - (n - a.T)) * a.G / MASS_Q * MASS_Q;
+        const int tiles = R > q_from ? (R - q_from + MASS_Q - 1) / MASS_Q : 0;
         if (__syncthreads_or(near) && tiles > 0) {
             auto load = [&](int i) {                          /* query tile i and its columns' constants */
-                const int r0 = q_from + i * TILE_Q;
-                tile_load_q<HD, TILE_Q, MASS_TILE_THREADS>(a, l, h, r0, smem + M::Q + (i & 1) * L::SIDE, tid);
-                if (tid < TILE_Q) {
+                const int r0 = q_from + i * MASS_Q;
+                tile_load_q<HD, MASS_Q, MASS_Q, MASS_TILE_THREADS>(a, l, h, r0, smem + M::Q + (i & 1) * M::QSIDE, tid);
+                if (tid < MASS_Q) {
                     const int r = r0 + tid;
                     const bool in = r < R;
                     const float2 nm = in ? a.norm[(int64_t)u * R + r] : make_float2(0.0f, 0.0f);
-                    float *c = s_cols + (i % 3) * 3 * TILE_Q + tid;
+                    float *c = s_cols + (i % 3) * 3 * MASS_Q + tid;
                     c[0] = log2f(nm.y) - nm.x;
                     if (EXTRA) {
-                        c[TILE_Q] = in && a.slopes ? -LOG2E * a.slopes[h * a.G + r % a.G] : 0.0f;
-                        c[2 * TILE_Q] = __int_as_float(in && want_pos ? a.tok_pos[l * a.tok_pos_stride + r / a.G] : 0);
+                        c[MASS_Q] = in && a.slopes ? -LOG2E * a.slopes[h * a.G + r % a.G] : 0.0f;
+                        c[2 * MASS_Q] = __int_as_float(in && want_pos ? a.tok_pos[l * a.tok_pos_stride + r / a.G] : 0);
                     }
                 }
             };
             const uint32_t lead = tid == 0;
             auto product = [&](int i) {
                 if (w != 0) return;
-                const uint32_t dk = tile_desc(smem + M::K, 16), dq = tile_desc(smem + M::Q + (i & 1) * L::SIDE, 16);
+                const uint32_t dk = tile_desc(smem + M::K, 16), dq = tile_desc(smem + M::Q + (i & 1) * M::QSIDE, 16);
                 tc_fence_after();
 #pragma unroll
                 for (int s = 0; s < L::PARTS * (HD / 16); s++) {
                     constexpr int PER = HD / 16;
-                    const int off = ((s % PER) / 4) * (L::PANEL >> 4) + (s % 4) * (32 >> 4);
-                    tc_mma_ss(lead, tmem + TILE_Q * (i & 1), dk + (s / PER) * (L::SIDE >> 4) + off, dq + off,
-                              tile_idesc(TILE_Q, false), s > 0);
+                    const int panel = (s % PER) / 4, in = (s % 4) * (32 >> 4);
+                    tc_mma_ss(lead, tmem + MASS_Q * (i & 1), dk + (s / PER) * (L::SIDE >> 4) + panel * (L::PANEL >> 4) + in,
+                              dq + panel * (MASS_Q * 128 >> 4) + in, tile_idesc(MASS_Q, false), s > 0);
                 }
                 tc_commit(lead, &b_done[(done + i) & 1]);
             };
@@ -966,16 +970,16 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArg
                 }
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; continue; }
                 tc_fence_after();
-                const int r0 = q_from + i * TILE_Q + 64 * half;
-                uint32_t v[64];
-                tc_ld64(v, tmem + ((uint32_t)(w & 3) << 21) + TILE_Q * (i & 1) + 64 * half);
+                const int r0 = q_from + i * MASS_Q + MASS_C * half;
+                uint32_t v[MASS_C];
+                tc_ld32(v, tmem + ((uint32_t)(w & 3) << 21) + MASS_Q * (i & 1) + MASS_C * half);
                 tc_wait_ld();
-                const float *c = s_cols + (i % 3) * 3 * TILE_Q + 64 * half;
+                const float *c = s_cols + (i % 3) * 3 * MASS_Q + MASS_C * half;
                 uint64_t mul = pair(map.scale, map.scale);
                 if (EXTRA) {
                     float far = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
+                    for (int e = 0; e < MASS_C / 2; e++) {
                         const float2 z = unpair(mul2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), mul));
                         v[2 * e] = __float_as_uint(z.x);
                         v[2 * e + 1] = __float_as_uint(z.y);
@@ -985,11 +989,11 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArg
                     if (map.cap > 0.0f) {
                         if (__any_sync(0xffffffffu, !(far < 0.4f))) {
 #pragma unroll
-                            for (int e = 0; e < 64; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
+                            for (int e = 0; e < MASS_C; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
                         } else {
                             const uint64_t cap = pair(map.cap, map.cap);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) {
+                            for (int e = 0; e < MASS_C / 2; e++) {
                                 const float2 z = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
                                 v[2 * e] = __float_as_uint(z.x);
                                 v[2 * e + 1] = __float_as_uint(z.y);
@@ -998,45 +1002,45 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArg
                     }
                     if (want_pos) {
 #pragma unroll
-                        for (int e = 0; e < 64; e++) {
-                            const int tp = __float_as_int(c[2 * TILE_Q + e]);
-                            float y = fmaf(c[TILE_Q + e], (float)(tp - pj), __uint_as_float(v[e]));
+                        for (int e = 0; e < MASS_C; e++) {
+                            const int tp = __float_as_int(c[2 * MASS_Q + e]);
+                            float y = fmaf(c[MASS_Q + e], (float)(tp - pj), __uint_as_float(v[e]));
                             if (a.window > 0 && !(pj >= (int64_t)tp - a.window || pj < a.sink)) y = -INFINITY;
                             v[e] = __float_as_uint(y);
                         }
                     }
                 }
-                if (j0 + TILE_K > n - a.T || r0 + 64 > R) {   /* some query rows of these see the cache row, not all */
+                if (j0 + TILE_K > n - a.T || r0 + MASS_C > R) {   /* some query rows of these see the cache row, not all */
                     const int own = j - (n - a.T);
-                    uint64_t bits = R - r0 >= 64 ? ~0ull : R > r0 ? (1ull << (R - r0)) - 1ull : 0ull;
-                    if (j >= n) bits = 0ull;
+                    uint32_t bits = R - r0 >= 32 ? ~0u : R > r0 ? (1u << (R - r0)) - 1u : 0u;
+                    if (j >= n) bits = 0u;
                     if (own > 0 && !a.tree) {
                         const int skip = own * a.G - r0;      /* tokens before `own` do not see it */
-                        bits &= skip >= 64 ? 0ull : skip > 0 ? ~0ull << skip : ~0ull;
+                        bits &= skip >= 32 ? 0u : skip > 0 ? ~0u << skip : ~0u;
                     }
                     if (own >= 0 && a.tree && j < n) {
                         int t = r0 / a.G, g = r0 - t * a.G;
                         bool see = false;
 #pragma unroll 1
-                        for (int e = 0; e < 64 && r0 + e < R; e++) {
+                        for (int e = 0; e < MASS_C && r0 + e < R; e++) {
                             if (e == 0 || g == 0)
                                 see = a.tree[l * a.tree_stride + (int64_t)t * a.tree_words + (own >> 5)] >> (own & 31) & 1u;
-                            if (!see) bits &= ~(1ull << e);
+                            if (!see) bits &= ~(1u << e);
                             if (++g == a.G) { g = 0; t++; }
                         }
                     }
                     if (!EXTRA) {                             /* a masked score stays masked only once it is final */
 #pragma unroll
-                        for (int e = 0; e < 64; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
+                        for (int e = 0; e < MASS_C; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * map.scale);
                         mul = pair(1.0f, 1.0f);
                     }
 #pragma unroll
-                    for (int e = 0; e < 64; e++)
-                        if (!(bits >> e & 1ull)) v[e] = 0xff800000u;
+                    for (int e = 0; e < MASS_C; e++)
+                        if (!(bits >> e & 1u)) v[e] = 0xff800000u;
                 }
                 uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
+                for (int e = 0; e < MASS_C / 4; e++) {
                     const float4 nc = reinterpret_cast<const float4 *>(c)[e];
                     const float2 x = unpair(fma2(pair(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1])), mul, pair(nc.x, nc.y)));
                     const float2 y = unpair(fma2(pair(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])), mul, pair(nc.z, nc.w)));
@@ -1072,7 +1076,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS) k_mass_tile(const AttendArg
             mbar_wait(&b_done[0], 0);
             __syncwarp();
         }
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem) : "memory");
     }
 }
 
