@@ -282,6 +282,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_attend_plan(const AttendArgs a
         const int64_t lo = (int64_t)first - a.window;
         const int32_t *pos = a.pos + (a.pos_shared ? 0 : (int64_t)u * a.n_cells);
         int tail = n, head = 0;
+#pragma unroll 8
         for (int j = threadIdx.x; j < n; j += PLAN_THREADS) {
             const int p = pos[j];
             if (p >= lo) tail = min(tail, j);

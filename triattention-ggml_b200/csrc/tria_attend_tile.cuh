@@ -235,36 +235,33 @@ __device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volati
     return true;
 }
 
-/* A q8_0 block's 32 values from p (2-byte aligned) as f16 pairs, the value
- * rounded (hi) and its remainder (lo = q d - hi, exact in one f16 fma). */
-__device__ __forceinline__ void dequant_block(const uint8_t *p, uint32_t (&hi)[16], uint32_t (&lo)[16]) {
-    uint32_t w[8];
-    __half d;
+/* A q8_0 block as nine words in registers (2-byte aligned in memory: a block
+ * on a 4-byte boundary as it lies, others as the scale and the eight words
+ * behind it), and its 32 values from them as f16 pairs: the value rounded (hi)
+ * and its remainder (lo = q d - hi, exact in one f16 fma). */
+__device__ __forceinline__ void block_words(const uint8_t *p, uint32_t (&x)[9]) {
     if (((uintptr_t)p & 2) == 0) {
         const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
-        uint32_t x = __ldg(q);
-        d = __ushort_as_half((unsigned short)x);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t y = i < 7 ? __ldg(q + i + 1) : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(q + 8));
-            w[i] = __funnelshift_r(x, y, 16);
-            x = y;
-        }
+        for (int i = 0; i < 8; i++) x[i] = __ldg(q + i);
+        x[8] = __ldg(reinterpret_cast<const uint16_t *>(q + 8));
     } else {
-        d = __ushort_as_half(__ldg(reinterpret_cast<const uint16_t *>(p)));
         const uint32_t *q = reinterpret_cast<const uint32_t *>(p + 2);
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = __ldg(q + i);
+        for (int i = 0; i < 8; i++) x[i] = __ldg(q + i);
+        x[8] = __ldg(reinterpret_cast<const uint16_t *>(p));
     }
-    const __half2 dd = __half2half2(d);
+}
+__device__ __forceinline__ void block_values(const uint32_t (&x)[9], bool even, uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+    const __half2 d = __half2half2(__ushort_as_half((unsigned short)(even ? x[0] : x[8])));
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        uint32_t x[2];
-        int8x4_half(w[i], x[0], x[1]);
+        uint32_t y[2];
+        int8x4_half(even ? __funnelshift_r(x[i], x[i + 1], 16) : x[i], y[0], y[1]);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const __half2 q = *reinterpret_cast<const __half2 *>(&x[j]);
-            const __half2 h = __hmul2(q, dd), r = __hfma2(q, dd, __hneg2(h));
+            const __half2 q = *reinterpret_cast<const __half2 *>(&y[j]);
+            const __half2 h = __hmul2(q, d), r = __hfma2(q, d, __hneg2(h));
             hi[2 * i + j] = *reinterpret_cast<const uint32_t *>(&h);
             lo[2 * i + j] = *reinterpret_cast<const uint32_t *>(&r);
         }
@@ -279,58 +276,72 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, ui
 template <int PR = TILE_K>
 __device__ __forceinline__ uint32_t tile_chunk(int r, int c) { return (c >> 3) * (PR * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
 
-/* Starts (f16) or does (q8_0) the copy of rows [r0, r0 + 128) of one side;
- * rows at and behind n become zeros. */
-template <int KT, int HD, int LOADERS>
-__device__ __forceinline__ void tile_load(const AttendArgs &a, const uint8_t *p, int r0, int n, uint32_t st, int x) {
-    using L = TileLayout<KT, HD>;
-    if constexpr (KT == KT_F16) {
-        constexpr int CH = HD / 8, RPW = 32 / CH, NW = LOADERS / 32;      /* rows a warp copies at a time */
-        if (a.copy16) {
-            const int w = x >> 5, r = (x & 31) / CH, c = x % CH;
-            const uint8_t *s = p + (int64_t)(r0 + r + RPW * w) * a.cell_stride + 16 * c;
-            const int64_t step = (int64_t)RPW * NW * a.cell_stride;
-            if (r0 + TILE_K <= n) {
+/* f16: starts the copy of rows [r0, r0 + 128) of one side; rows at and behind
+ * n become zeros. */
+template <int HD, int LOADERS>
+__device__ __forceinline__ void tile_copy(const AttendArgs &a, const uint8_t *p, int r0, int n, uint32_t st, int x) {
+    constexpr int CH = HD / 8, RPW = 32 / CH, NW = LOADERS / 32;      /* rows a warp copies at a time */
+    if (a.copy16) {
+        const int w = x >> 5, r = (x & 31) / CH, c = x % CH;
+        const uint8_t *s = p + (int64_t)(r0 + r + RPW * w) * a.cell_stride + 16 * c;
+        const int64_t step = (int64_t)RPW * NW * a.cell_stride;
+        if (r0 + TILE_K <= n) {
 #pragma unroll 4
-                for (int y = r + RPW * w; y < TILE_K; y += RPW * NW) {
-                    cp_async16(st + tile_chunk(y, c), s, 16u);
-                    s += step;
-                }
-            } else {
-                for (int y = r + RPW * w; y < TILE_K; y += RPW * NW) {
-                    const bool in = r0 + y < n;
-                    cp_async16(st + tile_chunk(y, c), in ? s : p, in ? 16u : 0u);
-                    s += step;
-                }
+            for (int y = r + RPW * w; y < TILE_K; y += RPW * NW) {
+                cp_async16(st + tile_chunk(y, c), s, 16u);
+                s += step;
             }
         } else {
-            for (int y = x; y < TILE_K * CH * 4; y += LOADERS) {
-                const int r = y / (CH * 4), c = y / 4 % CH, q = y & 3;
-                const bool in = r0 + r < n;
-                cp_async4(st + tile_chunk(r, c) + 4 * q, p + (in ? (int64_t)(r0 + r) * a.cell_stride + 16 * c + 4 * q : 0), in ? 4u : 0u);
+            for (int y = r + RPW * w; y < TILE_K; y += RPW * NW) {
+                const bool in = r0 + y < n;
+                cp_async16(st + tile_chunk(y, c), in ? s : p, in ? 16u : 0u);
+                s += step;
             }
         }
     } else {
-        constexpr int NB = HD / 32;
-#pragma unroll 1
-        for (int y = x; y < TILE_K * NB; y += LOADERS) {
-            const int r = y / NB, b = y % NB;
-            uint32_t hi[16], lo[16];
-            if (r0 + r < n) {
-                dequant_block(p + (int64_t)(r0 + r) * a.cell_stride + 34 * b, hi, lo);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; i++) hi[i] = lo[i] = 0;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t d = st + tile_chunk(r, 4 * b + i);
-                sts128(d, hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-                sts128(d + L::SIDE, lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-            }
+        for (int y = x; y < TILE_K * CH * 4; y += LOADERS) {
+            const int r = y / (CH * 4), c = y / 4 % CH, q = y & 3;
+            const bool in = r0 + r < n;
+            cp_async4(st + tile_chunk(r, c) + 4 * q, p + (in ? (int64_t)(r0 + r) * a.cell_stride + 16 * c + 4 * q : 0), in ? 4u : 0u);
         }
     }
 }
+
+/* q8_0: one side's blocks on their way through registers, so that the reads of
+ * a tile are out before its buffer is free.  A thread's blocks are the same
+ * one of their rows (LOADERS is a multiple of the blocks in a row). */
+template <int HD, int LOADERS>
+struct TileBlocks {
+    static constexpr int NB = HD / 32, PER = (TILE_K * NB + LOADERS - 1) / LOADERS;
+    uint32_t x[PER][9];
+    __device__ __forceinline__ void read(const AttendArgs &a, const uint8_t *p, int r0, int n, int tid) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int y = tid + i * LOADERS, r = y / NB;
+            if (y < TILE_K * NB && r0 + r < n) {
+                block_words(p + (int64_t)(r0 + r) * a.cell_stride + 34 * (y % NB), x[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 9; e++) x[i][e] = 0;      /* value 0, scale 0 */
+            }
+        }
+    }
+    __device__ __forceinline__ void write(uint32_t st, uint32_t part, int tid) const {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int y = tid + i * LOADERS, r = y / NB, b = y % NB;
+            if (y >= TILE_K * NB) break;
+            uint32_t hi[16], lo[16];
+            block_values(x[i], (b & 1) == 0, hi, lo);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t d = st + tile_chunk(r, 4 * b + e);
+                sts128(d, hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
+                sts128(d + part, lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]);
+            }
+        }
+    }
+};
 
 /* Starts the copy of query rows [r0, r0 + ROWS) of kv head h of cache l as
  * operands of PR rows; rows at and behind R become zeros.  A warp copies 32 /
@@ -452,12 +463,20 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             for (int i = wk.i0; i < wk.i1; i++) {
                 const int row0 = i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K;
                 const int ks = kc % L::STAGES, vs = vc % L::STAGES;
+                const uint32_t k_at = smem + L::K + ks * L::PARTS * L::SIDE, v_at = smem + L::V + vs * L::PARTS * L::SIDE;
+                TileBlocks<HD, L::LOADERS> kb, vb;            /* q8_0 only */
+                if (KT == KT_Q8_0) {
+                    kb.read(a, k, row0, n, x);
+                    vb.read(a, v, row0, n, x);
+                }
                 if (kc >= L::STAGES && !wait_free(&b_k_free[ks], (kc / L::STAGES - 1) & 1)) { ok = false; break; }
-                tile_load<KT, HD, L::LOADERS>(a, k, row0, n, smem + L::K + ks * L::PARTS * L::SIDE, x);
+                if (KT == KT_F16) tile_copy<HD, L::LOADERS>(a, k, row0, n, k_at, x);
+                else kb.write(k_at, L::SIDE, x);
                 issued(&b_k_full[ks]);
                 kc++;
                 if (vc >= L::STAGES && !wait_free(&b_v_free[vs], (vc / L::STAGES - 1) & 1)) { ok = false; break; }
-                tile_load<KT, HD, L::LOADERS>(a, v, row0, n, smem + L::V + vs * L::PARTS * L::SIDE, x);
+                if (KT == KT_F16) tile_copy<HD, L::LOADERS>(a, v, row0, n, v_at, x);
+                else vb.write(v_at, L::SIDE, x);
                 for (int y = x; want_pos && y < TILE_K; y += L::LOADERS) {      /* with V: free once the weights are made */
                     const bool in = row0 + y < n;
                     cp_async4(smem + L::POS + (vs * TILE_K + y) * 4, pos + (in ? row0 + y : 0), in ? 4u : 0u);
@@ -957,7 +976,13 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
                 tc_fence_before();
                 __syncthreads();
             };
-            tile_load<KT, HD, MASS_TILE_THREADS>(a, k, j0, n, smem + M::K, tid);
+            if (KT == KT_F16) {
+                tile_copy<HD, MASS_TILE_THREADS>(a, k, j0, n, smem + M::K, tid);
+            } else {
+                TileBlocks<HD, MASS_TILE_THREADS> kb;
+                kb.read(a, k, j0, n, tid);
+                kb.write(smem + M::K, L::SIDE, tid);
+            }
             load(0);
             ready();
             product(0);
