@@ -109,16 +109,44 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
 }
-/* tanh_small of both. */
+/* tanh_small of both; SHORT: two terms less, the first omitted one is below
+ * 2^-29 at |u| = 0.2. */
+template <bool SHORT>
 __device__ __forceinline__ uint64_t tanh_small2(uint64_t u) {
     const uint64_t z = mul2(u, u);
-    uint64_t s = pair(21844.0f / 6081075.0f, 21844.0f / 6081075.0f);
-    s = fma2(s, z, pair(-1382.0f / 155925.0f, -1382.0f / 155925.0f));
-    s = fma2(s, z, pair(62.0f / 2835.0f, 62.0f / 2835.0f));
+    uint64_t s = pair(62.0f / 2835.0f, 62.0f / 2835.0f);
+    if (!SHORT) {
+        s = pair(21844.0f / 6081075.0f, 21844.0f / 6081075.0f);
+        s = fma2(s, z, pair(-1382.0f / 155925.0f, -1382.0f / 155925.0f));
+        s = fma2(s, z, pair(62.0f / 2835.0f, 62.0f / 2835.0f));
+    }
     s = fma2(s, z, pair(-17.0f / 315.0f, -17.0f / 315.0f));
     s = fma2(s, z, pair(2.0f / 15.0f, 2.0f / 15.0f));
     s = fma2(s, z, pair(-1.0f / 3.0f, -1.0f / 3.0f));
     return fma2(mul2(s, z), u, u);
+}
+/* Caps N scores u = s / c (as bits), the largest magnitude being `far`: c tanh u. */
+template <int N>
+__device__ __forceinline__ void tile_cap(uint32_t (&v)[N], float c, float far) {
+    const uint64_t cc = pair(c, c);
+    if (__any_sync(0xffffffffu, !(far < 0.4f))) {
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = __float_as_uint(c * tanh_both(__uint_as_float(v[e])));
+    } else if (__any_sync(0xffffffffu, far > 0.2f)) {
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) {
+            const float2 z = unpair(mul2(cc, tanh_small2<false>(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
+            v[2 * e] = __float_as_uint(z.x);
+            v[2 * e + 1] = __float_as_uint(z.y);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) {
+            const float2 z = unpair(mul2(cc, tanh_small2<true>(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
+            v[2 * e] = __float_as_uint(z.x);
+            v[2 * e + 1] = __float_as_uint(z.y);
+        }
+    }
 }
 /* N scores x (as bits) to weights 2^(x mul - from) in f16 pairs; their fp32 sums go to `sum`. */
 template <int N>
@@ -639,20 +667,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                         v[2 * e + 1] = __float_as_uint(z.y);
                         far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
                     }
-                    if (map.cap > 0.0f) {
-                        const uint64_t cap = pair(map.cap, map.cap);
-                        if (__any_sync(0xffffffffu, !(far < 0.4f))) {
-#pragma unroll
-                            for (int e = 0; e < TILE_H; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < TILE_H / 2; e++) {
-                                const float2 z = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
-                                v[2 * e] = __float_as_uint(z.x);
-                                v[2 * e + 1] = __float_as_uint(z.y);
-                            }
-                        }
-                    }
+                    if (map.cap > 0.0f) tile_cap<TILE_H>(v, map.cap, far);
                     mul = pair(1.0f, 1.0f);
                 }
                 if (want_pos || !all || (!EXTRA && map.scale <= 0.0f)) {
@@ -800,23 +815,23 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                         const bool none = ss == 0.0f;
                         const float inv = none ? 0.0f : 1.0f / ss;
                         float fin = 0.0f;
-                        __half *dst = a.out + l * a.o_cache + tq * a.o_tok + hq * a.o_head;
+                        uint4 *dst = reinterpret_cast<uint4 *>(a.out + l * a.o_cache + tq * a.o_tok + hq * a.o_head);
 #pragma unroll 1
-                        for (int c = 0; c < HD / 16; c++) {
-                            float4 acc[4];
+                        for (int part = 0; part < HD / 32; part++) {     /* 32 dims at a time stay in registers */
+                            float4 acc[8];
 #pragma unroll
-                            for (int e = 0; e < 4; e++) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
+                            for (int e = 0; e < 8; e++) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
                             for (int s = 0; s < nS; s++) {
                                 const float2 y = __ldcg(&a.part_ml[slot_of(s) * TILE_ROWS + tid]);
-                                const float g = y.x == -INFINITY ? 0.0f : ex2(y.x - mm);
-                                float4 o[4];
+                                const float4 *src = reinterpret_cast<const float4 *>(a.part_o) + (slot_of(s) * (HD / 4) + 8 * part) * TILE_ROWS + tid;
+                                float4 o[8];
 #pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    o[e] = __ldcg(reinterpret_cast<const float4 *>(a.part_o) + (slot_of(s) * (HD / 4) + 4 * c + e) * TILE_ROWS + tid);
+                                for (int e = 0; e < 8; e++) o[e] = __ldcg(src + e * TILE_ROWS);
+                                const float g = y.x == -INFINITY ? 0.0f : ex2(y.x - mm);
                                 if (g != 0.0f) {
 #pragma unroll
-                                    for (int e = 0; e < 4; e++) {
+                                    for (int e = 0; e < 8; e++) {
                                         acc[e].x = fmaf(o[e].x, g, acc[e].x);
                                         acc[e].y = fmaf(o[e].y, g, acc[e].y);
                                         acc[e].z = fmaf(o[e].z, g, acc[e].z);
@@ -824,16 +839,19 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                                     }
                                 }
                             }
-                            uint2 h2[4];
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const float x0 = none ? 0.0f : acc[e].x * inv, x1 = none ? 0.0f : acc[e].y * inv;
-                                const float x2 = none ? 0.0f : acc[e].z * inv, x3 = none ? 0.0f : acc[e].w * inv;
-                                fin += x0 * 0.0f + x1 * 0.0f + x2 * 0.0f + x3 * 0.0f;
-                                h2[e] = make_uint2(pack_half2(x0, x1), pack_half2(x2, x3));
+                            for (int e = 0; e < 8; e++) {
+                                if (none) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                acc[e].x *= inv;
+                                acc[e].y *= inv;
+                                acc[e].z *= inv;
+                                acc[e].w *= inv;
+                                fin += acc[e].x * 0.0f + acc[e].y * 0.0f + acc[e].z * 0.0f + acc[e].w * 0.0f;
                             }
-                            reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(h2[0].x, h2[0].y, h2[1].x, h2[1].y);
-                            reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(h2[2].x, h2[2].y, h2[3].x, h2[3].y);
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2)
+                                dst[4 * part + e / 2] = make_uint4(pack_half2(acc[e].x, acc[e].y), pack_half2(acc[e].z, acc[e].w),
+                                                                   pack_half2(acc[e + 1].x, acc[e + 1].y), pack_half2(acc[e + 1].z, acc[e + 1].w));
                         }
                         if (fin != 0.0f) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + rq;
                         if (a.lse) a.lse[((int64_t)l * a.T + tq) * a.n_head_kv * a.G + hq] = none ? -INFINITY : (mm - FEW_LIFT + log2f(ss)) * LN2;
@@ -1011,20 +1029,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
                         far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
                     }
                     mul = pair(1.0f, 1.0f);
-                    if (map.cap > 0.0f) {
-                        if (__any_sync(0xffffffffu, !(far < 0.4f))) {
-#pragma unroll
-                            for (int e = 0; e < MASS_C; e++) v[e] = __float_as_uint(map.cap * tanh_both(__uint_as_float(v[e])));
-                        } else {
-                            const uint64_t cap = pair(map.cap, map.cap);
-#pragma unroll
-                            for (int e = 0; e < MASS_C / 2; e++) {
-                                const float2 z = unpair(mul2(cap, tanh_small2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])))));
-                                v[2 * e] = __float_as_uint(z.x);
-                                v[2 * e + 1] = __float_as_uint(z.y);
-                            }
-                        }
-                    }
+                    if (map.cap > 0.0f) tile_cap<MASS_C>(v, map.cap, far);
                     if (want_pos) {
 #pragma unroll
                         for (int e = 0; e < MASS_C; e++) {

@@ -117,7 +117,7 @@ extern "C" TRIA_API int tria_append(tria_ctx *c, const tria_kv_view *v, const in
     if ((rc = note_capture(c, st)) < 0) return rc;
     /* enough blocks per unit to fill the GPU; one when the rows are few */
     const int rows_per_block = APPEND_THREADS / 32 * (256 / (int)c->hd);
-    const int want = std::max(1, 4 * c->sm_count / std::max(1, std::min(units_all, TRIA_MAX_UNITS)));
+    const int want = std::max(1, 16 * c->sm_count / std::max(1, std::min(units_all, TRIA_MAX_UNITS)));
     const int bx = std::max(1, std::min((p->n_tok + rows_per_block - 1) / rows_per_block, want));
     const bool later = alias && bx > 1;
     rc = for_cache_chunks(v, [&](int l0, int nl) -> int {
