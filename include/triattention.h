@@ -269,7 +269,8 @@ TRIA_API int64_t tria_ctx_launches(const tria_ctx *ctx);
 TRIA_API int tria_ctx_check(tria_ctx *ctx, void *stream);
 
 /* Fault-injection hook for tests of the timeout path: every pipeline wait of
- * the scoring kernel (TMA stages, partial buffers, position ring) gives up
+ * the scoring kernel (TMA stages, partial buffers, position ring) and of
+ * tria_attend's tensor-core kernels gives up
  * after `cycles` SM clock cycles instead of about a second, sets the
  * timeout status and lets the kernel return; copies already issued are
  * still waited for with the default bound before a block exits.  cycles <= 0

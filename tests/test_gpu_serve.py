@@ -353,6 +353,41 @@ def test_repeated_calls_give_the_same_bits(contexts, torch_dev):
             assert torch.equal(o, got[0][0]) and torch.equal(m, got[0][1])
 
 
+@pytest.mark.parametrize("type_id", [F16, Q8_0])
+def test_waits_that_give_up_are_reported(contexts, torch_dev, type_id):
+    """With a bound of one cycle the tensor-core kernels' pipeline waits give up:
+    the status says so, and the next call is right again."""
+    ctx = contexts(2, 4, 128)
+    c = Cache(type_id, 2, 2, 128, 3000, [3000, 2500, 1700, 2999], torch_dev)
+    T = 80
+    q = queries(2, T, 8, 128, torch_dev)
+    out, mass = torch.empty_like(q), torch.zeros((2, 2, 3000), device=torch_dev)
+    p, s = tria_b200.attend_params(128 ** -0.5), torch.cuda.current_stream()
+    ctx.attend(c.view(), c.rows, q, out, p, mass_out=mass, stream=s)        # sizes the workspace
+    ctx.check(s)
+    ctx.set_wait_limit(1)
+    try:
+        ctx.attend(c.view(), c.rows, q, out, p, mass_out=mass, stream=s)
+        with pytest.raises(tria_b200.TriaError) as e:
+            ctx.check(s)
+        assert e.value.status == tria_b200.ERR_TIMEOUT
+    finally:
+        ctx.set_wait_limit(0)
+    for _ in range(2):
+        ctx.attend(c.view(), c.rows, q, out, p, mass_out=mass, stream=s)
+        ctx.check(s)
+        attend_close(c, out, None, mass, attend_oracle(c, q, 128 ** -0.5))
+
+
+def test_every_value_not_finite(contexts, torch_dev):
+    """Values that every token sees: NaN results stand as they are, for any number of rows."""
+    for T in (1, 30, 200):
+        c = Cache(F16, 1, 2, 128, 2000, [1999, 1500], torch_dev)
+        c.unit(c.v, 0, 0).view(torch.float16)[100:200, 5] = float("nan")
+        out, _, _ = run_attend(contexts, c, 4, T, mass=False)
+        assert torch.isnan(out[0, :, :4, 5]).all() and not torch.isnan(out[0, :, 4:]).any()
+
+
 def test_binding_refuses_foreign_tensors(contexts, torch_dev):
     ctx = contexts(2, 4, 128)
     c = Cache(F16, 1, 2, 128, 64, [10, 5], torch_dev)

@@ -28,7 +28,7 @@ def view(**kw):
                                pos_shared=a["shared"], flags=a["flags"])
 
 
-def attend(L, v=None, n_rows=FAKE, q=FAKE, out=FAKE, lse=None, mass_in=None, mass_out=None, **kw):
+def attend(L, v=None, n_rows=FAKE, q=FAKE, out=2 * FAKE, lse=None, mass_in=None, mass_out=None, **kw):
     p = tria_b200.AttendParams()
     p.n_tok, p.scale, p.mass_decay = 1, 0.125, 1.0
     for k, x in kw.items():
@@ -92,6 +92,7 @@ def test_views(L, call, kw, word, status):
     (dict(reserved=1), "reserved"), (dict(scale=float("nan")), "finite"), (dict(softcap=-1.0), "softcap"),
     (dict(softcap=float("inf")), "finite"), (dict(mass_decay=float("inf")), "finite"),
     (dict(mass_in=FAKE), "mass_in without"), (dict(mass_out=FAKE + 2), "misaligned"), (dict(lse=FAKE + 2), "misaligned"),
+    (dict(out=FAKE), "overlap"), (dict(scale=3e38), "range"), (dict(scale=1e10, softcap=1e-30), "range"),
     (dict(q=None), "q or out"), (dict(out=FAKE + 8), "q or out"), (dict(q_tok_stride=4), "strides"),
     (dict(o_head_stride=-8), "strides"), (dict(slopes=FAKE), "tok_pos"), (dict(window=5), "tok_pos"),
     (dict(window=5, tok_pos=FAKE, tok_pos_stride=-1), "tok_pos_stride"), (dict(slopes=FAKE + 1, tok_pos=FAKE), "slopes"),

@@ -37,6 +37,7 @@ struct AttendArgs {
     int64_t tree_stride;
     int32_t tree_words;
     int32_t *status;
+    long long wait_limit;                /* cycles a pipeline wait may take before it gives up (ST_TIMEOUT) */
     /* plan and workspace (host-filled) */
     int32_t copy16;                      /* rows start on 16-byte boundaries (f16), 8-byte ones (q8_0) */
     int32_t groups;                      /* groups of query rows per unit */
@@ -213,6 +214,20 @@ __device__ void attend_row(const AttendArgs &a, int u, int g, int t, RowShared<H
         a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + head] = any && sum != 0.0f ? (m + log2f(sum)) * LN2 : -INFINITY;
 }
 
+
+/* Whether some value that one token of unit u sees and another does not is not
+ * finite: only then can a result that is not finite be wrong (0 times it).
+ * For all threads of a block of ROW_THREADS. */
+template <int KT, int HD>
+__device__ bool values_not_finite(const AttendArgs &a, int u) {
+    const int l = u / a.n_head_kv, h = u - l * a.n_head_kv, n = attend_rows(a, u);
+    const int from = a.window > 0 ? 0 : max(0, n - a.T);
+    const uint8_t *v = a.v[l] + (int64_t)h * a.head_stride;
+    bool bad = false;
+    for (int64_t x = threadIdx.x; x < (int64_t)(n - from) * HD; x += ROW_THREADS)
+        bad |= !(fabsf(row_value<KT>(v + (from + x / HD) * a.cell_stride, (int)(x % HD))) < INFINITY);
+    return __syncthreads_or(bad);
+}
 
 /* ------------------------------------------------------------------ */
 /* Plan: which rows of the cache each group of query rows walks         */
@@ -396,7 +411,7 @@ struct FewStage {
 /* Blocks an SM holds, by registers (value sums and queries are 48 of them per
  * 8 query rows), and the stages that their warps' rings leave room for. */
 template <int KT, int NT>
-__host__ __device__ constexpr int few_blocks() { return NT > 1 ? 2 : KT == KT_F16 ? 3 : 4; }
+__host__ __device__ constexpr int few_blocks() { return NT == 2 ? 2 : KT == KT_F16 ? 3 : 4; }
 template <int KT, int HD, int NT>
 __host__ __device__ constexpr int few_stages() {
     const int fit = 200 * 1024 / few_blocks<KT, NT>() / FEW_WARPS / FewStage<KT, HD>::BYTES;
@@ -1028,8 +1043,10 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
                 }
             }
             /* a value that is not finite may be 0 times another token's row: those query rows again, one by one */
-            if (a.T > 1) {
-                __syncthreads();
+            int any = 0;
+            __syncthreads();
+            for (int r = tid; r < rows; r += FEW_THREADS) any |= s_redo[r];
+            if (a.T > 1 && __syncthreads_or(any) && values_not_finite<KT, HD>(a, u)) {
                 for (int r = 0; r < rows; r++)
                     if (s_redo[r]) attend_row<KT, HD>(a, u, (grp * ROWS + r) % a.G, (grp * ROWS + r) / a.G, s_row);
             }

@@ -251,13 +251,13 @@ __device__ __forceinline__ void tile_walk_next(TileWalk &w) {
     w.first = false;
 }
 
-/* One thread's wait on a pipeline barrier: false when it gave up or another
- * role did, with the status set. */
-__device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volatile int *s_abort, int32_t *status) {
-    if (mbar_try(bar, parity)) return true;
-    if (*s_abort || !mbar_wait(bar, parity)) {
+/* One thread's wait on a pipeline barrier, bounded by the context's wait
+ * limit: false when it gave up or another role did, with the status set. */
+__device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volatile int *s_abort, const AttendArgs &a) {
+    if (mbar_test(bar, parity)) return true;
+    if (*s_abort || !mbar_wait(bar, parity, a.wait_limit)) {
         *s_abort = 1;
-        atomicOr(status, ST_TIMEOUT);
+        atomicOr(a.status, ST_TIMEOUT);
         return false;
     }
     return true;
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
     using L = TileLayout<KT, HD>;
     constexpr int NB = EXTRA || KT == KT_Q8_0 ? 2 : 1, TILE_H = TILE_K / NB;      /* score buffers of a row tile, cache rows of each */
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t b_q_full, b_q_free, b_o_full, b_pv[2], b_s_full[2][2], b_p_ready[2][2];
+    __shared__ __align__(8) uint64_t b_q_full, b_q_free, b_o_full, b_drain, b_pv[2], b_s_full[2][2], b_p_ready[2][2];
     __shared__ __align__(8) uint64_t b_k_full[L::STAGES], b_k_free[L::STAGES], b_v_full[L::STAGES], b_v_free[L::STAGES];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
@@ -413,6 +413,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
         mbar_init(&b_q_full, L::LOADERS / 32);
         mbar_init(&b_q_free, 1);
         mbar_init(&b_o_full, 1);
+        mbar_init(&b_drain, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&b_pv[i], 1);
             for (int d = 0; d < 2; d++) {
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                 cp_async_wait<0>();
                 announce();
             }
-            return __all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a.status));
+            return __all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a));
         };
         auto issued = [&](uint64_t *bar) {
             cp_async_commit();
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             constexpr uint32_t HALF = 64 * 128 >> 4;                                     /* 64 rows of a panel */
             const uint32_t d_q = tile_desc(smem + L::Q, 16), d_k = tile_desc(smem + L::K, 16), d_v = tile_desc(smem + L::V, L::PANEL);
             uint32_t ks = 0, kp = 0, vs = 0, vp = 0, pp = 0;            /* stages and phases; pp: bit 2 x + d */
-            auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a.status)); };
+            auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tile_wait(bar, parity, &s_abort, a)); };
             /* O += P V over cache rows 64 e .. 64 e + 63 of the step */
             auto values = [&](uint32_t x, uint32_t e, uint32_t vd, bool add) {
                 const uint32_t o = 256 + 128 * x, p = 128 * x + (NB == 2 ? 64 : 32) * e;
@@ -644,12 +645,12 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const int64_t lo = (int64_t)tp - a.window;
             float m = -INFINITY;
             uint64_t sum = 0ull;                              /* two partial sums */
-            for (int y = 0; active && y < NB * (wk.i1 - wk.i0); y++) {
+            for (int y = 0; ok && active && y < NB * (wk.i1 - wk.i0); y++) {
                 const int i = wk.i0 + y / NB;
                 const uint32_t d = y % NB, tc = tiles + y / NB, T = S + 64 * d;
                 const int j0 = (i < hs ? i * TILE_K : span.y + (i - hs) * TILE_K) + TILE_H * d;
-                if (!tile_wait(&b_s_full[x][d], sc / NB & 1, &s_abort, a.status)) ok = false;
-                if (want_pos && ok && !tile_wait(&b_v_full[tc % L::STAGES], (tc / L::STAGES) & 1, &s_abort, a.status)) ok = false;
+                if (!tile_wait(&b_s_full[x][d], sc / NB & 1, &s_abort, a)) ok = false;
+                if (want_pos && ok && !tile_wait(&b_v_full[tc % L::STAGES], (tc / L::STAGES) & 1, &s_abort, a)) ok = false;
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tc_fence_after();
                 const bool all = j0 + TILE_H <= n - a.T && (!EXTRA || a.window <= 0);    /* every token sees every row */
@@ -703,7 +704,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                     m = to;
                     sum = mul2(sum, pair(f, f));
                     if (y > 0) {                              /* (with one buffer they have, or S would not be full) */
-                        if (NB == 2 && !tile_wait(&b_pv[x], (sc - 1) & 1, &s_abort, a.status)) ok = false;
+                        if (NB == 2 && !tile_wait(&b_pv[x], (sc - 1) & 1, &s_abort, a)) ok = false;
                         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                         tc_fence_after();
 #pragma unroll 1
@@ -733,9 +734,10 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                 }
                 sc++;
             }
-            if (!ok) break;
-            if (!tile_wait(&b_o_full, seg & 1, &s_abort, a.status)) ok = false;
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            /* a wait that gave up leaves the sums as they are (that call's output is undefined), but every thread still
+             * comes to the barriers below, as often as the others */
+            if (ok && !tile_wait(&b_o_full, seg & 1, &s_abort, a)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
 
             const float2 halves = unpair(sum);
@@ -870,12 +872,8 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
     if (w == TILE_SOFT / 32) {
         tc_fence_after();
         if (s_abort) {                                        /* products may still run: wait for them, within a bound */
-            if (lane == 0) {
-                mbar_init(&b_q_full, 1);
-                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-                tc_commit(1, &b_q_full);
-                mbar_wait(&b_q_full, 0);
-            }
+            tc_commit(lane == 0, &b_drain);
+            mbar_wait(&b_drain, 0);
             __syncwarp();
         }
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -909,7 +907,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
     using L = TileLayout<KT, HD>;
     using M = MassTileLayout<KT, HD>;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t b_done[2];
+    __shared__ __align__(8) uint64_t b_done[2], b_drain;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ int s_first[MASS_TILE_THREADS / 32];
@@ -928,6 +926,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
     if (tid == 0) {
         mbar_init(&b_done[0], 1);
         mbar_init(&b_done[1], 1);
+        mbar_init(&b_drain, 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -1006,7 +1005,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
             product(0);
             for (int i = 0; i < tiles; i++) {
                 if (i + 1 < tiles) load(i + 1);
-                if (!tile_wait(&b_done[(done + i) & 1], ((done + i) >> 1) & 1, &s_abort, a.status)) ok = false;
+                if (!tile_wait(&b_done[(done + i) & 1], ((done + i) >> 1) & 1, &s_abort, a)) ok = false;
                 if (i + 1 < tiles) {
                     ready();                                  /* everyone is done with the product before this one, too */
                     product(i + 1);
@@ -1097,13 +1096,8 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
     if (w == 0) {
         tc_fence_after();
         if (s_abort) {                                        /* a product may still run: wait for it, within a bound */
-            if (lane == 0) {
-                mbar_init(&b_done[0], 1);
-                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            }
-            __syncwarp();
-            tc_commit(lane == 0, &b_done[0]);
-            mbar_wait(&b_done[0], 0);
+            tc_commit(lane == 0, &b_drain);
+            mbar_wait(&b_drain, 0);
             __syncwarp();
         }
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem) : "memory");
@@ -1115,9 +1109,13 @@ template <int KT, int HD>
 __global__ void __launch_bounds__(ROW_THREADS) k_attend_redo(const AttendArgs a) {
     __shared__ RowShared<HD> sm;
     const int R = a.T * a.G, many = a.redo[0];
+    int last = -1;
+    bool bad = false;
     for (int i = blockIdx.x; i < many; i += gridDim.x) {
         const int q = a.redo[1 + i], u = q / R, r = q - u * R;
-        attend_row<KT, HD>(a, u, r % a.G, r / a.G, sm);
+        if (u != last) bad = values_not_finite<KT, HD>(a, u);
+        last = u;
+        if (bad) attend_row<KT, HD>(a, u, r % a.G, r / a.G, sm);
     }
 }
 

@@ -16,6 +16,18 @@
 
 using namespace tria;
 
+/* The host side may allocate: what it throws stops at the C boundary. */
+template <class F>
+static int no_throw(const char *what, F &&f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        FAIL(TRIA_ERR_NOMEM, "%s: host allocation failed", what);
+    } catch (...) {
+        FAIL(TRIA_ERR_CUDA, "%s: unexpected exception", what);
+    }
+}
+
 /* A view whose rows attention reads or the serving calls write: any number of
  * caches (no stats are read), post-RoPE keys, K and V. */
 static int validate_cache(const tria_kv_view *v, const char *what) {
@@ -82,9 +94,9 @@ static void launch_append(const AppendArgs &a, bool f32, dim3 grid, cudaStream_t
     else k_append<KT, HD, false><<<grid, APPEND_THREADS, 0, st>>>(a);
 }
 
-extern "C" TRIA_API int tria_append(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
-                                    const tria_append_params *p, const void *k, const void *vv, float *mass,
-                                    int32_t *n_rows_out, void *stream) {
+static int do_append(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
+                     const tria_append_params *p, const void *k, const void *vv, float *mass,
+                     int32_t *n_rows_out, void *stream) {
     NvtxRange range("tria_append");
     const char *fn = "tria_append";
     if (!p) FAIL(TRIA_ERR_INVALID, "%s: null parameters", fn);
@@ -169,9 +181,9 @@ extern "C" TRIA_API int tria_append(tria_ctx *c, const tria_kv_view *v, const in
 /* Accept                                                               */
 /* ------------------------------------------------------------------ */
 
-extern "C" TRIA_API int tria_accept(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, int32_t n_tok,
-                                    const int32_t *path, int64_t path_stride, const int32_t *n_path, float *mass,
-                                    int32_t *n_rows_out, void *stream) {
+static int do_accept(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, int32_t n_tok,
+                     const int32_t *path, int64_t path_stride, const int32_t *n_path, float *mass,
+                     int32_t *n_rows_out, void *stream) {
     NvtxRange range("tria_accept");
     const char *fn = "tria_accept";
     int rc = validate_cache(v, fn);
@@ -221,9 +233,9 @@ extern "C" TRIA_API int tria_accept(tria_ctx *c, const tria_kv_view *v, const in
 /* Eviction by mass                                                     */
 /* ------------------------------------------------------------------ */
 
-extern "C" TRIA_API int tria_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d,
-                                        const int32_t *n_rows, const float *mass, float *mass_dst,
-                                        const tria_evict_params *p, int32_t *n_kept_out, void *stream) {
+static int do_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d,
+                         const int32_t *n_rows, const float *mass, float *mass_dst,
+                         const tria_evict_params *p, int32_t *n_kept_out, void *stream) {
     NvtxRange range("tria_evict_mass");
     const char *fn = "tria_evict_mass";
     if (!n_rows || !p || !mass) FAIL(TRIA_ERR_INVALID, "%s: null argument", fn);
@@ -299,7 +311,7 @@ static int ensure_attend(tria_ctx *c, size_t need, cudaStream_t st) {
 
 template <int KT>
 static int few_blocks_of(int nt) {
-    return nt == 1 ? few_blocks<KT, 1>() : nt == 2 ? few_blocks<KT, 2>() : few_blocks<KT, 4>();
+    return nt == 1 ? few_blocks<KT, 1>() : few_blocks<KT, 2>();
 }
 
 /* Launch plan of one chunk of caches. */
@@ -326,7 +338,7 @@ static int plan_attend(const tria_ctx *c, const tria_kv_view *v, int nl, int T, 
     const int64_t units = (int64_t)nl * v->n_head_kv, R = (int64_t)T * c->G;
     pl = AttendPlan{};
     pl.tile = R > TILE_FROM;
-    pl.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
+    pl.nt = R <= 8 ? 1 : 2;
     const int rows = pl.rows = pl.tile ? TILE_ROWS : 8 * pl.nt;
     const int step = pl.tile ? TILE_STEP : ATT_STEP;
     const int64_t groups = (R + rows - 1) / rows, items = units * groups;
@@ -420,8 +432,7 @@ static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStre
             a.span = span;
         }
         const int rc = pl.tile ? launch_tile<KT, HD>(c, a, pl, st)
-                     : pl.nt == 1 ? launch_few<KT, HD, 1>(c, a, pl, st)
-                     : pl.nt == 2 ? launch_few<KT, HD, 2>(c, a, pl, st) : launch_few<KT, HD, 4>(c, a, pl, st);
+                     : pl.nt == 1 ? launch_few<KT, HD, 1>(c, a, pl, st) : launch_few<KT, HD, 2>(c, a, pl, st);
         if (rc) return rc;
     }
     if (a.mass_out) {
@@ -441,9 +452,9 @@ static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStre
     return TRIA_OK;
 }
 
-extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
-                                    const tria_attend_params *p, const void *q, void *out, float *lse,
-                                    const float *mass_in, float *mass_out, void *stream) {
+static int do_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
+                     const tria_attend_params *p, const void *q, void *out, float *lse,
+                     const float *mass_in, float *mass_out, void *stream) {
     NvtxRange range("tria_attend");
     const char *fn = "tria_attend";
     if (!p) FAIL(TRIA_ERR_INVALID, "%s: null parameters", fn);
@@ -456,12 +467,16 @@ extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const in
     if (!std::isfinite(p->scale) || !std::isfinite(p->mass_decay) || !std::isfinite(p->softcap) || p->softcap < 0.0f)
         FAIL(TRIA_ERR_INVALID, "%s: scale %g, softcap %g or mass_decay %g not finite, or softcap < 0", fn,
              (double)p->scale, (double)p->softcap, (double)p->mass_decay);
+    if (!std::isfinite(p->scale * LOG2E) || !std::isfinite(p->softcap * LOG2E) ||
+        (p->softcap > 0.0f && !std::isfinite(p->scale / p->softcap)))
+        FAIL(TRIA_ERR_INVALID, "%s: scale %g and softcap %g are out of fp32's range together", fn, (double)p->scale, (double)p->softcap);
     if (mass_in && !mass_out) FAIL(TRIA_ERR_INVALID, "%s: mass_in without mass_out", fn);
     if (((uintptr_t)mass_in & 3) || ((uintptr_t)mass_out & 3) || ((uintptr_t)lse & 3))
         FAIL(TRIA_ERR_INVALID, "%s: lse or mass misaligned", fn);
     if (T > 0) {
         if (!q || !out || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))
             FAIL(TRIA_ERR_INVALID, "%s: q or out null or not 16-byte aligned", fn);
+        if (q == out) FAIL(TRIA_ERR_INVALID, "%s: out must not overlap q", fn);
         const int64_t s[6] = {p->q_cache_stride, p->q_tok_stride, p->q_head_stride,
                               p->o_cache_stride, p->o_tok_stride, p->o_head_stride};
         for (int64_t x : s)
@@ -533,8 +548,33 @@ extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const in
         a.tree_stride = p->tree_stride;
         a.tree_words = p->tree_words;
         a.status = c->d_status;
+        a.wait_limit = c->wait_limit;
         if (v->type == TRIA_TYPE_F16)
             return c->hd == 128 ? run_attend<KT_F16, 128>(c, a, pl, st) : run_attend<KT_F16, 64>(c, a, pl, st);
         return c->hd == 128 ? run_attend<KT_Q8_0, 128>(c, a, pl, st) : run_attend<KT_Q8_0, 64>(c, a, pl, st);
     });
+}
+
+extern "C" TRIA_API int tria_append(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
+                                    const tria_append_params *p, const void *k, const void *vv, float *mass,
+                                    int32_t *n_rows_out, void *stream) {
+    return no_throw("tria_append", [&] { return do_append(c, v, n_rows, p, k, vv, mass, n_rows_out, stream); });
+}
+
+extern "C" TRIA_API int tria_accept(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, int32_t n_tok,
+                                    const int32_t *path, int64_t path_stride, const int32_t *n_path, float *mass,
+                                    int32_t *n_rows_out, void *stream) {
+    return no_throw("tria_accept", [&] { return do_accept(c, v, n_rows, n_tok, path, path_stride, n_path, mass, n_rows_out, stream); });
+}
+
+extern "C" TRIA_API int tria_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d,
+                                        const int32_t *n_rows, const float *mass, float *mass_dst,
+                                        const tria_evict_params *p, int32_t *n_kept_out, void *stream) {
+    return no_throw("tria_evict_mass", [&] { return do_evict_mass(c, s, d, n_rows, mass, mass_dst, p, n_kept_out, stream); });
+}
+
+extern "C" TRIA_API int tria_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
+                                    const tria_attend_params *p, const void *q, void *out, float *lse,
+                                    const float *mass_in, float *mass_out, void *stream) {
+    return no_throw("tria_attend", [&] { return do_attend(c, v, n_rows, p, q, out, lse, mass_in, mass_out, stream); });
 }
