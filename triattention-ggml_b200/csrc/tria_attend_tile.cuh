@@ -125,13 +125,30 @@ __device__ __forceinline__ uint64_t tanh_small2(uint64_t u) {
     s = fma2(s, z, pair(-1.0f / 3.0f, -1.0f / 3.0f));
     return fma2(mul2(s, z), u, u);
 }
-/* Caps N scores u = s / c (as bits), the largest magnitude being `far`: c tanh u. */
+/* Caps N scores u = s / c (as bits), the largest magnitude being `far`: c tanh u.
+ * Scores large enough to need the exponential are rare; they take a rolled
+ * loop through `scratch` (N columns of the warp's tensor memory), so that the
+ * common paths stay short enough for the instruction cache. */
 template <int N>
-__device__ __forceinline__ void tile_cap(uint32_t (&v)[N], float c, float far) {
+__device__ __forceinline__ void tile_cap(uint32_t (&v)[N], float c, float far, uint32_t scratch) {
     const uint64_t cc = pair(c, c);
     if (__any_sync(0xffffffffu, !(far < 0.4f))) {
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] = __float_as_uint(c * tanh_both(__uint_as_float(v[e])));
+        for (int e = 0; e < N / 32; e++) tc_st32(scratch + 32 * e, *reinterpret_cast<const uint32_t (*)[32]>(v + 32 * e));
+        tc_wait_st();
+#pragma unroll 1
+        for (int x = 0; x < N / 16; x++) {
+            uint32_t y[16];
+            tc_ld16(y, scratch + 16 * x);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e++) y[e] = __float_as_uint(c * tanh_both(__uint_as_float(y[e])));
+            tc_st16(scratch + 16 * x, y);
+        }
+        tc_wait_st();
+#pragma unroll
+        for (int e = 0; e < N / 32; e++) tc_ld32(*reinterpret_cast<uint32_t (*)[32]>(v + 32 * e), scratch + 32 * e);
+        tc_wait_ld();
     } else if (__any_sync(0xffffffffu, far > 0.2f)) {
 #pragma unroll
         for (int e = 0; e < N / 2; e++) {
@@ -668,7 +685,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                         v[2 * e + 1] = __float_as_uint(z.y);
                         far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
                     }
-                    if (map.cap > 0.0f) tile_cap<TILE_H>(v, map.cap, far);
+                    if (map.cap > 0.0f) tile_cap<TILE_H>(v, map.cap, far, T);
                     mul = pair(1.0f, 1.0f);
                 }
                 if (want_pos || !all || (!EXTRA && map.scale <= 0.0f)) {
@@ -1014,7 +1031,8 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
                 tc_fence_after();
                 const int r0 = q_from + i * MASS_Q + MASS_C * half;
                 uint32_t v[MASS_C];
-                tc_ld32(v, tmem + ((uint32_t)(w & 3) << 21) + MASS_Q * (i & 1) + MASS_C * half);
+                const uint32_t mine = tmem + ((uint32_t)(w & 3) << 21) + MASS_Q * (i & 1) + MASS_C * half;
+                tc_ld32(v, mine);
                 tc_wait_ld();
                 const float *c = s_cols + (i % 3) * 3 * MASS_Q + MASS_C * half;
                 uint64_t mul = pair(map.scale, map.scale);
@@ -1028,7 +1046,7 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
                         far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
                     }
                     mul = pair(1.0f, 1.0f);
-                    if (map.cap > 0.0f) tile_cap<MASS_C>(v, map.cap, far);
+                    if (map.cap > 0.0f) tile_cap<MASS_C>(v, map.cap, far, mine);
                     if (want_pos) {
 #pragma unroll
                         for (int e = 0; e < MASS_C; e++) {

@@ -59,20 +59,23 @@ __device__ __forceinline__ void load8(const uint8_t *p, float (&x)[8]) {
  * warp converts 256 / HD rows at a time.  A converted row is put together in
  * shared memory and leaves as 4-byte words in order: a q8_0 row is 2-byte
  * data at a 4-byte alignment, and storing each lane's bytes directly would
- * send every 32-byte sector four times. */
+ * send every 32-byte sector four times.  blockIdx.x is the unit, so the heads
+ * of a cell, whose rows share sectors, are written side by side in time.
+ * Bound by DRAM: 512 fp32 tokens of 36 layers of 8 heads to q8_0, 192 MB, take
+ * 40 us from a warm L2 and 57 us from a cold one, against 29 us at copy rate. */
 template <int KT, int HD, bool F32>
 __global__ void __launch_bounds__(APPEND_THREADS) k_append(const AppendArgs a) {
     constexpr int LPR = HD / 8, RPW = 32 / LPR;
     constexpr int RB = KT == KT_F16 ? 2 * HD : HD / 32 * 34, WORDS = RB / 4;
     __shared__ __align__(16) uint8_t s_row[APPEND_THREADS / 32][RPW][RB];
-    const int u = blockIdx.y, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
+    const int u = blockIdx.x, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = lane % LPR, sub = lane / LPR;
     const int n = a.n_rows[u];
     const bool fits = n >= 0 && n <= a.n_cells && a.n_tok <= a.n_cells - n;
     if (!fits) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(a.status, ST_ROWS);
+        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.status, ST_ROWS);
     } else {
-        const int wg = blockIdx.x * (APPEND_THREADS / 32) + w, nw = gridDim.x * (APPEND_THREADS / 32);
+        const int wg = blockIdx.y * (APPEND_THREADS / 32) + w, nw = gridDim.y * (APPEND_THREADS / 32);
         const uint8_t *sk = a.src_k + l * a.src_cache + h * a.src_head;
         const uint8_t *sv = a.src_v + l * a.src_cache + h * a.src_head;
         uint8_t *dk = a.k[l] + (int64_t)h * a.head_stride, *dv = a.v[l] + (int64_t)h * a.head_stride;
@@ -124,7 +127,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_append(const AppendArgs a) {
                 __syncwarp();
             }
         }
-        const int tid = blockIdx.x * APPEND_THREADS + threadIdx.x, nt = gridDim.x * APPEND_THREADS;
+        const int tid = blockIdx.y * APPEND_THREADS + threadIdx.x, nt = gridDim.y * APPEND_THREADS;
         const int64_t row0 = (int64_t)u * a.n_cells + n;
         for (int t = tid; t < a.n_tok; t += nt) {
             const int32_t p = a.tok_pos[l * a.tok_pos_stride + t];
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_append(const AppendArgs a) {
     }
     /* the host gives n_rows_out only where this block is the unit's one reader
      * of n_rows, or the two are different arrays */
-    if (a.n_rows_out && blockIdx.x == 0) {
+    if (a.n_rows_out && blockIdx.y == 0) {
         __syncthreads();
         if (threadIdx.x == 0) a.n_rows_out[u] = fits ? n + a.n_tok : n;
     }

@@ -156,7 +156,7 @@ static int do_append(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
         a.tok_pos_stride = p->tok_pos_stride;
         a.mass = mass ? mass + u0 * v->n_cells : nullptr;
         a.status = c->d_status;
-        const dim3 grid((unsigned)bx, (unsigned)(nl * v->n_head_kv));
+        const dim3 grid((unsigned)(nl * v->n_head_kv), (unsigned)bx);
         if (v->type == TRIA_TYPE_F16) {
             if (c->hd == 128) launch_append<KT_F16, 128>(a, f32, grid, st);
             else launch_append<KT_F16, 64>(a, f32, grid, st);
