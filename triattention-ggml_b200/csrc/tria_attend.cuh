@@ -335,6 +335,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_attend_plan(const AttendArgs a
     }
 }
 
+/* Blocks that share `total` steps of `items` items: at most the grid, and so
+ * many that a block takes at least sqrt(join * steps of an item) steps.  A step
+ * more in a row costs its time once; a partial result more costs `join` of that
+ * in the one block that joins an item's results: their sum is least there. */
+__device__ __forceinline__ int blocks_used(int64_t total, int items, int grid, float join) {
+    const int64_t least = (int64_t)ceilf(sqrtf(join * (float)total / (float)items));
+    return (int)min((int64_t)grid, (total + least - 1) / max(least, (int64_t)1));
+}
+
 /* ------------------------------------------------------------------ */
 /* Few query rows: warps on mma tiles, rows streamed once               */
 /* ------------------------------------------------------------------ */
@@ -428,6 +437,7 @@ __host__ __device__ constexpr int few_smem() {
  * rows far below the maximum stay normal f16 numbers (2^-14 and up) down to
  * 2^-20 of it, and the maximum may fall FEW_SLACK behind before the sums are
  * rescaled: 2^(FEW_LIFT + FEW_SLACK) is still finite in f16. */
+constexpr float FEW_JOIN = 0.2f;
 constexpr float FEW_LIFT = 6.0f, FEW_SLACK = 8.0f;
 
 /* Copies one side of the warp's slice: rows [r0, r0 + 16) from p to `st`, row
@@ -648,7 +658,7 @@ __device__ __forceinline__ float merge_row(int S, Ml &&ml, O &&o, float &m, floa
 
 /* Attention of the items' query rows (8 NT a group) over their steps.  The
  * steps of all items are shared out evenly: block b takes steps
- * [b * total / grid, (b + 1) * total / grid) (grid: at most `total`), whatever
+ * [b * total / grid, (b + 1) * total / grid) (grid: blocks_used), whatever
  * units they fall in, so ragged counts read from the device keep every SM busy
  * without the host knowing them.  Within a step each warp takes 16 cache rows
  * of its own and keeps its own running maximum, sum and value sums: the loop
@@ -691,7 +701,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
         steps = s_steps;
     }
     const int64_t total = uniform(steps[items - 1]);
-    const int b = blockIdx.x, grid = (int)min((int64_t)gridDim.x, total);     /* no block between an item's first and last is idle */
+    const int b = blockIdx.x, grid = blocks_used(total, items, gridDim.x, FEW_JOIN);     /* none idle between an item's first and last */
     const ScoreMap map(a);
     const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
     uint8_t *const ring = smem + w * ST * S::BYTES;

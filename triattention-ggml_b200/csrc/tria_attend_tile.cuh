@@ -212,6 +212,7 @@ __device__ __forceinline__ uint32_t order_bits(const AttendArgs &a, int l, int t
 
 constexpr int TILE_Q = 128, TILE_ROWS = 2 * TILE_Q, TILE_K = 128;      /* cache rows a step */
 static_assert(TILE_K == TILE_STEP, "plan");
+constexpr float TILE_JOIN = 0.5f;
 constexpr int TILE_SOFT = 2 * TILE_Q;                    /* threads of the two weight groups */
 
 /* q8_0 rows become two f16 operands, the rounded value and what the rounding
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
     const int units = a.n_layer * a.n_head_kv, items = units * a.groups, R = a.T * a.G;
     const int32_t *steps = a.steps;
     const int64_t total = uniform(steps[items - 1]);
-    const int b = blockIdx.x, grid = (int)min((int64_t)gridDim.x, total);
+    const int b = blockIdx.x, grid = blocks_used(total, items, gridDim.x, TILE_JOIN);
     const bool want_pos = EXTRA && (a.window > 0 || a.slopes != nullptr);
 
     if (tid == 0) {
