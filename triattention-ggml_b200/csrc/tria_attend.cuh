@@ -437,6 +437,8 @@ __host__ __device__ constexpr int few_smem() {
  * rows far below the maximum stay normal f16 numbers (2^-14 and up) down to
  * 2^-20 of it, and the maximum may fall FEW_SLACK behind before the sums are
  * rescaled: 2^(FEW_LIFT + FEW_SLACK) is still finite in f16. */
+/* Measured (blocks_used): 4000 rows, 12 query rows: 30 us at 0.05, 27 at 0.2, 23 at
+ * 0.6; 500 rows: 16, 16 and 27 us. */
 constexpr float FEW_JOIN = 0.2f;
 constexpr float FEW_LIFT = 6.0f, FEW_SLACK = 8.0f;
 
@@ -671,7 +673,14 @@ __device__ __forceinline__ float merge_row(int S, Ml &&ml, O &&o, float &m, floa
  * Cache rows are the matrix rows and query rows its columns, so few query rows
  * waste little: 16 cache rows cost 16 mma per 8 query rows (head_dim 128), and
  * the weights turn around in registers (movmatrix) for the value product.
- * EXTRA: the call caps, biases or windows its scores. */
+ * EXTRA: the call caps, biases or windows its scores.
+ *
+ * Bound by memory: 8 units of 65521 f16 rows (268 MB), 4 query rows each, take
+ * 62 us (4.3 TB/s; 42 at copy rate) with start and join 12 of them; 128 units of
+ * 8197 to 32768 q8_0 rows (710 MB) take 217 us, because a 136-byte row costs the
+ * 64-byte pieces that it touches (1.27 GB read, 5.8 TB/s).  Three blocks an SM
+ * for f16, whose 8 KB stages fill shared memory, four for q8_0, whose bytes
+ * need more instructions. */
 template <int KT, int HD, int NT, bool EXTRA>
 __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_few(const AttendArgs a) {
     using S = FewStage<KT, HD>;
@@ -1071,7 +1080,8 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
 /* ------------------------------------------------------------------ */
 
 /* From the scores that k_attend_few left: a thread per cache row, R weights
- * each; reads 4 R + 4 bytes a row. */
+ * each; reads 4 R + 4 bytes a row and writes 4 (8 units of 65521 rows, R = 4:
+ * 8 us, a launch and two rounds of memory latency). */
 __global__ void __launch_bounds__(256) k_mass_scores(const AttendArgs a) {
     const int u = blockIdx.y, n = attend_rows(a, u), R = a.T * a.G;
     const int2 span = a.span ? a.span[u] : make_int2(0, 0);
@@ -1094,9 +1104,10 @@ __global__ void __launch_bounds__(256) k_mass_scores(const AttendArgs a) {
 
 constexpr int MASS_THREADS = 128, MASS_KEYS = 64;
 
-/* Scores again, now with the denominators known: each warp holds 16 cache rows
- * of a unit and goes over all query rows, 16 at a time, so the weights of a
- * cache row are summed where they are made, in one order. */
+/* Scores again, now with the denominators known, for at most 16 query rows a
+ * unit whose scores were too many to keep (and for no query row at all): each
+ * warp holds 16 cache rows of a unit, so the weights of a cache row are summed
+ * where they are made, in one order. */
 template <int KT, int HD>
 __global__ void __launch_bounds__(MASS_THREADS) k_mass_tiles(const AttendArgs a) {
     using S = FewStage<KT, HD>;

@@ -328,16 +328,25 @@ struct AttendPlan {
 /* Most blocks of an attention kernel (the workspace's counters). */
 constexpr int ATTEND_MAX_GRID = 1024;
 
-/* Query rows of a unit from which the tensor-core tiles are taken. */
-constexpr int TILE_FROM = 16;
+/* Query rows of a unit above which the tensor-core tiles are taken.  Groups of
+ * 16 on mma read a unit's rows once a group (mostly from L2); tiles of 256 read
+ * them once, but start, join and convert q8_0 rows at a higher price.  Measured
+ * with 8 units of head_dim 128 over 500 / 4000 / 32000 rows (us, groups against
+ * tiles): f16 R = 32: 18 / 35 / 72 against 23 / 38 / 87, R = 64: 19 / 38 / 110
+ * against 24 / 39 / 91; q8_0 R = 64: 19 / 39 / 116 against 27 / 51 / 144. */
+constexpr int TILE_FROM_F16 = 32, TILE_FROM_Q8_0 = 64;
 
-/* Most bytes of scores that a call with masses keeps instead of scoring twice. */
+/* A call with masses and at most 16 query rows a unit keeps its scores (4 bytes
+ * a query row and cache row) instead of scoring twice, up to this many bytes.
+ * Measured with 8 units over 500 / 4000 / 65000 rows (us, kept against scored
+ * again): f16 R = 4: 14 / 24 / 70 against 17 / 27 / 106, R = 16: 22 / 36 / 102
+ * against 24 / 40 / 144; q8_0 alike. */
 constexpr size_t SCORES_MAX = (size_t)1 << 30;
 
 static int plan_attend(const tria_ctx *c, const tria_kv_view *v, int nl, int T, bool window, bool mass, AttendPlan &pl) {
     const int64_t units = (int64_t)nl * v->n_head_kv, R = (int64_t)T * c->G;
     pl = AttendPlan{};
-    pl.tile = R > TILE_FROM;
+    pl.tile = R > (v->type == TRIA_TYPE_F16 ? TILE_FROM_F16 : TILE_FROM_Q8_0);
     pl.nt = R <= 8 ? 1 : 2;
     const int rows = pl.rows = pl.tile ? TILE_ROWS : 8 * pl.nt;
     const int step = pl.tile ? TILE_STEP : ATT_STEP;
@@ -439,7 +448,7 @@ static int run_attend(tria_ctx *c, AttendArgs &a, const AttendPlan &pl, cudaStre
         if (pl.keep_scores && a.T > 0) {
             const int gx = std::max(1, std::min((a.n_cells + 255) / 256, 8 * c->sm_count / std::min(units, 8 * c->sm_count)));
             k_mass_scores<<<dim3((unsigned)gx, (unsigned)units), 256, 0, st>>>(a);
-        } else if (pl.tile) {
+        } else if (a.T * a.G > 16) {
             const int rc = launch_mass_tile<KT, HD>(a, units, st);
             if (rc) return rc;
         } else {
