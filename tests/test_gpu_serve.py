@@ -214,6 +214,68 @@ def test_strided_queries_and_outputs(contexts, torch_dev, T):
     assert (store[..., 128:] == 5.0).all()
 
 
+@pytest.mark.parametrize("type_id", [F16, Q8_0])
+@pytest.mark.parametrize("G,T", [(6, 3), (8, 3), (4, 8), (3, 11), (8, 6), (4, 16), (5, 13)])
+@pytest.mark.parametrize("opt", ["plain", "all"])
+def test_attend_between_the_kernels(contexts, torch_dev, type_id, G, T, opt):
+    """17 to 65 query rows a unit: several groups of the one kernel, the first tiles of the other."""
+    c = Cache(type_id, 1, 2, 128, 900, [880, T + 3], torch_dev, seed=T)
+    o = {} if opt == "plain" else dict(cap=25.0, window=700, sink=5, slopes=slopes_of(2 * G, torch_dev))
+    run_attend(contexts, c, G, T, o)
+    sees, depth = a_tree(T, seed=T)
+    tok = torch.from_numpy(depth).to(torch_dev).int() + 1760
+    run_attend(contexts, c, G, T, o, sees=sees, tok_pos=tok)
+
+
+def test_more_units_than_the_kernel_scans_itself(contexts, torch_dev):
+    rng = np.random.default_rng(3)
+    c = Cache(F16, 70, 8, 64, 80, rng.integers(0, 80, (70, 8)), torch_dev)
+    ctx, q = contexts(8, 2, 64), queries(70, 1, 16, 64, torch_dev)
+    out, mass = torch.full_like(q, float("nan")), torch.zeros((70, 8, 80), device=torch_dev)
+    ctx.attend(c.view(), c.rows, q, out, tria_b200.attend_params(0.125), mass_out=mass, stream=torch.cuda.current_stream())
+    ctx.check(torch.cuda.current_stream())
+    attend_close(c, out, None, mass, attend_oracle(c, q, 0.125))
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_rows_past_two_gigabytes(contexts, torch_dev, T):
+    """A cache whose rows lie up to 2.25 GB behind its base.  All keys are 0 but
+    one near the end, all values 0 but that row's, so with s its score the
+    output is v e^s / (e^s + the other rows that the token sees)."""
+    n, cs = 1_100_000, 2048
+    k = torch.zeros((n + 8) * cs, dtype=torch.uint8, device=torch_dev)
+    v = torch.zeros((n + 8) * cs, dtype=torch.uint8, device=torch_dev)
+    pos = torch.zeros((1, 1, n + 8), dtype=torch.int32, device=torch_dev)
+    at = n - 200
+    kr, vr = k[at * cs:at * cs + 256].view(torch.float16), v[at * cs:at * cs + 256].view(torch.float16)
+    q = torch.ones((1, T, 4, 128), dtype=torch.float16, device=torch_dev)
+    kr.fill_(1.0)
+    vr.copy_(torch.arange(128, device=torch_dev).half() / 64 - 1)
+    scale = 14.5 / 128
+    view = tria_b200.make_view(F16, [k], [v], pos, n + 8, cs, 256, 1, flags=tria_b200.VIEW_POST_ROPE)
+    ctx, s = contexts(1, 4, 128), torch.cuda.current_stream()
+    rows = torch.tensor([[n]], dtype=torch.int32, device=torch_dev)
+    out, mass = torch.empty_like(q), torch.zeros((1, 1, n + 8), device=torch_dev)
+    ctx.attend(view, rows, q, out, tria_b200.attend_params(scale), mass_out=mass, stream=s)
+    ctx.check(s)
+    others = torch.arange(n - T, n, device=torch_dev).double()                # n - T + t + 1 rows seen, one of them apart
+    w = np.exp(14.5) / (np.exp(14.5) + others)
+    want = w[None, :, None, None] * vr.double()
+    # f16: the weights' and the result's rounding; the score to fp32
+    assert ((out.double() - want).abs() <= want.abs() * 2.0 ** -9 + 2.0 ** -24).all()
+    assert abs(float(mass[0, 0, at]) / float(4 * w.sum()) - 1) < 1e-4
+    x = torch.full((1, 3, 1, 128), 2.0, dtype=torch.float16, device=torch_dev)
+    ctx.append(view, rows, x, x, torch.arange(3, device=torch_dev).int(), stream=s)
+    path = torch.tensor([[0, 2, 0]], dtype=torch.int32, device=torch_dev)
+    v[(n + 2) * cs:(n + 2) * cs + 256].view(torch.float16).fill_(3.0)
+    ctx.accept(view, rows, 3, path, torch.tensor([2], dtype=torch.int32, device=torch_dev), stream=s)
+    ctx.check(s)
+    assert int(rows) == n + 2
+    assert (k[n * cs:n * cs + 256].view(torch.float16) == 2).all()
+    assert (v[(n + 1) * cs:(n + 1) * cs + 256].view(torch.float16) == 3).all()
+    assert (k[:at * cs] == 0).all()
+
+
 def test_mass_in_place_and_from_nothing(contexts, torch_dev):
     for T in (1, 20):
         c = Cache(Q8_0, 1, 2, 128, 300, [290, 100], torch_dev)
