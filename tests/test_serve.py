@@ -31,6 +31,7 @@ def view(**kw):
 def attend(L, v=None, n_rows=FAKE, q=FAKE, out=2 * FAKE, lse=None, mass_in=None, mass_out=None, **kw):
     p = tria_b200.AttendParams()
     p.n_tok, p.scale, p.mass_decay = 1, 0.125, 1.0
+    p.o_cache_stride, p.o_tok_stride, p.o_head_stride = 512, 512, 128
     for k, x in kw.items():
         setattr(p, k, x)
     return L.tria_attend(None, C.byref(v if v is not None else view()), n_rows, C.byref(p), q, out, lse, mass_in, mass_out, None)
@@ -92,6 +93,7 @@ def test_views(L, call, kw, word, status):
     (dict(reserved=1), "reserved"), (dict(scale=float("nan")), "finite"), (dict(softcap=-1.0), "softcap"),
     (dict(softcap=float("inf")), "finite"), (dict(mass_decay=float("inf")), "finite"),
     (dict(mass_in=FAKE), "mass_in without"), (dict(mass_out=FAKE + 2), "misaligned"), (dict(lse=FAKE + 2), "misaligned"),
+    (dict(o_cache_stride=0), "overlap"), (dict(n_tok=2, o_tok_stride=0), "overlap"), (dict(o_head_stride=0), "overlap"),
     (dict(out=FAKE), "overlap"), (dict(scale=3e38), "range"), (dict(scale=1e10, softcap=1e-30), "range"),
     (dict(q=None), "q or out"), (dict(out=FAKE + 8), "q or out"), (dict(q_tok_stride=4), "strides"),
     (dict(o_head_stride=-8), "strides"), (dict(slopes=FAKE), "tok_pos"), (dict(window=5), "tok_pos"),

@@ -490,6 +490,8 @@ static int do_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
                               p->o_cache_stride, p->o_tok_stride, p->o_head_stride};
         for (int64_t x : s)
             if (x < 0 || x % 8) FAIL(TRIA_ERR_INVALID, "%s: q and out strides must be multiples of 8 elements, not negative", fn);
+        if ((v->n_layer > 1 && !p->o_cache_stride) || (T > 1 && !p->o_tok_stride) || (KV > 1 && !p->o_head_stride))
+            FAIL(TRIA_ERR_INVALID, "%s: an out stride of 0 lets outputs overlap", fn);
         if (p->slopes && ((uintptr_t)p->slopes & 3)) FAIL(TRIA_ERR_INVALID, "%s: slopes misaligned", fn);
         if (p->window > 0 || p->slopes) {
             if ((rc = check_ints(fn, "tok_pos", p->tok_pos))) return rc;
