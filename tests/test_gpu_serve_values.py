@@ -1,0 +1,90 @@
+"""GPU tests of attention over values and scores of every size: small and large
+values, rows that take nearly all of the weight and hold none of the value
+(attention sinks), and scores that rise late.  Tolerances are attend_close's,
+which go by the number formats alone."""
+import math
+
+import pytest
+import torch
+
+from serve_cases import Cache, F16, Q8_0, rows_of_values
+from test_gpu_serve import contexts, queries, run_attend  # noqa: F401 (contexts is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+G, HD, SCALE, LEAD = 4, 128, 128 ** -0.5, 16.0
+
+
+def raised(type_id, dev, T, rows, spread, bits, at, value, alike=False):
+    """(cache, q) whose rows at(j) score `bits` (base 2) above the largest of the
+    others for every query, by a dimension of their own, and hold values of the
+    size `value`; the other rows' values have the size `spread`.  alike: the other
+    rows share one key."""
+    c = Cache(type_id, 1, 2, HD, max(rows) + 21, rows, dev, seed=T)
+    q = queries(1, T, 2 * G, HD, dev, sigma=0.6)
+    q[..., 0] = LEAD
+    g = torch.Generator(device=dev)
+    g.manual_seed(11)
+    up = at(torch.arange(c.cells, device=dev))
+    for h in range(2):
+        k = torch.randn((c.cells, HD), generator=g, device=dev)
+        if alike:
+            k[:] = k[0]
+        k[:, 0] = 0
+        top = float((q[0, :, h * G:(h + 1) * G].float().reshape(-1, HD) @ k.T).max()) * SCALE
+        k[up] = 0
+        k[up, 0] = (top + bits * math.log(2.0)) / (LEAD * SCALE)
+        v = torch.randn((c.cells, HD), generator=g, device=dev) * spread
+        if alike:
+            v = v.abs()
+        v[up] *= value / spread
+        c.unit(c.k, 0, h).copy_(rows_of_values(type_id, k))
+        c.unit(c.v, 0, h).copy_(rows_of_values(type_id, v))
+    return c, q
+
+
+TOKENS = [1, 3, 12, 16, 40, 140]      # 4 to 560 query rows: one group, several, tiles
+
+
+@pytest.mark.parametrize("type_id", [F16, Q8_0])
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("spread", [1e-3, 0.02, 0.3, 4.0, 600.0, 8000.0])
+@pytest.mark.parametrize("bits", [12, 20])
+def test_sinks_without_value(contexts, torch_dev, type_id, T, spread, bits):
+    c, q = raised(type_id, torch_dev, T, [1500, 700], spread, bits, lambda j: j % 16 == 5, 0.0)
+    run_attend(contexts, c, G, T, q=q)
+
+
+@pytest.mark.parametrize("type_id", [F16, Q8_0])
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("spread", [1e-3, 4.0, 600.0, 8000.0])
+@pytest.mark.parametrize("bits", [2.9, 7.9, 30.0])
+def test_scores_that_rise_late(contexts, torch_dev, type_id, T, spread, bits):
+    c, q = raised(type_id, torch_dev, T, [2000, 1100], spread, bits, lambda j: (j % 256 >= 128) & (j % 16 == 3), spread)
+    run_attend(contexts, c, G, T, q=q)
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_q8_0_scales_of_all_sizes_in_a_row(contexts, torch_dev, T):
+    """Blocks of one row from the smallest scale to a large one."""
+    c, q = raised(Q8_0, torch_dev, T, [1200, 500], 1.0, 9, lambda j: j % 16 == 2, 0.0)
+    for h in range(2):
+        v = torch.randn((c.cells, HD), device=torch_dev)
+        v *= torch.tensor([2.0 ** -15, 2.0 ** -8, 1.0, 2.0 ** 10], device=torch_dev).repeat_interleave(32)
+        c.unit(c.v, 0, h).copy_(rows_of_values(Q8_0, v))
+    run_attend(contexts, c, G, T, q=q)
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_a_visible_q8_0_infinity(contexts, torch_dev, T):
+    """An infinite block scale that every token sees: the stored integers' signs,
+    NaN where they are 0, and the other values as they are."""
+    c = Cache(Q8_0, 1, 2, HD, 700, [600, 450], torch_dev)
+    u = c.unit(c.v, 0, 1)
+    u[7, 34:36].view(torch.float16)[0] = float("inf")
+    u[7, 36:40].view(torch.int8).copy_(torch.tensor([5, -3, 0, 127], device=torch_dev))
+    out, _, _ = run_attend(contexts, c, G, T, mass=False)
+    got = out[0, :, G:, 32:36].float()
+    assert (got[..., 0] == math.inf).all() and (got[..., 1] == -math.inf).all()
+    assert torch.isnan(got[..., 2]).all() and (got[..., 3] == math.inf).all()
+    assert torch.isfinite(out[0, :, :G]).all() and torch.isfinite(out[0, :, G:, :32]).all()

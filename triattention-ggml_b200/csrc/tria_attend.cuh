@@ -216,12 +216,13 @@ __device__ void attend_row(const AttendArgs &a, int u, int g, int t, RowShared<H
 
 
 /* Whether some value that one token of unit u sees and another does not is not
- * finite: only then can a result that is not finite be wrong (0 times it).
- * For all threads of a block of ROW_THREADS. */
+ * finite: only then can a result that is not finite be wrong (0 times it).  Of
+ * q8_0 rows any value: an infinite scale leaves no finite remainder of a
+ * weight.  For all threads of a block of ROW_THREADS. */
 template <int KT, int HD>
 __device__ bool values_not_finite(const AttendArgs &a, int u) {
     const int l = u / a.n_head_kv, h = u - l * a.n_head_kv, n = attend_rows(a, u);
-    const int from = a.window > 0 ? 0 : max(0, n - a.T);
+    const int from = a.window > 0 || KT == KT_Q8_0 ? 0 : max(0, n - a.T);
     const uint8_t *v = a.v[l] + (int64_t)h * a.head_stride;
     bool bad = false;
     for (int64_t x = threadIdx.x; x < (int64_t)(n - from) * HD; x += ROW_THREADS)
@@ -401,6 +402,29 @@ __device__ __forceinline__ void int8x4_half(uint32_t w, uint32_t &lo, uint32_t &
     hi = *reinterpret_cast<const uint32_t *>(&y);
 }
 
+/* d += a b, 16 x 8 x 16, bf16 operands, fp32 sums. */
+__device__ __forceinline__ void mma16816_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+/* x and y as bf16 pairs, rounded (hi) and what the rounding left (lo): 16 bits
+ * of each over fp32's range. */
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &lo) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+    const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(ry), "f"(rx));
+}
+/* The int8 pairs (byte 0, byte 1) and (byte 2, byte 3) of w as bf16 pairs,
+ * exactly: 0x4300 | the low seven bits is 128 + them, 0x4300 | the sign bit is
+ * 128 or, for a negative x = low bits - 128, 256; their difference is x. */
+__device__ __forceinline__ void int8x4_bf16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a & 0xff7fff7fu), "r"(a & 0xff80ff80u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(b & 0xff7fff7fu), "r"(b & 0xff80ff80u));
+}
+
 constexpr int FEW_WARPS = 4, FEW_THREADS = FEW_WARPS * 32;
 constexpr int FEW_SLICE = ATT_STEP / FEW_WARPS;      /* cache rows a warp takes per step */
 static_assert(FEW_SLICE == 16 && FEW_THREADS == ROW_THREADS, "warp tile");
@@ -420,7 +444,7 @@ struct FewStage {
 /* Blocks an SM holds, by registers (value sums and queries are 48 of them per
  * 8 query rows), and the stages that their warps' rings leave room for. */
 template <int KT, int NT>
-__host__ __device__ constexpr int few_blocks() { return NT == 2 ? 2 : KT == KT_F16 ? 3 : 4; }
+__host__ __device__ constexpr int few_blocks() { return NT == 2 ? 2 : 3; }
 template <int KT, int HD, int NT>
 __host__ __device__ constexpr int few_stages() {
     const int fit = 200 * 1024 / few_blocks<KT, NT>() / FEW_WARPS / FewStage<KT, HD>::BYTES;
@@ -436,7 +460,8 @@ __host__ __device__ constexpr int few_smem() {
 /* Scores are kept in units where a weight is 2^(x - m + FEW_LIFT): weights of
  * rows far below the maximum stay normal f16 numbers (2^-14 and up) down to
  * 2^-20 of it, and the maximum may fall FEW_SLACK behind before the sums are
- * rescaled: 2^(FEW_LIFT + FEW_SLACK) is still finite in f16. */
+ * rescaled: 2^(FEW_LIFT + FEW_SLACK) is still finite in f16.  (q8_0 weights take
+ * no part in this: see few_pv.) */
 /* Measured (blocks_used): 4000 rows, 12 query rows: 30 us at 0.05, 27 at 0.2, 23 at
  * 0.6; 500 rows: 16, 16 and 27 us. */
 constexpr float FEW_JOIN = 0.2f;
@@ -572,7 +597,13 @@ __device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], con
 /* o += v^T p over the slice's 16 rows.  FULL: every query row sees them all.
  * Otherwise a weight of 0 meets 0: keep0, keep1 (f16) have the bits of a V pair
  * whose row some query row sees, and a q8_0 scale only enters where p is not 0
- * (a row that is not seen may hold NaN). */
+ * (a row that is not seen may hold NaN).
+ *
+ * q8_0: the V operands are the stored integers, so the scales go into the
+ * weights: products whose size follows the values', not the weights' alone,
+ * and for which f16 has no range.  bf16 has it, and two of them (the rounded
+ * product and its remainder) keep 16 bits; the tensor pipe has room (128 units
+ * of 8197 to 32768 rows: 236 us, with one f16 operand 242). */
 template <int KT, int HD, int NT, bool FULL>
 __device__ __forceinline__ void few_pv(const float (&p)[NT][4], const uint8_t *st, int lead, int lane, uint32_t keep0, uint32_t keep1,
                                        float (&o)[NT][HD / 16][4]) {
@@ -613,9 +644,12 @@ __device__ __forceinline__ void few_pv(const float (&p)[NT][4], const uint8_t *s
                 if (sh == 0) w[i] = word_at(at + 2);
                 else w[i] = __funnelshift_r(word_at(at), word_at(at + 4), 16);
             }
+            uint32_t lo[4], hi[4];
+            int8x4_bf16(__byte_perm(w[0], w[1], 0x5140), lo[0], lo[1]);
+            int8x4_bf16(__byte_perm(w[0], w[1], 0x7362), hi[0], hi[1]);
+            int8x4_bf16(__byte_perm(w[2], w[3], 0x5140), lo[2], lo[3]);
+            int8x4_bf16(__byte_perm(w[2], w[3], 0x7362), hi[2], hi[3]);
             const float da = half_at(d0 + 34 * blk), db = half_at(d0 + 8 * VS + 34 * blk);
-            /* the scales go into the weights before their one rounding to f16; the V operands are the stored integers */
-            uint32_t pf[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 float x[4] = {p[t][0] * da, p[t][1] * da, p[t][2] * db, p[t][3] * db};
@@ -623,19 +657,17 @@ __device__ __forceinline__ void few_pv(const float (&p)[NT][4], const uint8_t *s
 #pragma unroll
                     for (int i = 0; i < 4; i++) x[i] = p[t][i] == 0.0f ? 0.0f : x[i];
                 }
-                pf[t][0] = transpose8(pack_half2(x[0], x[1]));
-                pf[t][1] = transpose8(pack_half2(x[2], x[3]));
-            }
-            uint32_t x[4], y[4];
-            int8x4_half(__byte_perm(w[0], w[1], 0x5140), x[0], x[1]);
-            int8x4_half(__byte_perm(w[0], w[1], 0x7362), x[2], x[3]);
-            int8x4_half(__byte_perm(w[2], w[3], 0x5140), y[0], y[1]);
-            int8x4_half(__byte_perm(w[2], w[3], 0x7362), y[2], y[3]);
-            const uint32_t lo[4] = {x[0], x[1], y[0], y[1]}, hi[4] = {x[2], x[3], y[2], y[3]};
+                uint32_t h[2], r[2];
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                mma16816(o[t][2 * blk], lo, pf[t][0], pf[t][1]);
-                mma16816(o[t][2 * blk + 1], hi, pf[t][0], pf[t][1]);
+                for (int i = 0; i < 2; i++) {
+                    split_bf16(x[2 * i], x[2 * i + 1], h[i], r[i]);
+                    h[i] = transpose8(h[i]);
+                    r[i] = transpose8(r[i]);
+                }
+                mma16816_bf16(o[t][2 * blk], lo, h[0], h[1]);
+                mma16816_bf16(o[t][2 * blk + 1], hi, h[0], h[1]);
+                mma16816_bf16(o[t][2 * blk], lo, r[0], r[1]);
+                mma16816_bf16(o[t][2 * blk + 1], hi, r[0], r[1]);
             }
         }
     }
@@ -677,10 +709,10 @@ __device__ __forceinline__ float merge_row(int S, Ml &&ml, O &&o, float &m, floa
  *
  * Bound by memory: 8 units of 65521 f16 rows (268 MB), 4 query rows each, take
  * 62 us (4.3 TB/s; 42 at copy rate) with start and join 12 of them; 128 units of
- * 8197 to 32768 q8_0 rows (710 MB) take 217 us, because a 136-byte row costs the
- * 64-byte pieces that it touches (1.27 GB read, 5.8 TB/s).  Three blocks an SM
- * for f16, whose 8 KB stages fill shared memory, four for q8_0, whose bytes
- * need more instructions. */
+ * 8197 to 32768 q8_0 rows (710 MB) take 236 us a call, because a 136-byte row
+ * costs the 64-byte pieces that it touches.  Three blocks an SM: f16 stages of
+ * 8 KB fill shared memory, and q8_0 bytes need registers (that case in 279 us
+ * with four, which spill). */
 template <int KT, int HD, int NT, bool EXTRA>
 __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_few(const AttendArgs a) {
     using S = FewStage<KT, HD>;
@@ -1065,7 +1097,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
             int any = 0;
             __syncthreads();
             for (int r = tid; r < rows; r += FEW_THREADS) any |= s_redo[r];
-            if (a.T > 1 && __syncthreads_or(any) && values_not_finite<KT, HD>(a, u)) {
+            if ((a.T > 1 || KT == KT_Q8_0) && __syncthreads_or(any) && values_not_finite<KT, HD>(a, u)) {
                 for (int r = 0; r < rows; r++)
                     if (s_redo[r]) attend_row<KT, HD>(a, u, (grp * ROWS + r) % a.G, (grp * ROWS + r) / a.G, s_row);
             }
