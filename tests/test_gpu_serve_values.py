@@ -7,7 +7,8 @@ import math
 import pytest
 import torch
 
-from serve_cases import Cache, F16, Q8_0, rows_of_values
+import tria_b200
+from serve_cases import Cache, F16, Q8_0, attend_close, attend_oracle, rows_of_values, values_of_rows
 from test_gpu_serve import contexts, queries, run_attend  # noqa: F401 (contexts is a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -62,6 +63,30 @@ def test_sinks_without_value(contexts, torch_dev, type_id, T, spread, bits):
 def test_scores_that_rise_late(contexts, torch_dev, type_id, T, spread, bits):
     c, q = raised(type_id, torch_dev, T, [2000, 1100], spread, bits, lambda j: (j % 256 >= 128) & (j % 16 == 3), spread)
     run_attend(contexts, c, G, T, q=q)
+
+
+@pytest.mark.parametrize("type_id", [F16, Q8_0])
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("bits", [16, 20, 24, 28])
+@pytest.mark.parametrize("spread", [1.0, 600.0])
+def test_equal_weights_far_below_a_sink(contexts, torch_dev, type_id, T, bits, spread):
+    """The rows that carry the value all have one weight: a rounding of it does
+    not average out.  A weight is rounded by 2^-11 of itself or, where that is
+    less than half a step of f16's subnormal numbers, by 2^-25 / 2^10 of the
+    row's largest (the lift of the weights): in all 2^-35 sum_j |v_j|, since the
+    largest weight is at most 1.  attend_close's bound takes it as 2^-24 sum_j
+    |v_j| more under the factor 2^-11 of the weights' own rounding."""
+    c, q = raised(type_id, torch_dev, T, [1300, 900], spread, bits, lambda j: j % 16 == 9, 0.0, alike=True)
+    want = list(attend_oracle(c, q, SCALE))
+    for h in range(2):
+        n = int(c.rows_host[0, h])
+        want[3][0, :, h * G:(h + 1) * G] += 2.0 ** -24 * values_of_rows(type_id, c.unit(c.v, 0, h)[:n], HD).abs().sum(0)
+    out, s = torch.empty_like(q), torch.cuda.current_stream(torch_dev)
+    lse, mass = torch.empty((1, T, 2 * G), device=torch_dev), torch.empty((1, 2, c.cells), device=torch_dev)
+    ctx = contexts(2, G, HD)
+    ctx.attend(c.view(), c.rows, q, out, tria_b200.attend_params(SCALE), lse=lse, mass_out=mass, stream=s)
+    ctx.check(s)
+    attend_close(c, out, lse, mass, want)
 
 
 @pytest.mark.parametrize("T", TOKENS)

@@ -459,13 +459,14 @@ __host__ __device__ constexpr int few_smem() {
 
 /* Scores are kept in units where a weight is 2^(x - m + FEW_LIFT): weights of
  * rows far below the maximum stay normal f16 numbers (2^-14 and up) down to
- * 2^-20 of it, and the maximum may fall FEW_SLACK behind before the sums are
+ * 2^-26 of it, and the maximum may fall FEW_SLACK behind before the sums are
  * rescaled: 2^(FEW_LIFT + FEW_SLACK) is still finite in f16.  (q8_0 weights take
- * no part in this: see few_pv.) */
+ * no part in this: see few_pv.)  A sum rescaled is some 64 multiplications of a
+ * warp: slack 3 and 8 measure the same. */
+constexpr float FEW_LIFT = 12.0f, FEW_SLACK = 3.0f;
 /* Measured (blocks_used): 4000 rows, 12 query rows: 30 us at 0.05, 27 at 0.2, 23 at
  * 0.6; 500 rows: 16, 16 and 27 us. */
 constexpr float FEW_JOIN = 0.2f;
-constexpr float FEW_LIFT = 6.0f, FEW_SLACK = 8.0f;
 
 /* Copies one side of the warp's slice: rows [r0, r0 + 16) from p to `st`, row
  * stride RS; rows at and behind n become zeros.  A full slice of aligned rows
