@@ -113,3 +113,29 @@ def test_a_visible_q8_0_infinity(contexts, torch_dev, T):
     assert (got[..., 0] == math.inf).all() and (got[..., 1] == -math.inf).all()
     assert torch.isnan(got[..., 2]).all() and (got[..., 3] == math.inf).all()
     assert torch.isfinite(out[0, :, :G]).all() and torch.isfinite(out[0, :, G:, :32]).all()
+
+
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("where", ["keys", "values"])
+def test_q8_0_blocks_beyond_f16(contexts, torch_dev, T, where):
+    """Scales whose block reaches past 65504 (tria_append stores them from fp32):
+    keys along a dimension in which the queries are small, values of rows with
+    little weight."""
+    c = Cache(Q8_0, 1, 2, HD, 900, [870, 333], torch_dev)
+    q = queries(1, T, 2 * G, HD, torch_dev, sigma=0.6)
+    q[..., 0] = 2.0 ** -13
+    for h, rows in ((0, [3, 200, 869]), (1, [77, 300])):
+        for r in rows:
+            if where == "keys":
+                b = c.unit(c.k, 0, h)[r]
+                b[:2].view(torch.float16)[0] = 900.0
+                b[2:34] = 0
+                b[2] = 120 if r % 2 else 136                       # +120, -120
+            else:
+                k = torch.zeros((1, HD), device=torch_dev)
+                k[0, 0] = -16 * math.log(2.0) / (SCALE * 2.0 ** -13)   # 16 (base 2) below a score of 0
+                c.unit(c.k, 0, h)[r:r + 1].copy_(rows_of_values(Q8_0, k))
+                b = c.unit(c.v, 0, h)[r]
+                b[34:36].view(torch.float16)[0] = 2000.0
+    out, lse, mass = run_attend(contexts, c, G, T, q=q)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()

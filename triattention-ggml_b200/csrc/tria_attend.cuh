@@ -122,6 +122,8 @@ struct ScoreMap {
     }
 };
 
+__device__ __forceinline__ float half_at(const uint8_t *p) { return __half2float(*reinterpret_cast<const __half *>(p)); }
+
 /* Element d of the cache row at p. */
 template <int KT>
 __device__ __forceinline__ float row_value(const uint8_t *p, int d) {
@@ -135,11 +137,11 @@ __device__ __forceinline__ float row_value(const uint8_t *p, int d) {
 
 /* The base-2 score of a query against a cache row, in fp32 throughout;
  * slope2: log2(e) times the head's slope. */
-template <int KT, int HD>
-__device__ __forceinline__ float attend_score(const ScoreMap &f, const uint8_t *krow, const float *q, float slope2,
+template <int KT, int HD, class Q>
+__device__ __forceinline__ float attend_score(const ScoreMap &f, const uint8_t *krow, const Q *q, float slope2,
                                               int tok_pos, int pos) {
     float s = 0.0f;
-    for (int d = 0; d < HD; d++) s = fmaf(q[d], row_value<KT>(krow, d), s);
+    for (int d = 0; d < HD; d++) s = fmaf((float)q[d], row_value<KT>(krow, d), s);
     return fmaf(-slope2, (float)(tok_pos - pos), f(s));
 }
 
@@ -208,25 +210,38 @@ __device__ void attend_row(const AttendArgs &a, int u, int g, int t, RowShared<H
         }
         __syncthreads();
     }
-    if (tid < HD)
-        a.out[l * a.o_cache + t * a.o_tok + head * a.o_head + tid] = __float2half_rn(any && sum != 0.0f ? acc / sum : 0.0f);
-    if (a.lse && tid == 0)
-        a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + head] = any && sum != 0.0f ? (m + log2f(sum)) * LN2 : -INFINITY;
+    const bool none = !any || sum == 0.0f;
+    if (tid < HD) a.out[l * a.o_cache + t * a.o_tok + head * a.o_head + tid] = __float2half_rn(none ? 0.0f : acc / sum);
+    if (tid == 0) {
+        if (a.lse) a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + head] = none ? -INFINITY : (m + log2f(sum)) * LN2;
+        if (a.norm) a.norm[((int64_t)u * a.T + t) * a.G + g] = none ? make_float2(0.0f, 0.0f) : make_float2(m, 1.0f / sum);
+    }
 }
 
 
-/* Whether some value that one token of unit u sees and another does not is not
- * finite: only then can a result that is not finite be wrong (0 times it).  Of
- * q8_0 rows any value: an infinite scale leaves no finite remainder of a
- * weight.  For all threads of a block of ROW_THREADS. */
-template <int KT, int HD>
-__device__ bool values_not_finite(const AttendArgs &a, int u) {
+/* Whether a result of unit u that is not finite can be wrong.  f16: if some
+ * value that one token sees and another does not is not finite (0 times it).
+ * q8_0: if a block's scale is not finite (it leaves no finite remainder of a
+ * weight) or, on the tiles, so large that its values pass f16's 65504 and their
+ * remainders are lost.  For all threads of a block of ROW_THREADS. */
+constexpr float TILE_SCALE = 512.0f;     /* 127 times it is 65024 */
+template <int KT, int HD, bool TILE>
+__device__ bool result_in_doubt(const AttendArgs &a, int u) {
     const int l = u / a.n_head_kv, h = u - l * a.n_head_kv, n = attend_rows(a, u);
-    const int from = a.window > 0 || KT == KT_Q8_0 ? 0 : max(0, n - a.T);
-    const uint8_t *v = a.v[l] + (int64_t)h * a.head_stride;
+    const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
     bool bad = false;
-    for (int64_t x = threadIdx.x; x < (int64_t)(n - from) * HD; x += ROW_THREADS)
-        bad |= !(fabsf(row_value<KT>(v + (from + x / HD) * a.cell_stride, (int)(x % HD))) < INFINITY);
+    if constexpr (KT == KT_F16) {
+        const int from = a.window > 0 ? 0 : max(0, n - a.T);
+        for (int64_t x = threadIdx.x; x < (int64_t)(n - from) * HD; x += ROW_THREADS)
+            bad |= !(fabsf(row_value<KT>(v + (from + x / HD) * a.cell_stride, (int)(x % HD))) < INFINITY);
+    } else {
+        constexpr int NB = HD / 32;
+        for (int64_t x = threadIdx.x; x < (int64_t)n * NB; x += ROW_THREADS) {
+            const int64_t at = x / NB * a.cell_stride + x % NB * 34;
+            const float dk = fabsf(half_at(k + at)), dv = fabsf(half_at(v + at));
+            bad |= TILE ? !(dk <= TILE_SCALE && dv <= TILE_SCALE) : !(dv < INFINITY);
+        }
+    }
     return __syncthreads_or(bad);
 }
 
@@ -385,7 +400,6 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a
 }
 __device__ __forceinline__ uint32_t word_at(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 __device__ __forceinline__ uint2 two_words_at(const uint8_t *p) { return *reinterpret_cast<const uint2 *>(p); }
-__device__ __forceinline__ float half_at(const uint8_t *p) { return __half2float(*reinterpret_cast<const __half *>(p)); }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -1098,7 +1112,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
             int any = 0;
             __syncthreads();
             for (int r = tid; r < rows; r += FEW_THREADS) any |= s_redo[r];
-            if ((a.T > 1 || KT == KT_Q8_0) && __syncthreads_or(any) && values_not_finite<KT, HD>(a, u)) {
+            if ((a.T > 1 || KT == KT_Q8_0) && __syncthreads_or(any) && result_in_doubt<KT, HD, false>(a, u)) {
                 for (int r = 0; r < rows; r++)
                     if (s_redo[r]) attend_row<KT, HD>(a, u, (grp * ROWS + r) % a.G, (grp * ROWS + r) / a.G, s_row);
             }

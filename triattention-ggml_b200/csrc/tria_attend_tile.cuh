@@ -935,6 +935,27 @@ struct MassTileLayout {
     static constexpr int BYTES = SUM + TILE_K * 4 + 1024;
 };
 
+/* The mass of row j of unit u, whose position is pj, by one thread. */
+template <int KT, int HD>
+__device__ __noinline__ float row_mass(const AttendArgs &a, int u, int j, int n, int pj) {
+    const int l = u / a.n_head_kv, h = u - l * a.n_head_kv;
+    const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride + (int64_t)j * a.cell_stride;
+    const ScoreMap map(a);
+    float mass = 0.0f;
+    for (int t = 0; t < a.T; t++) {
+        const int tp = a.tok_pos ? a.tok_pos[l * a.tok_pos_stride + t] : 0;
+        if (!attend_sees(a, l, t, j, n, pj, (int64_t)tp - a.window)) continue;
+        for (int g = 0; g < a.G; g++) {
+            const int head = h * a.G + g;
+            const float2 nm = a.norm[((int64_t)u * a.T + t) * a.G + g];
+            const float x = attend_score<KT, HD>(map, k, a.q + l * a.q_cache + t * a.q_tok + head * a.q_head,
+                                                 a.slopes ? a.slopes[head] * LOG2E : 0.0f, tp, pj);
+            mass = fmaf(ex2(x - nm.x), nm.y, mass);
+        }
+    }
+    return mass;
+}
+
 /* The scores again, now with the denominators known: S^T = K Q^T with the 128
  * cache rows as the matrix rows, so a thread owns a cache row and adds up its
  * weights over the query rows as they come by, 64 a tile, in one order; no
@@ -945,7 +966,7 @@ struct MassTileLayout {
  * query rows, window 8192: 141 us with 128 query rows a tile and one block an
  * SM, 86 us so). */
 template <int KT, int HD, bool EXTRA>
-__global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const AttendArgs a) {
+__global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const __grid_constant__ AttendArgs a) {
     using L = TileLayout<KT, HD>;
     using M = MassTileLayout<KT, HD>;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -1128,7 +1149,9 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const Attend
         tc_fence_before();
         __syncthreads();
         if (!half && j < n) {
-            const float mass = s2.x + s2.y + s_sum[row];
+            float mass = s2.x + s2.y + s_sum[row];
+            /* a key that f16 operands do not hold (TILE_SCALE): its weights from the definition */
+            if (KT == KT_Q8_0 && mass != mass) mass = row_mass<KT, HD>(a, u, j, n, pj);
             const int64_t x = (int64_t)u * a.n_cells + j;
             a.mass_out[x] = a.mass_in ? fmaf(a.mass_decay, a.mass_in[x], mass) : mass;
         }
@@ -1156,7 +1179,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_attend_redo(const AttendArgs a)
     bool bad = false;
     for (int i = blockIdx.x; i < many; i += gridDim.x) {
         const int q = a.redo[1 + i], u = q / R, r = q - u * R;
-        if (u != last) bad = values_not_finite<KT, HD>(a, u);
+        if (u != last) bad = result_in_doubt<KT, HD, true>(a, u);
         last = u;
         if (bad) attend_row<KT, HD>(a, u, r % a.G, r / a.G, sm);
     }
