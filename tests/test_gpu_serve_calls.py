@@ -1,0 +1,101 @@
+"""GPU tests of how the serving calls may be made: steps of other sizes between
+a capture and its replay, and views, strides and arrays that the calls refuse."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import tria_b200
+from serve_cases import Cache, F16, Q8_0, attend_close, attend_oracle
+from test_gpu_serve import contexts, kept_oracle, queries  # noqa: F401 (contexts is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def eviction(L, rows, cells, dev, seed):
+    """An evict_mass step over L layers of two kv heads: (caches, masses, call)."""
+    c, d = Cache(F16, L, 2, 128, cells, rows, dev, seed=seed), Cache(F16, L, 2, 128, cells, rows, dev, seed=seed + 1)
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    mass = torch.rand((L, 2, cells), generator=g, device=dev)
+    md = torch.zeros_like(mass)
+    prm = tria_b200.EvictParams(10 ** 5, 60 + seed, 100, 0, 0, 0)
+    n = np.asarray(rows, np.int32)
+    keep = np.minimum(n, 60 + seed)
+
+    def call(ctx, stream):
+        ctx.evict_mass(c.view(), d.view(), n, mass, md, prm, stream=stream)
+
+    def check():
+        for u in range(2 * L):
+            l, h = divmod(u, 2)
+            idx = kept_oracle(mass[l, h].cpu().numpy(), c.pos[l, h].cpu().numpy(), int(n[u]), int(keep[u]), 10 ** 5, 0, 0)
+            assert torch.equal(md[l, h, :len(idx)], mass[l, h][torch.from_numpy(idx).to(dev)])
+    return call, check, keep
+
+
+def test_replayed_evictions_of_several_sizes(torch_dev, tmp_path):
+    """A step of one layer captured, then an eager one of three layers, then one
+    of three layers captured: every replay reads back its own counts, whatever
+    ran in between, and the read-back buffer stays where the graphs have it."""
+    import workloads
+    p = str(tmp_path / "s.tria")
+    workloads.write_tria(p, 3, 8, 2, 128, seed=1)
+    st = tria_b200.load(p)
+    ctx = tria_b200.Context(st, 0)
+    s = torch.cuda.Stream()
+    small, small_ok, small_n = eviction(1, [700, 500], 900, torch_dev, 0)
+    large, large_ok, large_n = eviction(3, [100, 200, 300, 40, 0, 128], 128 + 172, torch_dev, 9)
+    torch.cuda.synchronize()
+    graphs = []
+    for call in (small, large):
+        with torch.cuda.stream(s):
+            call(ctx, s)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            call(ctx, torch.cuda.current_stream())
+        graphs.append(g)
+    for i in (0, 1, 0, 0, 1):
+        ok, want = ((small_ok, small_n), (large_ok, large_n))[i]
+        with torch.cuda.stream(s):
+            graphs[i].replay()
+        most, counts = ctx.get_n_kv(6)
+        assert counts[:len(want)].tolist() == want.tolist() and most == want.max()
+        assert (counts[len(want):] == 0).all()
+        ok()
+    with torch.cuda.stream(s):
+        large(ctx, s)
+        graphs[0].replay()
+    most, counts = ctx.get_n_kv(6)
+    assert counts.tolist() == small_n.tolist() + [0] * 4 and most == small_n.max()
+    del graphs, g
+    ctx.close()
+    tria_b200.free(st)
+
+
+def test_a_larger_step_captured_first(torch_dev, tmp_path):
+    """More units than any step before, in scratch that is large enough: nothing has to grow inside the capture."""
+    import workloads
+    p = str(tmp_path / "s.tria")
+    workloads.write_tria(p, 3, 8, 2, 128, seed=1)
+    st = tria_b200.load(p)
+    ctx = tria_b200.Context(st, 0)
+    s = torch.cuda.Stream()
+    wide, _, wide_n = eviction(1, [3000, 2900], 3000, torch_dev, 0)
+    tall, tall_ok, tall_n = eviction(3, [100, 200, 300, 40, 0, 128], 300, torch_dev, 5)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        wide(ctx, s)
+    assert ctx.get_n_kv(2)[1].tolist() == wide_n.tolist()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        tall(ctx, torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g.replay()
+    assert ctx.get_n_kv(6)[1].tolist() == tall_n.tolist()
+    tall_ok()
+    del g
+    ctx.close()
+    tria_b200.free(st)

@@ -185,8 +185,11 @@ extern "C" TRIA_API int tria_ctx_create(const tria_stats *s, int device, tria_ct
     if (e == cudaSuccess) e = cudaMemcpy(c->d_q, q.data(), q.size() * sizeof(float), cudaMemcpyHostToDevice);
     if (e == cudaSuccess) e = cudaMalloc(&c->d_omega, fc * sizeof(float));
     if (e == cudaSuccess) e = cudaMemcpy(c->d_omega, s->omega, fc * sizeof(float), cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaMalloc(&c->d_status, sizeof(int32_t));
-    if (e == cudaSuccess) e = cudaMemset(c->d_status, 0, sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaMalloc(&c->d_status, 2 * sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaMemset(c->d_status, 0, 2 * sizeof(int32_t));
+    const size_t pinned = ((size_t)c->L * c->KV + 2) * sizeof(int32_t);
+    if (e == cudaSuccess) e = cudaMallocHost(&c->h_pinned, pinned);
+    if (e == cudaSuccess) memset(c->h_pinned, 0, pinned);
     if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->ev_done, cudaEventDisableTiming);
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&c->own_stream, cudaStreamNonBlocking);
     if (e != cudaSuccess) {
@@ -280,13 +283,6 @@ int ensure_scratch(tria_ctx *c, int64_t units, int64_t cells, cudaStream_t st) {
     c->cnt = (int32_t *)p;
     c->raw_stride = stride;
     c->cell_stride = stride;
-    if (c->pinned_cap < units + 1) {
-        if (c->h_pinned) { cudaDeviceSynchronize(); cudaFreeHost(c->h_pinned); }
-        c->h_pinned = nullptr;
-        c->pinned_cap = 0;
-        CUDA_TRY(cudaMallocHost(&c->h_pinned, (size_t)(units + 1) * 4));
-        c->pinned_cap = (int32_t)(units + 1);
-    }
     return TRIA_OK;
 }
 
@@ -691,7 +687,7 @@ static int select_split(const tria_ctx *c, int units, int n_max, bool fused) {
 
 int launch_select(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, const std::vector<int32_t> &keep,
                          const tria_evict_params *p, bool fused, const float *scores, int32_t *kept_idx,
-                         int64_t kept_stride, int32_t *n_kept, cudaStream_t st) {
+                         int64_t kept_stride, int32_t *n_kept, cudaStream_t st, int64_t step_units) {
     return for_layer_chunks(v, [&](int l0, int nl) -> int {
         SelectArgs *a = new (std::nothrow) SelectArgs;
         if (!a) FAIL(TRIA_ERR_NOMEM, "host allocation failed");
@@ -715,6 +711,8 @@ int launch_select(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, con
         a->kept_idx = kept_idx + u0 * kept_stride;
         a->kept_stride = kept_stride;
         a->n_kept = n_kept + u0;
+        a->step_units = step_units ? c->d_status + 1 : nullptr;
+        a->units_all = (int32_t)step_units;
         a->status = c->d_status;
         for (int u = 0; u < units; u++) {
             a->n_rows[u] = n_rows[u0 + u];
@@ -835,6 +833,14 @@ int launch_compact(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d, co
         CUDA_TRY(cudaGetLastError());
         return TRIA_OK;
     });
+}
+
+int read_back_step(tria_ctx *c, const int32_t *cnt, int64_t units, cudaStream_t st) {
+    CUDA_TRY(cudaMemcpyAsync(c->h_pinned, c->d_status, 8, cudaMemcpyDeviceToHost, st));
+    CUDA_TRY(cudaMemcpyAsync(c->h_pinned + 2, cnt, (size_t)units * 4, cudaMemcpyDeviceToHost, st));
+    CUDA_TRY(record_done(c->ev_done, st));
+    c->have_step = true;
+    return TRIA_OK;
 }
 
 /* ------------------------------------------------------------------ */
@@ -981,7 +987,7 @@ extern "C" TRIA_API int tria_evict(tria_ctx *c, const tria_kv_view *s, const tri
     if ((rc = stage(2))) return rc;
     if ((rc = run_znorm(c, s, n_rows, st))) return rc;
     if ((rc = stage(3))) return rc;
-    if ((rc = launch_select(c, s, n_rows, keep, p, true, nullptr, c->kept, c->cell_stride, cnt, st))) return rc;
+    if ((rc = launch_select(c, s, n_rows, keep, p, true, nullptr, c->kept, c->cell_stride, cnt, st, units))) return rc;
     if ((rc = stage(4))) return rc;
     int hint = 0;
     for (int32_t k : keep) hint = std::max(hint, k);
@@ -989,12 +995,7 @@ extern "C" TRIA_API int tria_evict(tria_ctx *c, const tria_kv_view *s, const tri
     if ((rc = launch_compact(c, s, d, n_rows, c->kept, c->cell_stride, cnt, st, hint))) return rc;
     if ((rc = stage(5))) return rc;
     c->have_timing = c->timing;
-    CUDA_TRY(cudaMemcpyAsync(c->h_pinned, c->d_status, 4, cudaMemcpyDeviceToHost, st));
-    CUDA_TRY(cudaMemcpyAsync(c->h_pinned + 1, cnt, (size_t)units * 4, cudaMemcpyDeviceToHost, st));
-    CUDA_TRY(record_done(c->ev_done, st));
-    c->last_units = (int32_t)units;
-    c->have_step = true;
-    return TRIA_OK;
+    return read_back_step(c, cnt, units, st);
 }
 
 extern "C" TRIA_API int tria_get_n_kv(tria_ctx *c, int32_t *n_kept, int32_t cap) {
@@ -1009,9 +1010,10 @@ extern "C" TRIA_API int tria_get_n_kv(tria_ctx *c, int32_t *n_kept, int32_t cap)
         return status_of_bits(bits, "tria_get_n_kv");
     }
     int mx = 0;
-    for (int u = 0; u < c->last_units; u++) {
-        mx = std::max(mx, c->h_pinned[1 + u]);
-        if (n_kept && u < cap) n_kept[u] = c->h_pinned[1 + u];
+    const int32_t *counts = c->h_pinned + 2;
+    for (int u = 0; u < c->h_pinned[1]; u++) {
+        mx = std::max(mx, counts[u]);
+        if (n_kept && u < cap) n_kept[u] = counts[u];
     }
     return mx;
 }
@@ -1181,7 +1183,7 @@ extern "C" TRIA_API int tria_evict_host(tria_ctx *c, const tria_kv_view *s, cons
         int32_t *cnt = c->d_cnt_all + u0;
         if ((rc = run_score(c, &dv, nr, p->cur_pos, s->type, st))) return rc;
         if ((rc = run_znorm(c, &dv, nr, st))) return rc;
-        if ((rc = launch_select(c, &dv, nr, kc, p, true, nullptr, c->kept, c->cell_stride, cnt, st))) return rc;
+        if ((rc = launch_select(c, &dv, nr, kc, p, true, nullptr, c->kept, c->cell_stride, cnt, st, units))) return rc;
         int hint = 0;
         for (int32_t k : kc) hint = std::max(hint, k);
         if (extra) hint += extra + 1;
@@ -1190,21 +1192,7 @@ extern "C" TRIA_API int tria_evict_host(tria_ctx *c, const tria_kv_view *s, cons
         c->hs_used[b] = true;
     }
     c->have_timing = false;
-    CUDA_TRY(cudaMemcpyAsync(c->h_pinned, c->d_status, 4, cudaMemcpyDeviceToHost, st));
-    if (c->pinned_cap < units + 1) {
-        cudaStreamSynchronize(st);
-        if (c->h_pinned) cudaFreeHost(c->h_pinned);
-        c->h_pinned = nullptr;
-        c->pinned_cap = 0;
-        CUDA_TRY(cudaMallocHost(&c->h_pinned, (size_t)(units + 1) * 4));
-        c->pinned_cap = (int32_t)(units + 1);
-        CUDA_TRY(cudaMemcpyAsync(c->h_pinned, c->d_status, 4, cudaMemcpyDeviceToHost, st));
-    }
-    CUDA_TRY(cudaMemcpyAsync(c->h_pinned + 1, c->d_cnt_all, (size_t)units * 4, cudaMemcpyDeviceToHost, st));
-    CUDA_TRY(record_done(c->ev_done, st));
-    c->last_units = (int32_t)units;
-    c->have_step = true;
-    return TRIA_OK;
+    return read_back_step(c, c->d_cnt_all, units, st);
 }
 
 /* ---- global budget ---- */

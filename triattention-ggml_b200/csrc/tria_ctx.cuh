@@ -91,12 +91,12 @@ struct tria_ctx {
     size_t io_cap = 0;
     cudaStream_t own_stream = nullptr;
     /* status / counts read-back */
-    int32_t *d_status = nullptr;         /* ST_* bits the kernels set; cleared when read back */
+    int32_t *d_status = nullptr;         /* [0] ST_* bits the kernels set, cleared when read back; [1] units of the last step */
     long long wait_limit = tria::WAIT_LIMIT_DEFAULT;   /* bound of the scoring kernel's pipeline waits */
     int select_split = 0;                        /* CTAs per unit in selection: 0 automatic, 1 one block */
-    int32_t *h_pinned = nullptr;         /* [0] = status, [1..] counts */
-    int32_t pinned_cap = 0;
-    int32_t last_units = 0;
+    /* [0] status, [1] units, [2..] counts: room for every unit of the stats, so that it never moves (captured steps
+     * write it), and its unit count from the device, so that a replayed step brings its own */
+    int32_t *h_pinned = nullptr;
     cudaEvent_t ev_done = nullptr;
     bool have_step = false;
     /* stage timing (tria_ctx_set_timing) */
@@ -138,7 +138,9 @@ void keep_requests(const tria_ctx *c, const tria_kv_view *v, const int32_t *n_ro
                    std::vector<int32_t> &keep);
 int launch_select(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, const std::vector<int32_t> &keep,
                   const tria_evict_params *p, bool fused, const float *scores, int32_t *kept_idx,
-                  int64_t kept_stride, int32_t *n_kept, cudaStream_t st);
+                  int64_t kept_stride, int32_t *n_kept, cudaStream_t st, int64_t step_units = 0);
+/* Queues the read-back of a step's status, unit count (launch_select's step_units) and kept counts, and records its end. */
+int read_back_step(tria_ctx *c, const int32_t *cnt, int64_t units, cudaStream_t st);
 int launch_compact(tria_ctx *c, const tria_kv_view *s, const tria_kv_view *d, const int32_t *n_rows,
                    const int32_t *kept_idx, int64_t kept_stride, const int32_t *n_kept, cudaStream_t st,
                    int rows_hint = -1);

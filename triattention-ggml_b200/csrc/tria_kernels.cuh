@@ -1513,6 +1513,8 @@ struct SelectArgs {
     int32_t *kept_idx;
     int64_t kept_stride;
     int32_t *n_kept;
+    int32_t *step_units;              /* gets units_all, the units of the whole step, for the counts' read-back; or NULL */
+    int32_t units_all;
     int32_t *status;                  /* ST_BOUNDS of the checked build */
     int32_t n_rows[TRIA_MAX_UNITS];
     int32_t keep_req[TRIA_MAX_UNITS];
@@ -1835,6 +1837,7 @@ __global__ void __launch_bounds__(SMK ? SELECT_BLOCK_SM : SELECT_BLOCK, SMK ? 1 
     __shared__ float2 s_zs[TRIA_MAX_GQA];           /* (mean, std) of the unit's query heads */
     extern __shared__ __align__(16) uint32_t s_keys[];
     const int u = blockIdx.x;
+    if (a.step_units && blockIdx.x == 0 && threadIdx.x == 0) *a.step_units = a.units_all;
     if (FUSED && (int)threadIdx.x < a.G) s_zs[threadIdx.x] = a.ms[(int64_t)u * a.G + threadIdx.x];
     select_unit<FUSED, SMK>(a, u, SMK ? s_keys : a.keys + (int64_t)u * a.key_stride,
                        SMK ? (int64_t)(dynamic_smem_bytes() / 4) : a.key_stride, s_zs, s_hist, s_warp, s_bc);
@@ -1891,6 +1894,7 @@ __global__ void __launch_bounds__(SELECT_BLOCK_SM, 1) k_select_cl(const SelectAr
     const int ncl = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int tid = threadIdx.x, bd = blockDim.x;
     const int u = blockIdx.x / ncl;
+    if (a.step_units && blockIdx.x == 0 && tid == 0) *a.step_units = a.units_all;
     const bool prot_on = a.window > 0 || a.sink > 0;
     int n = a.n_rows[u];
     if (!bounds_ok(select_rows_ok(a, n, (int64_t)ncl * (dynamic_smem_bytes() / 4), FUSED, prot_on) &&

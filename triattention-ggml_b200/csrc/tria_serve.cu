@@ -261,7 +261,7 @@ static int do_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view 
     std::vector<int32_t> keep;
     keep_requests(c, s, n_rows, p, keep);
     int32_t *cnt = n_kept_out ? n_kept_out : c->cnt;
-    if ((rc = launch_select(c, s, n_rows, keep, p, false, mass, c->kept, c->cell_stride, cnt, st))) return rc;
+    if ((rc = launch_select(c, s, n_rows, keep, p, false, mass, c->kept, c->cell_stride, cnt, st, units))) return rc;
     int64_t hint = 0;
     for (int32_t k : keep) hint = std::max<int64_t>(hint, k);
     if (p->window > 0 || p->sink > 0) hint += (int64_t)std::max(0, p->window) + std::max(0, p->sink) + 1;
@@ -278,12 +278,7 @@ static int do_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view 
         }
     }
     c->have_timing = false;
-    CUDA_TRY(cudaMemcpyAsync(c->h_pinned, c->d_status, 4, cudaMemcpyDeviceToHost, st));
-    CUDA_TRY(cudaMemcpyAsync(c->h_pinned + 1, cnt, (size_t)units * 4, cudaMemcpyDeviceToHost, st));
-    CUDA_TRY(record_done(c->ev_done, st));
-    c->last_units = (int32_t)units;
-    c->have_step = true;
-    return TRIA_OK;
+    return read_back_step(c, cnt, units, st);
 }
 
 /* ------------------------------------------------------------------ */
