@@ -470,7 +470,9 @@ struct tria_attend_params {
 };
 
 /* q, out: device f16 [n_layer][n_tok][n_head_kv*gqa][head_dim] by the strides
- * of `p`, 16-byte aligned; they must not overlap.  lse: device fp32 [n_layer]
+ * of `p`, 16-byte aligned; they must not overlap (both may lie in one buffer,
+ * at the same strides), and each stride of out must step over all that the
+ * smaller ones span.  lse: device fp32 [n_layer]
  * [n_tok][n_head_kv*gqa], the natural log of the softmax's denominator, or
  * NULL.  mass_out: device fp32 [n_layer][n_head_kv][n_cells], or NULL; row j
  * of a unit gets mass_decay * mass_in[j] + the sum of its weights over the

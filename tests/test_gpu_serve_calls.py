@@ -99,3 +99,50 @@ def test_a_larger_step_captured_first(torch_dev, tmp_path):
     del g
     ctx.close()
     tria_b200.free(st)
+
+
+def strided(b, *strides, at=0, shape=(2, 3, 8, 128)):
+    return torch.as_strided(b, shape, strides + (1,), at)
+
+
+@pytest.mark.parametrize("kv,heads", [(2, 8), (1, 4)])
+def test_outputs_that_overlap_are_refused(contexts, torch_dev, kv, heads):
+    """Strides below a row, below what the smaller ones span, and 0, for several
+    kv heads and for one with several query heads; q and out that share bytes."""
+    c = Cache(F16, 2, kv, 128, 100, [90, 80, 70, 60][:2 * kv], torch_dev)
+    ctx, q = contexts(kv, 4, 128), queries(2, 3, heads, 128, torch_dev)
+    b = torch.zeros(1 << 16, dtype=torch.float16, device=torch_dev)
+    shape = (2, 3, heads, 128)
+    p = tria_b200.attend_params(0.1)
+    w = heads * 128
+    for o in ((3 * w, w, 0), (3 * w, w, 8), (3 * w, w, 120), (3 * w, w - 8, 128), (3 * w - 8, w, 128), (0, w, 128), (3 * w, 0, 128),
+              (3 * w, 128, 3 * 128 - 8), (2 * 128 - 8, 2 * w, 128 * 2)):
+        with pytest.raises(tria_b200.TriaError, match="overlap"):
+            ctx.attend(c.view(), c.rows, q, strided(b, *o, shape=shape), p)
+    # one buffer: the same rows, rows half on one another, the last row on the first, another order over the same bytes
+    qb = strided(b, 3 * w, w, 128, at=4096, shape=shape)
+    for o, at in (((3 * w, w, 128), 4096), ((3 * w, w, 128), 4096 + 64), ((3 * w, w, 128), 4096 - 64), ((3 * w, w, 128), 4096 + 128),
+                  ((3 * w, w, 128), 4096 + 6 * w - 8), ((3 * w, 128, 3 * 128), 4096), ((3 * w, w, 128), 4096 - 6 * w + 8 if kv == 1 else 4104)):
+        with pytest.raises(tria_b200.TriaError, match="overlap"):
+            ctx.attend(c.view(), c.rows, qb, strided(b, *o, at=at, shape=shape), p)
+
+
+def test_queries_and_outputs_in_one_buffer(contexts, torch_dev):
+    """Interleaved head by head, token by token, behind one another, and with one
+    cache's outputs before the next one's queries."""
+    c = Cache(F16, 2, 2, 128, 300, [290, 222, 150, 151], torch_dev)
+    ctx, q = contexts(2, 4, 128), queries(2, 3, 8, 128, torch_dev)
+    want = attend_oracle(c, q, 128 ** -0.5)
+    p = tria_b200.attend_params(128 ** -0.5)
+    w, s = 8 * 128, torch.cuda.current_stream()
+    for strides, q_at, o_at in (((6 * w, 2 * w, 256), 0, 128), ((6 * w, 2 * w, 128), w, 0), ((3 * w, w, 128), 0, 6 * w),
+                                ((3 * w, w, 128), 6 * w, 0), ((6 * w, w, 128), 3 * w, 0), ((2 * 128, 3 * 512, 512), 0, 128)):
+        if strides[0] == 256:
+            strides = (256, 8 * 512, 512)                 # caches innermost, q and out side by side in each
+        b = torch.full((1 << 15,), 9.0, dtype=torch.float16, device=torch_dev)
+        qv, ov = strided(b, *strides, at=q_at), strided(b, *strides, at=o_at)
+        qv.copy_(q)
+        ctx.attend(c.view(), c.rows, qv, ov, p, stream=s)
+        ctx.check(s)
+        assert torch.equal(qv, q)
+        attend_close(c, ov, None, None, want)

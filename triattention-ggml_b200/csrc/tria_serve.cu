@@ -285,6 +285,60 @@ static int do_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view 
 /* Attention                                                            */
 /* ------------------------------------------------------------------ */
 
+/* Rows of `width` elements at the strides of up to three dimensions. */
+struct RowGrid {
+    using wide = __int128;               /* strides are the caller's: nothing here may overflow */
+    struct Dim { int64_t extent, stride; } dim[3];
+    int n = 0;
+    int64_t width;
+    explicit RowGrid(int64_t w) : width(w) {}
+    /* Dimensions of one entry have no stride; the others are kept by ascending stride. */
+    RowGrid &add(int64_t extent, int64_t stride) {
+        if (extent <= 1) return *this;
+        int i = n++;
+        for (; i > 0 && dim[i - 1].stride > stride; i--) dim[i] = dim[i - 1];
+        dim[i] = {extent, stride};
+        return *this;
+    }
+    /* Elements from the first row's start to the last row's end over the first k dimensions. */
+    wide span(int k) const {
+        wide s = width;
+        for (int i = 0; i < k; i++) s += (wide)(dim[i].extent - 1) * dim[i].stride;
+        return s;
+    }
+    /* Whether each stride steps over all that the smaller ones span. */
+    bool nested() const {
+        for (int i = 0; i < n; i++)
+            if (dim[i].stride < span(i)) return false;
+        return true;
+    }
+    bool same_strides(const RowGrid &o) const {
+        if (n != o.n || width != o.width) return false;
+        for (int i = 0; i < n; i++)
+            if (dim[i].extent != o.dim[i].extent || dim[i].stride != o.dim[i].stride) return false;
+        return true;
+    }
+    /* Whether a row of this nested grid and one of its copy `delta` elements on share one: of each dimension only the
+     * two steps around delta come near enough. */
+    bool meets_copy(wide delta, int k) const {
+        if (delta >= span(k) || -delta >= span(k)) return false;
+        if (k == 0) return true;
+        const Dim &d = dim[k - 1];
+        wide at = delta / d.stride;
+        if (delta % d.stride && delta < 0) at--;
+        for (int i = 0; i < 2; i++, at++)
+            if (at > -d.extent && at < d.extent && meets_copy(delta - at * d.stride, k - 1)) return true;
+        return false;
+    }
+};
+
+/* Whether f16 rows of q and out share elements.  Grids of different strides whose ranges overlap are taken to. */
+static bool grids_meet(const RowGrid &q, const void *qp, const RowGrid &o, const void *op) {
+    const RowGrid::wide delta = ((int64_t)(uintptr_t)op - (int64_t)(uintptr_t)qp) / 2;
+    if (delta >= q.span(q.n) || -delta >= o.span(o.n)) return false;
+    return !q.same_strides(o) || o.meets_copy(delta, o.n);
+}
+
 /* Grows tria_attend's workspace to `need` bytes. */
 static int ensure_attend(tria_ctx *c, size_t need, cudaStream_t st) {
     const int cap = note_capture(c, st);
@@ -485,8 +539,6 @@ static int do_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
                               p->o_cache_stride, p->o_tok_stride, p->o_head_stride};
         for (int64_t x : s)
             if (x < 0 || x % 8) FAIL(TRIA_ERR_INVALID, "%s: q and out strides must be multiples of 8 elements, not negative", fn);
-        if ((v->n_layer > 1 && !p->o_cache_stride) || (T > 1 && !p->o_tok_stride) || (KV > 1 && !p->o_head_stride))
-            FAIL(TRIA_ERR_INVALID, "%s: an out stride of 0 lets outputs overlap", fn);
         if (p->slopes && ((uintptr_t)p->slopes & 3)) FAIL(TRIA_ERR_INVALID, "%s: slopes misaligned", fn);
         if (p->window > 0 || p->slopes) {
             if ((rc = check_ints(fn, "tok_pos", p->tok_pos))) return rc;
@@ -497,11 +549,21 @@ static int do_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
             if (p->tree_words < (T + 31) / 32 || p->tree_stride < 0)
                 FAIL(TRIA_ERR_INVALID, "%s: tree_words %d < %d, or a negative tree_stride", fn, p->tree_words, (T + 31) / 32);
         }
+        /* the least rows that any context has; its own follow below */
+        if (!RowGrid(64).add(v->n_layer, p->o_cache_stride).add(T, p->o_tok_stride).add(KV, p->o_head_stride).nested())
+            FAIL(TRIA_ERR_INVALID, "%s: out strides let outputs overlap", fn);
     }
     if ((rc = check_ctx(c, fn))) return rc;
     const int H = KV * (int)c->G;
     if ((int64_t)v->n_layer * H * T > INT32_MAX / 2)
         FAIL(TRIA_ERR_UNSUPPORTED, "%s: %lld query rows in one call", fn, (long long)v->n_layer * H * T);
+    if (T > 0) {
+        RowGrid qg((int)c->hd), og((int)c->hd);
+        qg.add(v->n_layer, p->q_cache_stride).add(T, p->q_tok_stride).add(H, p->q_head_stride);
+        og.add(v->n_layer, p->o_cache_stride).add(T, p->o_tok_stride).add(H, p->o_head_stride);
+        if (!og.nested()) FAIL(TRIA_ERR_INVALID, "%s: out strides let outputs overlap", fn);
+        if (grids_meet(qg, q, og, out)) FAIL(TRIA_ERR_INVALID, "%s: out must not overlap q", fn);
+    }
     if (T == 0 && !mass_out) return TRIA_OK;
     DeviceGuard g(c->device);
     cudaStream_t st = (cudaStream_t)stream;
