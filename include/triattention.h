@@ -428,6 +428,8 @@ TRIA_API int tria_key_gather(const float *scores, int64_t score_stride, const in
  *   - A view lists caches of equal shape: the layers of one model, or one
  *     layer of several sequences.  layer0 and head0 are not looked at (no
  *     stats are read) except by tria_evict_mass, whose budget is per layer.
+ *   - No two rows of a view that a call writes share memory: strides that let
+ *     rows overlap, and a view that lists one cache twice, are refused.
  *   - Keys are stored as attention reads them: the view needs
  *     TRIA_VIEW_POST_ROPE.  Rows are f16 or q8_0, head_dim 64 or 128.
  *   - Row order matters: a call's n_tok tokens are the last n_tok rows of each

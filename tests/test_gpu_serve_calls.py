@@ -146,3 +146,41 @@ def test_queries_and_outputs_in_one_buffer(contexts, torch_dev):
         ctx.check(s)
         assert torch.equal(qv, q)
         attend_close(c, ov, None, None, want)
+
+
+def calls_that_write(ctx, c, view, dev):
+    """append, accept and (into `view`) evict_mass, as callables."""
+    x = torch.zeros((c.L, 1, c.KV, c.hd), dtype=torch.float16, device=dev)
+    one = torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    d = Cache(c.type, c.L, c.KV, c.hd, c.cells, c.rows_host, dev)
+    mass = torch.zeros((c.L, c.KV, c.cells), device=dev)
+    return [lambda: ctx.append(view, c.rows, x, x, torch.zeros(1, dtype=torch.int32, device=dev)),
+            lambda: ctx.accept(view, c.rows, 1, one, one[0]),
+            lambda: ctx.evict_mass(d.view(), view, c.rows_host.reshape(-1), mass, None, tria_b200.EvictParams(9, 4, 100, 0, 0, 0))]
+
+
+@pytest.mark.parametrize("type_id,hd", [(F16, 128), (Q8_0, 128), (F16, 64)])
+def test_views_that_writing_calls_refuse(contexts, torch_dev, type_id, hd):
+    """Rows of this context's head_dim that overlap, and one cache listed twice."""
+    ctx = contexts(2, 4, hd, layers=2)
+    c = Cache(type_id, 2, 2, hd, 40, [9, 8, 7, 6], torch_dev)
+    k, v, rb = [c.k[0], c.k[1]], [c.v[0], c.v[1]], c.rb
+    k0, v0 = c.k.clone(), c.v.clone()
+
+    def view(k, v, cell, head):
+        return tria_b200.make_view(type_id, k, v, c.pos, 40, cell, head, 2, flags=tria_b200.VIEW_POST_ROPE)
+
+    for cell, head, word in ((2 * rb, rb - 4, "rows of"), (2 * rb - 4, rb, "rows of"), (rb - 4, 20 * rb, "rows of"),
+                             (rb, 40 * rb - 4, "rows of")):
+        for call in calls_that_write(ctx, c, view(k, v, cell, head), torch_dev):
+            with pytest.raises(tria_b200.TriaError, match=word):
+                call()
+    for kk, vv in (([k[0], k[0]], v), (k, [v[1], v[1]]), (k, [v[0], k[0]]), ([v[1], k[1]], v)):
+        for call in calls_that_write(ctx, c, view(kk, vv, 2 * rb, rb), torch_dev):
+            with pytest.raises(tria_b200.TriaError, match="twice"):
+                call()
+    m = torch.zeros((2, 2, 40), device=torch_dev)
+    with pytest.raises(tria_b200.TriaError, match="different caches"):
+        ctx.evict_mass(c.view(), c.view(), c.rows_host.reshape(-1), m, None, tria_b200.EvictParams(9, 4, 100, 0, 0, 0))
+    torch.cuda.synchronize()
+    assert torch.equal(c.k, k0) and torch.equal(c.v, v0) and c.rows.tolist() == [[9, 8], [7, 6]]

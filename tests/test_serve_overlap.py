@@ -23,3 +23,26 @@ def test_out_strides(L, kw):
 ])
 def test_out_strides_that_keep_rows_apart(L, kw):
     refused(attend(L, **kw), "null context")
+
+
+@pytest.mark.parametrize("call", [append, accept])
+@pytest.mark.parametrize("kw,bad", [
+    (dict(head=0), True), (dict(head=64), True), (dict(cell=64), True), (dict(cell=128, head=64), True),
+    (dict(cell=192, head=128), True),                      # cells shorter than their two heads
+    (dict(cell=128, head=63 * 128), True),                 # head-major, the last row on the next head
+    (dict(cell=128, head=64 * 128 - 4), True), (dict(cell=512, head=3 * 512 - 64), True),
+    (dict(cell=2 ** 62, head=2 ** 62), True),              # a head on the next cell, past 63 bits
+    (dict(cell=256, head=128), False), (dict(cell=128, head=64 * 128), False), (dict(cell=260, head=132), False),
+    (dict(cell=384, head=256), False),                     # between the cells of the first head
+    (dict(cell=512, head=3 * 512 + 128), False),           # and some cells on
+    (dict(kv=1, head=0), False), (dict(n_cells=1, cell=4, head=128), False), (dict(n_cells=0, head=0), False),
+    (dict(type_id=8, cell=136, head=68), False), (dict(type_id=8, cell=136, head=64), True),
+    (dict(type_id=8, cell=132, head=68), True), (dict(type_id=8, kv=8, cell=8 * 68, head=68), False),
+    (dict(type_id=8, kv=8, cell=7 * 68, head=68), True),
+])
+def test_views_whose_rows_overlap(L, call, kw, bad):
+    refused(call(L, v=view(**kw)), "rows of" if bad else "null context")
+
+
+def test_views_that_are_only_read_may_overlap(L):
+    refused(attend(L, v=view(head=0)), "null context")     # one kv head for all

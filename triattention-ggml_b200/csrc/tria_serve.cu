@@ -52,6 +52,53 @@ static int validate_cache(const tria_kv_view *v, const char *what) {
     return TRIA_OK;
 }
 
+/* Whether rows of `rb` bytes of one cache of a view share bytes.  Heads may lie
+ * within cells, cells within heads, or neither: for each distance of heads the
+ * two cells around it are the ones that come near enough. */
+static bool rows_overlap(const tria_kv_view *v, int64_t rb) {
+    using wide = __int128;               /* strides are the caller's: nothing here may overflow */
+    if (v->cell_stride >= rb && v->head_stride >= rb &&
+        (v->cell_stride >= (wide)(v->n_head_kv - 1) * v->head_stride + rb || v->head_stride >= (wide)(v->n_cells - 1) * v->cell_stride + rb))
+        return false;                    /* one within the other */
+    if (v->n_cells > 1 && v->cell_stride < rb) return true;
+    for (int dh = 1; v->n_cells > 0 && dh < v->n_head_kv; dh++) {
+        const wide off = (wide)dh * v->head_stride;
+        const wide at = std::min<wide>(off / v->cell_stride, v->n_cells - 1);
+        const wide rest = off - at * v->cell_stride;         /* to the cell before, >= 0 */
+        if (rest < rb) return true;
+        if (at + 1 < v->n_cells && v->cell_stride - rest < rb) return true;
+    }
+    return false;
+}
+
+/* What a call writes to: no row twice (without a context, rows of the smallest head_dim). */
+static int check_written(const tria_kv_view *v, const char *what, const tria_ctx *c) {
+    if (rows_overlap(v, view_row_bytes(v->type, c ? (int)c->hd : 64)))
+        FAIL(TRIA_ERR_INVALID, "%s: the view's strides let rows of %d kv heads overlap", what, v->n_head_kv);
+    return TRIA_OK;
+}
+
+/* Caches of a view that is written: each k and v is memory of its own. */
+static int check_apart(const tria_kv_view *v, const char *what) {
+    const int L = v->n_layer;
+    auto addr = [](const void *p) { return (uintptr_t)p; };
+    /* K and V each by rising address, one behind the other: nothing to sort */
+    bool rising = !v->v || addr(v->k[L - 1]) < addr(v->v[0]) || addr(v->v[L - 1]) < addr(v->k[0]);
+    for (int l = 1; rising && l < L; l++)
+        rising = addr(v->k[l - 1]) < addr(v->k[l]) && (!v->v || addr(v->v[l - 1]) < addr(v->v[l]));
+    if (rising) return TRIA_OK;
+    std::vector<uintptr_t> at;
+    at.reserve(2 * (size_t)L);
+    for (int l = 0; l < L; l++) {
+        at.push_back(addr(v->k[l]));
+        if (v->v) at.push_back(addr(v->v[l]));
+    }
+    std::sort(at.begin(), at.end());
+    if (std::adjacent_find(at.begin(), at.end()) != at.end())
+        FAIL(TRIA_ERR_INVALID, "%s: the view lists one cache twice", what);
+    return TRIA_OK;
+}
+
 /* The context's part of the checks, after all that needs none. */
 static int check_ctx(const tria_ctx *c, const char *what) {
     if (!c) FAIL(TRIA_ERR_INVALID, "%s: null context", what);
@@ -123,7 +170,7 @@ static int do_append(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
     const int units_all = v->n_layer * v->n_head_kv;
     bool alias = false;
     if ((rc = counts_alias(fn, n_rows, n_rows_out, units_all, &alias))) return rc;
-    if ((rc = check_ctx(c, fn))) return rc;
+    if ((rc = check_written(v, fn, c)) || (rc = check_ctx(c, fn)) || (rc = check_apart(v, fn))) return rc;
     DeviceGuard g(c->device);
     cudaStream_t st = (cudaStream_t)stream;
     if ((rc = note_capture(c, st)) < 0) return rc;
@@ -197,7 +244,7 @@ static int do_accept(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows, 
     if (mass && ((uintptr_t)mass & 3)) FAIL(TRIA_ERR_INVALID, "%s: mass misaligned", fn);
     bool alias = false;
     if ((rc = counts_alias(fn, n_rows, n_rows_out, (int64_t)v->n_layer * v->n_head_kv, &alias))) return rc;
-    if ((rc = check_ctx(c, fn))) return rc;
+    if ((rc = check_written(v, fn, c)) || (rc = check_ctx(c, fn)) || (rc = check_apart(v, fn))) return rc;
     DeviceGuard g(c->device);
     cudaStream_t st = (cudaStream_t)stream;
     if ((rc = note_capture(c, st)) < 0) return rc;
@@ -246,7 +293,12 @@ static int do_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view 
     int rc = validate_view(c, s, n_rows, "tria_evict_mass src", false);
     if (!rc) rc = validate_view(c, d, nullptr, "tria_evict_mass dst", false);
     if (!rc) rc = check_pair(s, d);
+    if (!rc) rc = check_written(d, "tria_evict_mass dst", c);
+    if (!rc) rc = check_apart(d, "tria_evict_mass dst");
     if (rc) return rc;
+    for (int l = 0; l < s->n_layer; l++)
+        if (s->k[l] == d->k[l] || (s->v && s->v[l] == d->v[l]))
+            FAIL(TRIA_ERR_INVALID, "%s: src and dst must be different caches", fn);
     const int KV = s->n_head_kv;
     const int64_t units = (int64_t)s->n_layer * KV;
     int max_rows = 0;
