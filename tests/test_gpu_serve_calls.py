@@ -184,3 +184,27 @@ def test_views_that_writing_calls_refuse(contexts, torch_dev, type_id, hd):
         ctx.evict_mass(c.view(), c.view(), c.rows_host.reshape(-1), m, None, tria_b200.EvictParams(9, 4, 100, 0, 0, 0))
     torch.cuda.synchronize()
     assert torch.equal(c.k, k0) and torch.equal(c.v, v0) and c.rows.tolist() == [[9, 8], [7, 6]]
+
+
+def test_evicted_masses_that_overlap_are_refused(contexts, torch_dev):
+    """mass and mass_dst of different lengths, sharing bytes at either end; side by side they are taken."""
+    ctx = contexts(2, 4, 128)
+    c, d = Cache(F16, 1, 2, 128, 64, [60, 50], torch_dev), Cache(F16, 1, 2, 128, 96, [60, 50], torch_dev)
+    b = torch.rand(1024, device=torch_dev)
+    prm = tria_b200.EvictParams(1000, 20, 100, 0, 0, 0)
+    n = c.rows_host.reshape(-1)
+
+    def call(m, md):
+        ctx.evict_mass(c.view(), d.view(), n, b[m:m + 128].view(1, 2, 64), b[md:md + 192].view(1, 2, 96), prm,
+                       stream=torch.cuda.current_stream())
+
+    for m, md in ((0, 127), (0, 1), (192, 1), (192, 300), (200, 150)):
+        with pytest.raises(tria_b200.TriaError, match="overlap"):
+            call(m, md)
+    for m, md in ((0, 128), (192, 0)):
+        mass = b[m:m + 128].clone().view(2, 64)
+        call(m, md)
+        assert ctx.get_n_kv(2)[1].tolist() == [20, 20]
+        for h in range(2):
+            idx = kept_oracle(mass[h].cpu().numpy(), c.pos[0, h].cpu().numpy(), int(n[h]), 20, 1000, 0, 0)
+            assert torch.equal(b[md:md + 192].view(2, 96)[h, :20], mass[h][torch.from_numpy(idx).to(torch_dev)])

@@ -46,3 +46,11 @@ def test_views_whose_rows_overlap(L, call, kw, bad):
 
 def test_views_that_are_only_read_may_overlap(L):
     refused(attend(L, v=view(head=0)), "null context")     # one kv head for all
+
+
+@pytest.mark.parametrize("off,bad", [(4, True), (1020, True), (1024, False), (-4, True), (-1020, True), (-1024, False), (0, False)])
+def test_masses_that_overlap_in_part(L, off, bad):
+    """Arrays of 2 x 2 x 64 masses: the same one, apart, or neither."""
+    refused(attend(L, mass_in=16 * FAKE, mass_out=16 * FAKE + off), "overlap in part" if bad else "null context")
+    if off:
+        refused(evict(L, mass=16 * FAKE, mass_dst=16 * FAKE + off), "overlap" if bad else "null context")

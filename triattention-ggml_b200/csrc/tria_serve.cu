@@ -112,10 +112,16 @@ static int check_ints(const char *what, const char *name, const void *p) {
     return TRIA_OK;
 }
 
+/* Whether arrays of na and nb four-byte entries share some. */
+static bool arrays_meet(const void *a, int64_t na, const void *b, int64_t nb) {
+    const __int128 d = (__int128)(uintptr_t)b - (__int128)(uintptr_t)a;
+    return d < (__int128)na * 4 && -d < (__int128)nb * 4;
+}
+static int64_t view_cells(const tria_kv_view *v) { return (int64_t)v->n_layer * v->n_head_kv * std::max(v->n_cells, 0); }
+
 /* Whether the counts are updated in place; arrays that overlap in part are refused. */
 static int counts_alias(const char *what, const int32_t *in, const int32_t *out, int64_t units, bool *alias) {
-    const uintptr_t r0 = (uintptr_t)in, r1 = (uintptr_t)out, len = (uintptr_t)units * 4;
-    *alias = r0 < r1 + len && r1 < r0 + len;
+    *alias = arrays_meet(in, units, out, units);
     if (*alias && in != out) FAIL(TRIA_ERR_INVALID, "%s: n_rows and n_rows_out overlap in part", what);
     return TRIA_OK;
 }
@@ -289,6 +295,8 @@ static int do_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view 
     if (p->cur_pos < 0) FAIL(TRIA_ERR_INVALID, "%s: cur_pos %d < 0", fn, p->cur_pos);
     if (((uintptr_t)mass & 3) || ((uintptr_t)mass_dst & 3)) FAIL(TRIA_ERR_INVALID, "%s: mass misaligned", fn);
     if (mass == mass_dst) FAIL(TRIA_ERR_INVALID, "%s: mass and mass_dst must be different arrays", fn);
+    if (s && d && mass_dst && arrays_meet(mass, view_cells(s), mass_dst, view_cells(d)))
+        FAIL(TRIA_ERR_INVALID, "%s: mass and mass_dst overlap", fn);
     if (!c) FAIL(TRIA_ERR_INVALID, "%s: null context", fn);
     int rc = validate_view(c, s, n_rows, "tria_evict_mass src", false);
     if (!rc) rc = validate_view(c, d, nullptr, "tria_evict_mass dst", false);
@@ -583,6 +591,8 @@ static int do_attend(tria_ctx *c, const tria_kv_view *v, const int32_t *n_rows,
     if (mass_in && !mass_out) FAIL(TRIA_ERR_INVALID, "%s: mass_in without mass_out", fn);
     if (((uintptr_t)mass_in & 3) || ((uintptr_t)mass_out & 3) || ((uintptr_t)lse & 3))
         FAIL(TRIA_ERR_INVALID, "%s: lse or mass misaligned", fn);
+    if (mass_in && mass_in != mass_out && arrays_meet(mass_in, view_cells(v), mass_out, view_cells(v)))
+        FAIL(TRIA_ERR_INVALID, "%s: mass_in and mass_out overlap in part", fn);
     if (T > 0) {
         if (!q || !out || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))
             FAIL(TRIA_ERR_INVALID, "%s: q or out null or not 16-byte aligned", fn);
