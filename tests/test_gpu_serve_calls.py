@@ -208,3 +208,35 @@ def test_evicted_masses_that_overlap_are_refused(contexts, torch_dev):
         for h in range(2):
             idx = kept_oracle(mass[h].cpu().numpy(), c.pos[0, h].cpu().numpy(), int(n[h]), 20, 1000, 0, 0)
             assert torch.equal(b[md:md + 192].view(2, 96)[h, :20], mass[h][torch.from_numpy(idx).to(torch_dev)])
+
+
+@pytest.mark.parametrize("type_id", [F16, Q8_0])
+@pytest.mark.parametrize("opt", ["plain", "all"])
+@pytest.mark.parametrize("T,G", [(4, 4), (1, 5), (3, 4)])
+def test_masses_whose_scores_are_not_kept(contexts, torch_dev, type_id, opt, T, G):
+    """Scores are kept for the masses up to 1 GiB: caches of 1.1 million cells,
+    a few hundred of them in use, would need more at 16 query rows a unit (and
+    with fewer query rows, more cells)."""
+    KV, L = 8, 2
+    cells = 1_100_000 * 16 // (T * G)
+    rows = [290, 17, 64, 203, 130, 299, 65, 128, 16, 33, 300, 256, 100, 4, 211, 48]
+    c = Cache(type_id, L, KV, 128, 300, rows, torch_dev, shared=True)
+    pos = torch.zeros(cells, dtype=torch.int32, device=torch_dev)
+    pos[:300] = c.pos
+    view = tria_b200.make_view(type_id, [c.k[0], c.k[1]], [c.v[0], c.v[1]], pos, cells, c.cell_stride, c.head_stride, KV,
+                               pos_shared=True, flags=tria_b200.VIEW_POST_ROPE)
+    q = queries(L, T, KV * G, 128, torch_dev)
+    o = dict(cap=20.0, window=300, sink=8, slopes=torch.linspace(0.001, 0.05, KV * G, device=torch_dev)) if opt == "all" else {}
+    tok = (torch.arange(T, device=torch_dev) * 2 + 590).int()
+    p = tria_b200.attend_params(128 ** -0.5, o.get("cap", 0.0), o.get("window", 0), o.get("sink", 0), o.get("slopes"), tok,
+                                mass_decay=0.5)
+    before = torch.rand((L, KV, cells), device=torch_dev)
+    mass = before.clone()
+    out, lse = torch.empty_like(q), torch.empty((L, T, KV * G), device=torch_dev)
+    ctx, s = contexts(KV, G, 128), torch.cuda.current_stream()
+    ctx.attend(view, c.rows, q, out, p, lse=lse, mass_in=mass, mass_out=mass, stream=s)
+    ctx.check(s)
+    want = attend_oracle(c, q, 128 ** -0.5, o.get("cap", 0.0), o.get("window", 0), o.get("sink", 0), o.get("slopes"), tok)
+    attend_close(c, out, lse, mass[:, :, :300].contiguous(), want, before[:, :, :300] * 0.5)
+    live = torch.arange(cells, device=torch_dev) < c.rows[..., None]
+    assert torch.equal(torch.where(live, before, mass), before)

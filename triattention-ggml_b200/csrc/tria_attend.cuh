@@ -1182,14 +1182,11 @@ __global__ void __launch_bounds__(MASS_THREADS) k_mass_tiles(const AttendArgs a)
             pk[1] = (int)word_at(st + 16 * S::KS + 4 * (r8 + 8));
         }
         float mass[2] = {0.0f, 0.0f};                           /* cache rows r8, r8 + 8 */
-        /* by order, token t sees row j only if j <= n - T + t: query rows before that see none of these 16 */
-        int q0 = 0;
-        if (!a.tree) q0 = max(0, row0 - (n - a.T)) * a.G / (8 * NT) * (8 * NT);
-        for (; q0 < R; q0 += 8 * NT) {
+        if (R > 0) {
             uint32_t qf[NT][HD / 16][2];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const int r = q0 + 8 * t + r8;
+                const int r = 8 * t + r8;
                 const bool in = r < R;
                 const __half *q = a.q + l * a.q_cache + (in ? (r / a.G) * a.q_tok + (h * a.G + r % a.G) * a.q_head : 0);
 #pragma unroll
@@ -1200,12 +1197,12 @@ __global__ void __launch_bounds__(MASS_THREADS) k_mass_tiles(const AttendArgs a)
             }
             float s[NT][4];
             few_qk<KT, HD, NT>(qf, st, lead, lane, s);
-            const bool all = row0 + 16 <= n - a.T && a.window <= 0 && q0 + 8 * NT <= R;
+            const bool all = row0 + 16 <= n - a.T && a.window <= 0 && R == 8 * NT;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const int r = q0 + 8 * t + 2 * c + e, tk = r / a.G;
+                    const int r = 8 * t + 2 * c + e, tk = r / a.G;
                     const bool in = r < R;
                     const float2 nm = in ? a.norm[(int64_t)u * R + r] : make_float2(0.0f, 0.0f);
                     const int tp = in && want_pos ? a.tok_pos[l * a.tok_pos_stride + tk] : 0;
