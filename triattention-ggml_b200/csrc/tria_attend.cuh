@@ -63,6 +63,16 @@ __device__ __forceinline__ int attend_rows(const AttendArgs &a, int u) {
     return n < 0 ? 0 : a.n_cells;
 }
 
+/* Checked build: a block's walk stands at step `at` of item `it`, whose rows
+ * are shared by blocks c0 .. c1; span as the plan left it. */
+__device__ __forceinline__ bool walk_ok(const AttendArgs &a, int items, int it, int64_t at, int64_t total, int2 span, int step) {
+    return bounds_ok(it >= 0 && it < items && at >= 0 && at < total && span.x >= 0 && span.y >= 0 && span.x <= a.n_cells &&
+                     span.y <= (a.n_cells + step - 1) / step * step && span.y % step == 0, a.status);
+}
+__device__ __forceinline__ bool share_ok(const AttendArgs &a, int c0, int c1, int b, int grid) {
+    return bounds_ok(c0 >= 0 && c0 <= b && b <= c1 && c1 < grid && grid <= (int)gridDim.x, a.status);
+}
+
 /* Whether token t of cache l sees row j of a unit with n rows; pos: the row's
  * position, lo: tok_pos[t] - window (both read only with a window). */
 __device__ __forceinline__ bool attend_sees(const AttendArgs &a, int l, int t, int j, int n, int pos, int64_t lo) {
@@ -70,6 +80,7 @@ __device__ __forceinline__ bool attend_sees(const AttendArgs &a, int l, int t, i
     const int own = j - (n - a.T);
     if (own >= 0) {
         if (a.tree) {
+            if (!bounds_ok(own < a.T && (own >> 5) < a.tree_words && t >= 0 && t < a.T, a.status)) return false;
             if (!(a.tree[l * a.tree_stride + (int64_t)t * a.tree_words + (own >> 5)] >> (own & 31) & 1u)) return false;
         } else if (own > t) {
             return false;
@@ -799,6 +810,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
         const int n = uniform(attend_rows(a, u));
         int2 span = a.span ? a.span[it] : make_int2(0, 0);
         span = make_int2(uniform(span.x), uniform(span.y));
+        if (!walk_ok(a, items, it, at, total, span, ATT_STEP)) break;
         const int head_steps = (min(span.x, n) + ATT_STEP - 1) / ATT_STEP;
         auto slice_row = [&](int i) { return (i < head_steps ? i * ATT_STEP : span.y + (i - head_steps) * ATT_STEP) + FEW_SLICE * w; };
         const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
@@ -916,6 +928,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
                         for (int e = 0; e < 2; e++) {
                             const int r = grp * ROWS + 8 * t + 2 * c + e;
                             if (r >= R) continue;
+                            if (!bounds_ok(row0 >= 0 && row0 + FEW_SLICE <= a.score_stride, a.status)) continue;
                             float *d = a.scores + ((int64_t)u * R + r) * a.score_stride + row0 + r8;
                             d[0] = s[t][e];
                             d[8] = s[t][e + 2];
@@ -999,6 +1012,8 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
         /* blocks that share the item: owner(s) = the block whose range holds step s */
         const int c0 = (int)(((base + 1) * grid - 1) / total), c1 = (int)((upto * grid - 1) / total);
         const int rows = min(ROWS, R - grp * ROWS);
+        if (!share_ok(a, c0, c1, b, grid) ||
+            !bounds_ok((int64_t)(c1 - c0 + 1) * rows * 8 <= (int64_t)dynamic_smem_bytes(), a.status)) break;
         constexpr int DPT = FEW_THREADS / HD;                 /* rows a pass covers */
         const int d = tid % HD, dr = tid / HD;
         bool last = true;
@@ -1140,6 +1155,7 @@ __global__ void __launch_bounds__(256) k_mass_scores(const AttendArgs a) {
         /* whole steps of the head were walked, and everything from the tail on */
         if (j >= span.y || j < (span.x + ATT_STEP - 1) / ATT_STEP * ATT_STEP) {
             for (int r = 0; r < R; r++) {
+                if (!bounds_ok(j < a.score_stride, a.status)) continue;
                 const float x = __ldcs(&a.scores[((int64_t)u * R + r) * a.score_stride + j]);
                 mass = fmaf(ex2(x - s_norm[r].x), s_norm[r].y, mass);
             }

@@ -260,15 +260,15 @@ __device__ __forceinline__ void tile_walk_start(TileWalk &w, const int32_t *step
     }
     w.it = lo;
 }
-__device__ __forceinline__ bool tile_walk_segment(TileWalk &w, const int32_t *steps) {
-    if (w.at >= w.end) return false;
+__device__ __forceinline__ bool tile_walk_segment(const AttendArgs &a, TileWalk &w, const int32_t *steps, int items, int64_t total) {
+    if (w.at >= w.end || !bounds_ok(w.at >= 0 && w.end <= total, a.status)) return false;
     while (steps[w.it] <= w.at) w.it++;
     w.it = uniform(w.it);
     const int base = uniform(w.it ? steps[w.it - 1] : 0), last = uniform(steps[w.it]);
     w.base = base;
     w.i0 = (int)(w.at - base);
     w.i1 = (int)(min(w.end, (int64_t)last) - base);
-    return true;
+    return walk_ok(a, items, w.it, w.at, total, a.span ? a.span[w.it] : make_int2(0, 0), TILE_STEP);
 }
 __device__ __forceinline__ void tile_walk_next(TileWalk &w) {
     w.at = w.base + w.i1;
@@ -285,6 +285,12 @@ __device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volati
         return false;
     }
     return true;
+}
+
+/* Notes a query row (of `all`) for k_attend_redo. */
+__device__ __forceinline__ void tile_redo(const AttendArgs &a, int row, int all) {
+    const int i = atomicAdd(a.redo, 1);
+    if (bounds_ok(i < all && row >= 0 && row < all, a.status)) a.redo[1 + i] = row;
 }
 
 /* A q8_0 block as nine words in registers (2-byte aligned in memory: a block
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             }
         };
         bool ok = true;
-        for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+        for (uint32_t seg = 0; ok && tile_walk_segment(a, wk, steps, items, total); seg++, tile_walk_next(wk)) {
             const int u = wk.it / a.groups, grp = wk.it - u * a.groups, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
             const int n = attend_rows(a, u);
             const int2 span = a.span ? a.span[wk.it] : make_int2(0, 0);
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                 atomicOr(a.status, ST_TIMEOUT);
             }
             bool ok = tmem == 0;
-            for (uint32_t seg = 0; ok && tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+            for (uint32_t seg = 0; ok && tile_walk_segment(a, wk, steps, items, total); seg++, tile_walk_next(wk)) {
                 const bool two = R - (wk.it % a.groups) * TILE_ROWS > TILE_Q;
                 const int N = wk.i1 - wk.i0;
                 if (!(ok = wait(&b_q_full, seg & 1) && wait(&b_k_full[ks], kp))) break;
@@ -670,7 +676,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             }
         }
 
-        for (uint32_t seg = 0; tile_walk_segment(wk, steps); seg++, tile_walk_next(wk)) {
+        for (uint32_t seg = 0; tile_walk_segment(a, wk, steps, items, total); seg++, tile_walk_next(wk)) {
             const int u = wk.it / a.groups, grp = wk.it - u * a.groups, l = u / a.n_head_kv, h = u - l * a.n_head_kv;
             const int n = attend_rows(a, u);
             const int rows = min(TILE_ROWS, R - grp * TILE_ROWS);
@@ -784,7 +790,9 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
             const float total_w = halves.x + halves.y;
             const int64_t base = wk.base;
             const int c0 = (int)(((base + 1) * grid - 1) / total), c1 = (int)(((int64_t)steps[wk.it] * grid - 1) / total);
-            if (c0 == c1) {
+            if (!share_ok(a, c0, c1, b, grid)) {
+                /* checked build: nothing is put out (the same for all threads) */
+            } else if (c0 == c1) {
                 const bool none = total_w == 0.0f;
                 const float inv = none ? 0.0f : 1.0f / total_w;
                 bool bad = false;
@@ -815,7 +823,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                     if (in) {
                         if (a.lse) a.lse[((int64_t)l * a.T + t) * a.n_head_kv * a.G + head] = none ? -INFINITY : (m - TILE_LIFT + log2f(total_w)) * LN2;
                         if (a.norm) a.norm[(int64_t)u * R + r] = none ? make_float2(0.0f, 0.0f) : make_float2(m - TILE_LIFT, inv);
-                        if (bad) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + r;
+                        if (bad) tile_redo(a, u * R + r, units * R);
                     }
                 }
             } else {
@@ -895,7 +903,7 @@ __global__ void __launch_bounds__(TileLayout<KT, HD>::THREADS, 1) k_attend_tile(
                                 dst[4 * part + e / 2] = make_uint4(pack_half2(acc[e].x, acc[e].y), pack_half2(acc[e].z, acc[e].w),
                                                                    pack_half2(acc[e + 1].x, acc[e + 1].y), pack_half2(acc[e + 1].z, acc[e + 1].w));
                         }
-                        if (fin != 0.0f) a.redo[1 + atomicAdd(a.redo, 1)] = u * R + rq;
+                        if (fin != 0.0f) tile_redo(a, u * R + rq, units * R);
                         if (a.lse) a.lse[((int64_t)l * a.T + tq) * a.n_head_kv * a.G + hq] = none ? -INFINITY : (mm - TILE_LIFT + log2f(ss)) * LN2;
                         if (a.norm) a.norm[(int64_t)u * R + rq] = none ? make_float2(0.0f, 0.0f) : make_float2(mm - TILE_LIFT, inv);
                     }
@@ -1174,11 +1182,14 @@ __global__ void __launch_bounds__(MASS_TILE_THREADS, 2) k_mass_tile(const __grid
 template <int KT, int HD>
 __global__ void __launch_bounds__(ROW_THREADS) k_attend_redo(const AttendArgs a) {
     __shared__ RowShared<HD> sm;
-    const int R = a.T * a.G, many = a.redo[0];
+    const int R = a.T * a.G, all = a.n_layer * a.n_head_kv * R;
+    int many = a.redo[0];
+    if (!bounds_ok(many >= 0 && many <= all, threadIdx.x == 0 ? a.status : nullptr)) many = 0;
     int last = -1;
     bool bad = false;
     for (int i = blockIdx.x; i < many; i += gridDim.x) {
         const int q = a.redo[1 + i], u = q / R, r = q - u * R;
+        if (!bounds_ok(q >= 0 && q < all, threadIdx.x == 0 ? a.status : nullptr)) continue;
         if (u != last) bad = result_in_doubt<KT, HD, true>(a, u);
         last = u;
         if (bad) attend_row<KT, HD>(a, u, r % a.G, r / a.G, sm);

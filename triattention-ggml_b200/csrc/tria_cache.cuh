@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_append(const AppendArgs a) {
                 __syncwarp();
                 for (int i = lane; i < RPW * WORDS; i += 32) {
                     const int rr = i / WORDS, ww = i - rr * WORDS;
-                    if (t0 + rr < a.n_tok)
+                    if (t0 + rr < a.n_tok && bounds_ok(n + t0 + rr < a.n_cells, a.status))
                         *reinterpret_cast<uint32_t *>((kv ? dv : dk) + (int64_t)(n + t0 + rr) * a.cell_stride + 4 * ww) =
                             *reinterpret_cast<const uint32_t *>(&s_row[w][rr][4 * ww]);
                 }
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_append(const AppendArgs a) {
         const int tid = blockIdx.y * APPEND_THREADS + threadIdx.x, nt = gridDim.y * APPEND_THREADS;
         const int64_t row0 = (int64_t)u * a.n_cells + n;
         for (int t = tid; t < a.n_tok; t += nt) {
+            if (!bounds_ok(n + t < a.n_cells, a.status)) continue;
             const int32_t p = a.tok_pos[l * a.tok_pos_stride + t];
             if (!a.pos_shared) a.pos[row0 + t] = p;
             else if (a.first && u == 0) a.pos[n + t] = p;
@@ -219,6 +220,7 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) k_accept(const AcceptArgs a) {
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 from[q] = i + q < m ? path[i + q] : i + q;
+                if (!bounds_ok(i + q >= m || (from[q] >= i + q && base + from[q] < a.n_cells), a.status)) from[q] = i + q;
                 if (from[q] != i + q) x[q] = *reinterpret_cast<const uint32_t *>(p + from[q] * stride);
             }
 #pragma unroll
@@ -236,11 +238,14 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) k_accept(const AcceptArgs a) {
  * grid-stride over its kept rows. */
 __global__ void __launch_bounds__(256) k_carry_mass(const float *mass, int64_t src_cells, float *out, int64_t dst_cells,
                                                     const int32_t *kept_idx, int64_t kept_stride,
-                                                    const int32_t *n_kept) {
+                                                    const int32_t *n_kept, int32_t *status) {
     const int64_t u = blockIdx.y;
-    const int nk = n_kept[u];
-    for (int j = blockIdx.x * 256 + threadIdx.x; j < nk; j += gridDim.x * 256)
-        out[u * dst_cells + j] = mass[u * src_cells + kept_idx[u * kept_stride + j]];
+    int nk = n_kept[u];
+    if (!bounds_ok(nk >= 0 && nk <= dst_cells && nk <= kept_stride, threadIdx.x == 0 ? status : nullptr)) nk = 0;
+    for (int j = blockIdx.x * 256 + threadIdx.x; j < nk; j += gridDim.x * 256) {
+        const int r = kept_idx[u * kept_stride + j];
+        if (bounds_ok(r >= j && r < src_cells, status)) out[u * dst_cells + j] = mass[u * src_cells + r];
+    }
 }
 
 }  // namespace tria

@@ -332,7 +332,7 @@ static int do_evict_mass(tria_ctx *c, const tria_kv_view *s, const tria_kv_view 
             const int nu = (int)std::min<int64_t>(TRIA_MAX_UNITS, units - u0);
             const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((hint + 1023) / 1024, 64)), (unsigned)nu);
             k_carry_mass<<<grid, 256, 0, st>>>(mass + u0 * s->n_cells, s->n_cells, mass_dst + u0 * d->n_cells, d->n_cells,
-                                               c->kept + u0 * c->cell_stride, c->cell_stride, cnt + u0);
+                                               c->kept + u0 * c->cell_stride, c->cell_stride, cnt + u0, c->d_status);
             CUDA_TRY(cudaGetLastError());
             c->launches++;
         }
