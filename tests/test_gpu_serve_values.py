@@ -139,3 +139,19 @@ def test_q8_0_blocks_beyond_f16(contexts, torch_dev, T, where):
                 b[34:36].view(torch.float16)[0] = 2000.0
     out, lse, mass = run_attend(contexts, c, G, T, q=q)
     assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("T", [1, 12, 40, 140])
+@pytest.mark.parametrize("d", [511.75, 512.0])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_q8_0_blocks_at_the_edge_of_f16(contexts, torch_dev, T, d, side):
+    """-128 (which other writers may store) times 511.75 is f16's largest number, times 512 past it."""
+    c = Cache(Q8_0, 1, 2, HD, 500, [470, 333], torch_dev)
+    q = queries(1, T, 2 * G, HD, torch_dev, sigma=0.6)
+    q[..., 0] = 2.0 ** -13
+    b = c.unit(getattr(c, side), 0, 1)[40]
+    b[:2].view(torch.float16)[0] = d
+    b[2:34] = 0
+    b[2] = 128
+    out, _, _ = run_attend(contexts, c, G, T, q=q)
+    assert torch.isfinite(out).all()

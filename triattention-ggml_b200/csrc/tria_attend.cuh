@@ -235,7 +235,7 @@ __device__ void attend_row(const AttendArgs &a, int u, int g, int t, RowShared<H
  * q8_0: if a block's scale is not finite (it leaves no finite remainder of a
  * weight) or, on the tiles, so large that its values pass f16's 65504 and their
  * remainders are lost.  For all threads of a block of ROW_THREADS. */
-constexpr float TILE_SCALE = 512.0f;     /* 127 times it is 65024 */
+constexpr float TILE_SCALE = 512.0f;     /* below it 128 times a scale is at most 65504 */
 template <int KT, int HD, bool TILE>
 __device__ bool result_in_doubt(const AttendArgs &a, int u) {
     const int l = u / a.n_head_kv, h = u - l * a.n_head_kv, n = attend_rows(a, u);
@@ -250,7 +250,7 @@ __device__ bool result_in_doubt(const AttendArgs &a, int u) {
         for (int64_t x = threadIdx.x; x < (int64_t)n * NB; x += ROW_THREADS) {
             const int64_t at = x / NB * a.cell_stride + x % NB * 34;
             const float dk = fabsf(half_at(k + at)), dv = fabsf(half_at(v + at));
-            bad |= TILE ? !(dk <= TILE_SCALE && dv <= TILE_SCALE) : !(dv < INFINITY);
+            bad |= TILE ? !(dk < TILE_SCALE && dv < TILE_SCALE) : !(dv < INFINITY);
         }
     }
     return __syncthreads_or(bad);
@@ -486,8 +486,9 @@ __host__ __device__ constexpr int few_smem() {
  * rows far below the maximum stay normal f16 numbers (2^-14 and up) down to
  * 2^-26 of it, and the maximum may fall FEW_SLACK behind before the sums are
  * rescaled: 2^(FEW_LIFT + FEW_SLACK) is still finite in f16.  (q8_0 weights take
- * no part in this: see few_pv.)  A sum rescaled is some 64 multiplications of a
- * warp: slack 3 and 8 measure the same. */
+ * no part in this: see few_pv.)  Sums rescaled sooner cost 32 multiplications a
+ * thread and 8 query rows: with slack 8, the same for one token (8 units of
+ * 65521 rows, 74 us) and 73 us instead of 75 for 32 query rows over 32000. */
 constexpr float FEW_LIFT = 12.0f, FEW_SLACK = 3.0f;
 /* Measured (blocks_used): 4000 rows, 12 query rows: 30 us at 0.05, 27 at 0.2, 23 at
  * 0.6; 500 rows: 16, 16 and 27 us. */

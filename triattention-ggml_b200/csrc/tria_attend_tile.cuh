@@ -943,11 +943,15 @@ struct MassTileLayout {
     static constexpr int BYTES = SUM + TILE_K * 4 + 1024;
 };
 
-/* The mass of row j of unit u, whose position is pj, by one thread. */
+/* The mass of q8_0 row j of unit u, whose position is pj, by one thread: where
+ * a block of the key passes f16's range, else it is NaN for another reason. */
 template <int KT, int HD>
 __device__ __noinline__ float row_mass(const AttendArgs &a, int u, int j, int n, int pj) {
     const int l = u / a.n_head_kv, h = u - l * a.n_head_kv;
     const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride + (int64_t)j * a.cell_stride;
+    bool past = false;
+    for (int b = 0; b < HD / 32; b++) past |= fabsf(half_at(k + 34 * b)) >= TILE_SCALE;
+    if (!past) return NAN;
     const ScoreMap map(a);
     float mass = 0.0f;
     for (int t = 0; t < a.T; t++) {
