@@ -442,7 +442,7 @@ constexpr int ATTEND_MAX_GRID = 1024;
  * them once, but start, join and convert q8_0 rows at a higher price.  Measured
  * with 8 units of head_dim 128 over 500 / 4000 / 32000 rows (us, groups against
  * tiles): f16 R = 32: 18 / 35 / 72 against 23 / 38 / 87, R = 64: 19 / 38 / 110
- * against 24 / 39 / 91; q8_0 R = 64: 19 / 39 / 116 against 27 / 51 / 144. */
+ * against 24 / 39 / 91; q8_0 R = 64: 20 / 40 / 120 against 28 / 50 / 143. */
 constexpr int TILE_FROM_F16 = 32, TILE_FROM_Q8_0 = 64;
 
 /* A call with masses and at most 16 query rows a unit keeps its scores (4 bytes
