@@ -481,9 +481,9 @@ struct tria_attend_params {
  * tokens and the query heads of its group (mass_in NULL: 0; it may be
  * mass_out), rows at and behind the unit's count are left as they were.
  * Scores, softmax statistics, sums and masses are held in fp32.  For the
- * product with the values a weight is rounded to f16 (2^-11 of itself, and
- * 2^-35 of the row's largest where it is that far below), or, with q8_0 rows
- * and few tokens, weight times block scale to 16 bits. */
+ * product with the values weights keep 16 bits or more up to 32 query rows a
+ * unit (n_tok times gqa; q8_0 64) and are rounded to f16 above (2^-11 of
+ * itself, and 2^-35 of the row's largest where a weight is that far below). */
 TRIA_API int tria_attend(tria_ctx *ctx, const struct tria_kv_view *kv, const int32_t *n_rows,
                          const struct tria_attend_params *p, const void *q, void *out, float *lse,
                          const float *mass_in, float *mass_out, void *stream);

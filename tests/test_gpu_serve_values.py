@@ -155,3 +155,22 @@ def test_q8_0_blocks_at_the_edge_of_f16(contexts, torch_dev, T, d, side):
     b[2] = 128
     out, _, _ = run_attend(contexts, c, G, T, q=q)
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("type_id,part", [(F16, 2.0 ** -20), (Q8_0, 2.0 ** -16)])
+@pytest.mark.parametrize("T", [1, 3, 8])
+@pytest.mark.parametrize("bits", [1, 3.3, 9.6])
+def test_few_tokens_keep_the_weights_bits(contexts, torch_dev, type_id, part, T, bits):
+    """Up to 32 query rows a unit the weights are not rounded to 11 bits: beyond
+    the result's own rounding (2^-11 of it) only the parts' and fp32's are left.
+    The rows that carry the value have one weight and positive values, so that
+    its rounding shows in full."""
+    c, q = raised(type_id, torch_dev, T, [390, 77], 1.0, bits, lambda j: j % 16 == 9, 0.0, alike=True)
+    out, s = torch.empty_like(q), torch.cuda.current_stream(torch_dev)
+    contexts(2, G, HD).attend(c.view(), c.rows, q, out, tria_b200.attend_params(SCALE), stream=s)
+    want, _, _, absum, serr = attend_oracle(c, q, SCALE)
+    # attend_close's terms with the weights' 2^-11 replaced by the parts'; the rows' scores share one error, and a
+    # factor on all of their weights, e^(2 serr) at most, is in rel
+    rel = part + 2 * torch.expm1(serr) + 2.0 ** -20 + 2 * (390 + 32) * 2.0 ** -24
+    tol = 2.0 ** -11 * want.abs() * (1 + 2.0 ** -9) + rel[..., None] * absum * (1 + 2.0 ** -9) + 2.0 ** -25
+    assert ((out.double() - want).abs() <= tol).all()

@@ -231,10 +231,11 @@ __device__ void attend_row(const AttendArgs &a, int u, int g, int t, RowShared<H
 
 
 /* Whether a result of unit u that is not finite can be wrong.  f16: if some
- * value that one token sees and another does not is not finite (0 times it).
- * q8_0: if a block's scale is not finite (it leaves no finite remainder of a
- * weight) or, on the tiles, so large that its values pass f16's 65504 and their
- * remainders are lost.  For all threads of a block of ROW_THREADS. */
+ * value that one token sees and another does not is not finite (0 times it), and
+ * where weights are two parts, if any value is not (one part may be 0 or
+ * negative).  q8_0: if a block's scale is not finite or, on the tiles, so large
+ * that its values pass f16's 65504 and their remainders are lost.  For all
+ * threads of a block of ROW_THREADS. */
 constexpr float TILE_SCALE = 512.0f;     /* below it 128 times a scale is at most 65504 */
 template <int KT, int HD, bool TILE>
 __device__ bool result_in_doubt(const AttendArgs &a, int u) {
@@ -242,7 +243,7 @@ __device__ bool result_in_doubt(const AttendArgs &a, int u) {
     const uint8_t *k = a.k[l] + (int64_t)h * a.head_stride, *v = a.v[l] + (int64_t)h * a.head_stride;
     bool bad = false;
     if constexpr (KT == KT_F16) {
-        const int from = a.window > 0 ? 0 : max(0, n - a.T);
+        const int from = !TILE || a.window > 0 ? 0 : max(0, n - a.T);
         for (int64_t x = threadIdx.x; x < (int64_t)(n - from) * HD; x += ROW_THREADS)
             bad |= !(fabsf(row_value<KT>(v + (from + x / HD) * a.cell_stride, (int)(x % HD))) < INFINITY);
     } else {
@@ -434,6 +435,12 @@ __device__ __forceinline__ void mma16816_bf16(float (&d)[4], const uint32_t (&a)
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+/* x and y as f16 pairs, rounded (hi) and what the rounding left (lo). */
+__device__ __forceinline__ void split_half(float x, float y, uint32_t &hi, uint32_t &lo) {
+    hi = pack_half2(x, y);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    lo = pack_half2(x - f.x, y - f.y);
+}
 /* x and y as bf16 pairs, rounded (hi) and what the rounding left (lo): 16 bits
  * of each over fp32's range. */
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -621,27 +628,33 @@ __device__ __forceinline__ void few_qk(const uint32_t (&qf)[NT][HD / 16][2], con
     }
 }
 
-/* o += v^T p over the slice's 16 rows.  FULL: every query row sees them all.
+/* o += v^T p over the slice's 16 rows, the weights in two parts (rounded value
+ * and remainder), for which the tensor pipe has room.  FULL: every query row sees them all.
  * Otherwise a weight of 0 meets 0: keep0, keep1 (f16) have the bits of a V pair
  * whose row some query row sees, and a q8_0 scale only enters where p is not 0
  * (a row that is not seen may hold NaN).
  *
+ * f16: one token over 8 units of 65521 rows takes 75 us with two parts and 74
+ * with one, whose rounding (2^-11 of each weight) showed in the results.
+ *
  * q8_0: the V operands are the stored integers, so the scales go into the
  * weights: products whose size follows the values', not the weights' alone,
- * and for which f16 has no range.  bf16 has it, and two of them (the rounded
- * product and its remainder) keep 16 bits; the tensor pipe has room (128 units
- * of 8197 to 32768 rows: 236 us, with one f16 operand 242). */
+ * and for which f16 has no range.  bf16 has it, and its two parts keep 16 bits
+ * (128 units of 8197 to 32768 rows: 236 us, with one f16 operand 242). */
 template <int KT, int HD, int NT, bool FULL>
 __device__ __forceinline__ void few_pv(const float (&p)[NT][4], const uint8_t *st, int lead, int lane, uint32_t keep0, uint32_t keep1,
                                        float (&o)[NT][HD / 16][4]) {
     constexpr int VS = FewStage<KT, HD>::VS;
     if constexpr (KT == KT_F16) {
-        uint32_t pf[NT][2];
+        uint32_t h[NT][2], r[NT][2];                           /* weights rounded, and what the rounding left */
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            pf[t][0] = transpose8(pack_half2(p[t][0], p[t][1]));
-            pf[t][1] = transpose8(pack_half2(p[t][2], p[t][3]));
-        }
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                split_half(p[t][2 * i], p[t][2 * i + 1], h[t][i], r[t][i]);
+                h[t][i] = transpose8(h[t][i]);
+                r[t][i] = transpose8(r[t][i]);
+            }
         const int row = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
         const uint32_t at = smem_u32(st) + row * VS;
 #pragma unroll
@@ -655,7 +668,10 @@ __device__ __forceinline__ void few_pv(const float (&p)[NT][4], const uint8_t *s
                 v[3] &= keep1;
             }
 #pragma unroll
-            for (int t = 0; t < NT; t++) mma16816(o[t][j], v, pf[t][0], pf[t][1]);
+            for (int t = 0; t < NT; t++) {
+                mma16816(o[t][j], v, h[t][0], h[t][1]);
+                mma16816(o[t][j], v, r[t][0], r[t][1]);
+            }
         }
     } else {
         const int r8 = lane >> 2, c = lane & 3;
@@ -1128,7 +1144,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_blocks<KT, NT>()) k_attend_fe
             int any = 0;
             __syncthreads();
             for (int r = tid; r < rows; r += FEW_THREADS) any |= s_redo[r];
-            if ((a.T > 1 || KT == KT_Q8_0) && __syncthreads_or(any) && result_in_doubt<KT, HD, false>(a, u)) {
+            if (__syncthreads_or(any) && result_in_doubt<KT, HD, false>(a, u)) {
                 for (int r = 0; r < rows; r++)
                     if (s_redo[r]) attend_row<KT, HD>(a, u, (grp * ROWS + r) % a.G, (grp * ROWS + r) / a.G, s_row);
             }
