@@ -751,7 +751,7 @@ __device__ __forceinline__ float merge_row(int S, Ml &&ml, O &&o, float &m, floa
  * EXTRA: the call caps, biases or windows its scores.
  *
  * Bound by memory: 8 units of 65521 f16 rows (268 MB), 4 query rows each, take
- * 62 us (4.3 TB/s; 42 at copy rate) with start and join 12 of them; 128 units of
+ * 64 us (4.2 TB/s; 42 at copy rate) with start and join 12 of them; 128 units of
  * 8197 to 32768 q8_0 rows (710 MB) take 236 us a call, because a 136-byte row
  * costs the 64-byte pieces that it touches.  Three blocks an SM: f16 stages of
  * 8 KB fill shared memory, and q8_0 bytes need registers (that case in 279 us

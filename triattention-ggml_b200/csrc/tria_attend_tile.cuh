@@ -428,7 +428,7 @@ __device__ __forceinline__ void tile_load_q(const AttendArgs &a, int l, int h, i
  * nearly those of 128).
  *
  * 8 units of 8192 f16 rows, 2048 tokens of 4 heads each, head_dim 128: 255 us
- * with the rows in L2 (945 TFLOP/s, tensor pipe 42 % active), 293 us from DRAM;
+ * with the rows in L2 (945 TFLOP/s), 295 us from DRAM (tensor pipe 42 % active);
  * 32768 rows: 1047 TFLOP/s.  Without the
  * weights a step of 128 cache rows takes 1.5 us, near cuBLAS's
  * rate, with them 2.4: bound by the chain scores - weights - values of a row
