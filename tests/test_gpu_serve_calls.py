@@ -1,6 +1,5 @@
 """GPU tests of how the serving calls may be made: steps of other sizes between
 a capture and its replay, and views, strides and arrays that the calls refuse."""
-import ctypes as C
 
 import numpy as np
 import pytest
